@@ -1,0 +1,412 @@
+"""Cases of the operators around the 4-bit KV cache: page planning, rotary
+positions, rotary with quantize-on-write, reading tokens back, and causal
+attention of packed prompts.
+
+``listed()`` names the cases, ``draw(rng)`` gives further ones of the same
+ranges, ``prepare(case, seed)`` makes a case's inputs on the GPU and
+``run(state)`` is one pass: elementary torch operations in 32 bits (angles in
+64) where ``own`` is false, the library's entry points where it is true.
+``exact(case, seed)`` computes the same outputs in 64 bits from the
+definitions.
+"""
+import math
+import random
+
+import numpy as np
+import torch
+
+own = False
+
+DEVICE = "cuda"
+BLOCK = 16  # tokens per page
+DTYPES = {"fp16": torch.float16, "bf16": torch.bfloat16}
+
+
+# ------------------------------------------------------------------- cases
+def listed():
+    return [
+        # the smallest serving step: a few one-token requests on the way
+        # through decode, some of them entering a new page
+        {"name": "plan_decode", "op": "plan", "requests": 256, "lo": 512, "hi": 4096, "new": 1, "pad": 0},
+        # a whole ragged batch of prompts placed at once (lengths of the
+        # ragged decode workload), with padded rows behind the last token
+        {"name": "plan_prompts", "op": "plan", "requests": 64, "lo": 128, "hi": 8192, "new": 0, "pad": 13},
+        # a prompt step of a 32/8-head model, full rotary, base 500000 at far positions
+        {"name": "rotary_prompt", "op": "rotary", "tokens": 8192, "hq": 32, "kv": 8, "d": 128, "rot": 128,
+         "interleaved": False, "base": 500000.0, "factor": 1.0, "first": 100000, "dtype": "bf16"},
+        # partial rotary of 32 of 80 dims, pairs next to one another, odd token count
+        {"name": "rotary_partial", "op": "rotary", "tokens": 777, "hq": 32, "kv": 32, "d": 80, "rot": 32,
+         "interleaved": True, "base": 10000.0, "factor": 1.25, "first": 0, "dtype": "fp16"},
+        # one decode step of a batch of 256 (TinyLlama heads)
+        {"name": "rotary_store_decode", "op": "rotary_store", "tokens": 256, "hq": 32, "kv": 4, "d": 64, "rot": 64,
+         "interleaved": False, "base": 10000.0, "factor": 1.0, "first": 4096, "dtype": "bf16"},
+        # a prompt step of 8192 tokens into the cache
+        {"name": "rotary_store_prompt", "op": "rotary_store", "tokens": 8192, "hq": 32, "kv": 8, "d": 128, "rot": 128,
+         "interleaved": False, "base": 500000.0, "factor": 1.0, "first": 0, "dtype": "bf16"},
+        # a short shared prefix read back out of the cache
+        {"name": "load_prefix", "op": "load", "tokens": 130, "kv": 4, "d": 64, "dtype": "bf16"},
+        # a long context read back whole
+        {"name": "load_long", "op": "load", "tokens": 131072, "kv": 8, "d": 128, "dtype": "fp16"},
+        # four short prompts, one of a single token
+        {"name": "prompt_small", "op": "prompt", "lens": "1,17,40,130", "hq": 32, "kv": 8, "d": 128, "dtype": "fp16"},
+        # a batch of chat turns of a 64-dim model, ragged
+        {"name": "prompt_ragged", "op": "prompt", "lens": ",".join(str(5 + (37 * i * i) % 389) for i in range(48)),
+         "hq": 32, "kv": 4, "d": 64, "dtype": "bf16"},
+        # one key head per query head, 80 dims, odd lengths
+        {"name": "prompt_d80", "op": "prompt", "lens": "1999,777,63", "hq": 32, "kv": 32, "d": 80, "dtype": "fp16"},
+        # one long prompt
+        {"name": "prompt_long", "op": "prompt", "lens": "16384", "hq": 32, "kv": 8, "d": 128, "dtype": "bf16"},
+    ]
+
+
+def _log_int(rng, lo, hi):
+    return min(hi, max(lo, int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))))
+
+
+def draw(rng: random.Random):
+    op = rng.choice(["plan", "rotary", "rotary_store", "load", "prompt", "prompt"])
+    if op == "plan":
+        r = _log_int(rng, 1, 512)
+        hi = _log_int(rng, 16, 8192)
+        return {"op": op, "requests": r, "lo": max(1, hi // rng.randint(1, 64)), "hi": hi, "new": rng.choice([0, 1, 1]),
+                "pad": rng.randint(0, 63)}
+    d = rng.choice([64, 80, 128])
+    hq, kv = rng.choice([(32, 8), (32, 4), (32, 32), (64, 8), (16, 1), (14, 2), (8, 8), (24, 8)])
+    dtype = rng.choice(["fp16", "bf16"])
+    if op in ("rotary", "rotary_store"):
+        return {"op": op, "tokens": _log_int(rng, 1, 8192), "hq": hq, "kv": kv, "d": d,
+                "rot": rng.choice([d, d, d // 2, 32, d - 10]), "interleaved": rng.random() < 0.4,
+                "base": rng.choice([10000.0, 500000.0, 1000000.0]), "factor": rng.choice([1.0, 1.0, 1.25]),
+                "first": _log_int(rng, 1, 131072), "dtype": dtype}
+    if op == "load":
+        return {"op": op, "tokens": _log_int(rng, 1, 65536), "kv": kv, "d": d, "dtype": dtype}
+    total = _log_int(rng, 1, 8192)  # tokens of the step, cut into requests at random
+    cuts = sorted(rng.randint(0, total) for _ in range(_log_int(rng, 1, 64) - 1))
+    lens = [b - a for a, b in zip([0] + cuts, cuts + [total])]
+    return {"op": op, "lens": ",".join(map(str, lens)), "hq": hq, "kv": kv, "d": d, "dtype": dtype}
+
+
+# ------------------------------------------------------------------ inputs
+def _lens(case):
+    return [int(x) for x in case["lens"].split(",")]
+
+
+def _inv_freq(rot, base):
+    return (1.0 / (base ** (torch.arange(0, rot, 2, dtype=torch.float64) / rot))).to(torch.float32)
+
+
+def _rows(g, n, h, d, dtype):
+    """Activations: normal values under a fixed spread between channels."""
+    spread = torch.exp(0.5 * torch.randn(h, d, device=DEVICE, generator=g))
+    return (torch.randn(n, h, d, device=DEVICE, generator=g) * spread).to(dtype)
+
+
+def _plan_host(case):
+    """The requests' lengths, a part of the case; the seed deals out the pages."""
+    r = case["requests"]
+    rng = random.Random(r)
+    seq = [rng.randint(case["lo"], case["hi"]) for _ in range(r)]
+    new = [case["new"] or n for n in seq]
+    return seq, new
+
+
+def prepare(case, seed):
+    g = torch.Generator(device=DEVICE).manual_seed(seed)
+    op = case["op"]
+    if op == "plan":
+        seq, new = _plan_host(case)
+        need = [-(-n // BLOCK) for n in seq]
+        have = [-(-(n - m) // BLOCK) for n, m in zip(seq, new)]
+        total = sum(need)
+        perm = torch.randperm(total + 7, generator=torch.Generator().manual_seed(seed)).to(torch.int32)
+        tables = torch.full((len(seq), max(need) + 2), -1, dtype=torch.int32)
+        at = 0
+        for i, n in enumerate(have):
+            tables[i, :n] = perm[at:at + n]
+            at += n
+        start = torch.zeros(len(seq) + 1, dtype=torch.int64)
+        start[1:] = torch.tensor(new).cumsum(0)
+        # the free list's cursor stands behind two blocks that others took
+        return {"op": op, "query_start_loc": start.to(torch.int32).to(DEVICE),
+                "seq_lens": torch.tensor(seq, dtype=torch.int32, device=DEVICE), "block_tables": tables.to(DEVICE),
+                "free_blocks": torch.cat([perm[:2], perm[at:]]).to(DEVICE),
+                "cursor": torch.tensor([2], dtype=torch.int32, device=DEVICE),
+                "num_tokens": int(start[-1]) + case["pad"]}
+    dtype = DTYPES[case["dtype"]]
+    d, kv = case["d"], case["kv"]
+    if op == "prompt":
+        lens = _lens(case)
+        n = sum(lens)
+        start = torch.tensor([0] + lens).cumsum(0)
+        return {"op": op, "q": _rows(g, n, case["hq"], d, dtype), "k": _rows(g, n, kv, d, dtype),
+                "v": _rows(g, n, kv, d, dtype), "query_start_loc": start.to(torch.int32).to(DEVICE),
+                "max_query_len": max(lens)}
+    n = case["tokens"]
+    blocks = -(-n // BLOCK) + 3
+    slots = torch.randperm(blocks, device=DEVICE, generator=g)[:-(-n // BLOCK)]
+    slots = (slots[:, None] * BLOCK + torch.arange(BLOCK, device=DEVICE)).reshape(-1)[:n].contiguous()
+    if op == "load":
+        cache = torch.randint(0, 256, (blocks, BLOCK, kv, d + 8), dtype=torch.uint8, device=DEVICE, generator=g)
+        lo = torch.randn(blocks, BLOCK, kv, 2, device=DEVICE, generator=g) - 3.0
+        step = 0.1 + torch.rand(blocks, BLOCK, kv, 2, device=DEVICE, generator=g)
+        cache[..., d:] = torch.stack([lo, step], dim=-1).to(torch.float16).reshape(blocks, BLOCK, kv, 4).view(torch.uint8)
+        return {"op": op, "cache": cache, "slots": slots, "dtype": dtype}
+    state = {"op": op, "q": _rows(g, n, case["hq"], d, dtype), "k": _rows(g, n, kv, d, dtype),
+             "positions": case["first"] + torch.randperm(n, device=DEVICE, generator=g),
+             "inv_freq": _inv_freq(case["rot"], case["base"]).to(DEVICE), "interleaved": case["interleaved"],
+             "factor": case["factor"]}
+    if op == "rotary_store":
+        state["v"] = _rows(g, n, kv, d, dtype)
+        state["cache"] = torch.zeros(blocks, BLOCK, kv, d + 8, dtype=torch.uint8, device=DEVICE)
+        state["slots"] = slots
+    return state
+
+
+# ------------------------------------------------------------- plain forms
+def _plain_plan(s):
+    start, seq, tables = s["query_start_loc"].long(), s["seq_lens"].long(), s["block_tables"]
+    r, width = tables.shape
+    dev = seq.device
+    new = start[1:] - start[:-1]
+    ctx = seq - new
+    have, need = (ctx + BLOCK - 1) // BLOCK, (seq + BLOCK - 1) // BLOCK
+    grow = need - have
+    off = torch.cumsum(grow, 0) - grow + s["cursor"].long()
+    col = torch.arange(width, device=dev)[None, :]
+    at = (off[:, None] + col - have[:, None]).clamp(0, s["free_blocks"].numel() - 1)
+    fresh = (col >= have[:, None]) & (col < need[:, None])
+    tables.copy_(torch.where(fresh, s["free_blocks"][at], tables))
+    tok = torch.arange(s["num_tokens"], device=dev)
+    req = torch.searchsorted(start[1:].contiguous(), tok, right=True)
+    live = req < r
+    req = req.clamp(max=r - 1)
+    pos = ctx[req] + tok - start[req]
+    page = torch.where(live, pos // BLOCK, torch.zeros_like(pos))
+    slot = tables[req, page].long() * BLOCK + pos % BLOCK
+    return {"block_tables": tables, "slot_mapping": torch.where(live, slot, torch.full_like(slot, -1)),
+            "positions": torch.where(live, pos, torch.zeros_like(pos)),
+            "cursor": (s["cursor"].long() + grow.sum()).to(torch.int32)}
+
+
+def _angles(s):
+    ang = s["positions"].double()[:, None] * s["inv_freq"].double()[None, :]
+    return (torch.cos(ang).float() * s["factor"])[:, None, :], (torch.sin(ang).float() * s["factor"])[:, None, :]
+
+
+def _plain_rotate(x, cos, sin, interleaved):
+    rot = 2 * cos.shape[-1]
+    xf = x.float()
+    y = xf.clone()
+    if interleaved:
+        a, b = xf[..., 0:rot:2], xf[..., 1:rot:2]
+        y[..., 0:rot:2], y[..., 1:rot:2] = a * cos - b * sin, b * cos + a * sin
+    else:
+        a, b = xf[..., :rot // 2], xf[..., rot // 2:rot]
+        y[..., :rot // 2], y[..., rot // 2:rot] = a * cos - b * sin, b * cos + a * sin
+    return y.to(x.dtype)
+
+
+def _plain_quantize(x):
+    """[N, KV, D] -> packed codes [N, KV, D/2] and fp16 (min, step) [N, KV, 2]."""
+    xf = x.float()
+    lo = xf.amin(-1, keepdim=True)
+    step = (xf.amax(-1, keepdim=True) - lo) / torch.full_like(lo, 15.0)  # a true division
+    step = torch.where(step > 0, step, torch.ones_like(step))
+    code = ((xf - lo) / step + 0.5).to(torch.int32).clamp(0, 15)
+    return (code[..., 0::2] | (code[..., 1::2] << 4)).to(torch.uint8), torch.cat([lo, step], -1).to(torch.float16)
+
+
+def _plain_load(cache, slots, dtype):
+    d = cache.shape[-1] - 8
+    rows = cache.reshape(-1, cache.shape[2], d + 8)[slots]
+    rulers = rows[..., d:].contiguous().view(torch.float16).float()
+    both = rows[..., :d].reshape(*rows.shape[:2], 2, d // 2)
+    code = torch.stack([both & 15, both >> 4], -1).reshape(*rows.shape[:2], 2, d).float()
+    return [(code[:, :, i] * rulers[..., 2 * i + 1:2 * i + 2] + rulers[..., 2 * i:2 * i + 1]).to(dtype) for i in (0, 1)]
+
+
+def _plain_prompt(s):
+    q, k, v = s["q"], s["k"], s["v"]
+    n, hq, d = q.shape
+    kv = k.shape[1]
+    tok = torch.arange(n, device=q.device)
+    req = torch.searchsorted(s["query_start_loc"][1:].long().contiguous(), tok, right=True)
+    hidden = (req[:, None] != req[None, :]) | (tok[:, None] < tok[None, :])
+    qf = q.float().transpose(0, 1)
+    kf = k.float().transpose(0, 1).repeat_interleave(hq // kv, 0)
+    vf = v.float().transpose(0, 1).repeat_interleave(hq // kv, 0)
+    p = torch.matmul(qf, kf.transpose(1, 2)).mul_(1.0 / math.sqrt(d)).masked_fill_(hidden, -math.inf)
+    p.sub_(p.amax(-1, keepdim=True)).exp_()
+    out = torch.matmul(p, vf) / p.sum(-1, keepdim=True)
+    return out.transpose(0, 1).to(q.dtype).contiguous()
+
+
+def _plain(s):
+    op = s["op"]
+    if op == "plan":
+        return _plain_plan(s)
+    if op == "prompt":
+        return {"out": _plain_prompt(s)}
+    if op == "load":
+        k, v = _plain_load(s["cache"], s["slots"], s["dtype"])
+        return {"k": k, "v": v}
+    cos, sin = _angles(s)
+    q, k = _plain_rotate(s["q"], cos, sin, s["interleaved"]), _plain_rotate(s["k"], cos, sin, s["interleaved"])
+    if op == "rotary":
+        return {"q": q, "k": k}
+    kc, kr = _plain_quantize(k)
+    vc, vr = _plain_quantize(s["v"])
+    n, kv = kc.shape[:2]
+    slots = torch.cat([kc, vc, torch.cat([kr, vr], -1).view(torch.uint8).reshape(n, kv, 8)], -1)
+    s["cache"].view(-1, kv, slots.shape[-1])[s["slots"]] = slots
+    k4, v4 = _plain_load(s["cache"], s["slots"], q.dtype)
+    return {"q": q, "k": k, "k4": k4, "v4": v4}
+
+
+# ---------------------------------------------------- the library's operators
+def _own(s):
+    from slm_turbo_b200.kernels import kv_dequant as kd
+    op = s["op"]
+    if op == "plan":
+        slots, positions, cursor = kd.kv_page_plan(s["query_start_loc"], s["seq_lens"], s["block_tables"], BLOCK,
+                                                   s["num_tokens"], free_blocks=s["free_blocks"],
+                                                   free_cursor=s["cursor"])
+        return {"block_tables": s["block_tables"], "slot_mapping": slots, "positions": positions, "cursor": cursor[0]}
+    if op == "prompt":
+        out = torch.empty_like(s["q"])
+        kd.kv_prompt_attention(s["q"], s["k"], s["v"], s["query_start_loc"], s["max_query_len"], out=out)
+        return {"out": out}
+    if op == "load":
+        k, v = kd.kv_dequantize_load(s["cache"], s["slots"], dtype=s["dtype"])
+        return {"k": k, "v": v}
+    if op == "rotary":
+        q, k = kd.kv_rotary(s["q"], s["k"], s["positions"], s["inv_freq"], interleaved=s["interleaved"],
+                            attention_scaling=s["factor"])
+        return {"q": q, "k": k}
+    q, k = kd.kv_rotary_store(s["q"], s["k"], s["v"], s["positions"], s["inv_freq"], s["cache"], s["slots"],
+                              interleaved=s["interleaved"], attention_scaling=s["factor"])
+    k4, v4 = kd.kv_dequantize_load(s["cache"], s["slots"], dtype=q.dtype)
+    return {"q": q, "k": k, "k4": k4, "v4": v4}
+
+
+def run(state):
+    return _own(state) if own else _plain(state)
+
+
+# -------------------------------------------------------------------- work
+def work(case):
+    op = case["op"]
+    if op == "plan":
+        # the lengths' expected sum; every new token's slot and position out
+        r = case["requests"]
+        toks = r * (case["new"] or (case["lo"] + case["hi"]) / 2) + case["pad"]
+        new_blocks = r / BLOCK if case["new"] else toks / BLOCK
+        return {"bytes": 8.0 * r + 16.0 * toks + 8.0 * new_blocks, "flops": 0}
+    d, kv = case["d"], case["kv"]
+    if op == "prompt":
+        lens = _lens(case)
+        n, pairs = sum(lens), sum(x * (x + 1) // 2 for x in lens)
+        return {"bytes": 2.0 * n * d * (2 * case["hq"] + 2 * kv), "flops": 4.0 * case["hq"] * d * pairs}
+    n = case["tokens"]
+    if op == "load":
+        return {"bytes": n * kv * (d + 8.0 + 4 * d) + 8.0 * n, "flops": 4.0 * n * kv * d}
+    qk = n * (case["hq"] + kv)
+    total = {"bytes": qk * 4.0 * d + 8.0 * n, "flops": 3.0 * qk * case["rot"]}
+    if op == "rotary_store":  # v in, the slots out and, for the values returned, in again
+        total["bytes"] += n * kv * (2.0 * d + 2 * (d + 8) + 4 * d) + 16.0 * n
+    return total
+
+
+# ------------------------------------------------------------------- exact
+def _exact_prompt(case, seed):
+    s = prepare(case, seed)
+    q, k, v = s["q"], s["k"], s["v"]
+    hq, d = q.shape[1], q.shape[2]
+    group = hq // k.shape[1]
+    out = torch.zeros(q.shape, dtype=torch.float64, device=q.device)
+    at = 0
+    for n in _lens(case):
+        for h in range(hq):
+            kk, vv = k[at:at + n, h // group].double(), v[at:at + n, h // group].double()
+            for i in range(0, n, 4096):
+                m = min(n, i + 4096)
+                w = (q[at + i:at + m, h].double() @ kk[:m].T) / math.sqrt(d)
+                w += torch.triu(torch.full_like(w, -math.inf), diagonal=i + 1)
+                out[at + i:at + m, h] = torch.softmax(w, dim=-1) @ vv[:m]
+        at += n
+    return {"out": out}
+
+
+def _exact_rotate(x, theta, interleaved, factor):
+    """Rotation as multiplication by factor * exp(i theta) of the pairs (a + ib)."""
+    rot = 2 * theta.shape[-1]
+    turn = torch.polar(torch.full_like(theta, factor), theta)[:, None, :]
+    y = x.double()
+    if interleaved:
+        z = torch.view_as_complex(y[..., :rot].reshape(*y.shape[:-1], rot // 2, 2).contiguous()) * turn
+        head = torch.view_as_real(z).reshape(*y.shape[:-1], rot)
+    else:
+        z = torch.complex(y[..., :rot // 2].contiguous(), y[..., rot // 2:rot].contiguous()) * turn
+        head = torch.cat([z.real, z.imag], -1)
+    return torch.cat([head, y[..., rot:]], -1)
+
+
+def _exact_four_bits(x):
+    """What a row of 16-bit values stands for once it is held in 4 bits.  The
+    codes are defined by 32-bit arithmetic (rows of 16-bit values often lie
+    halfway between two of them); their values are exact."""
+    y = x.float().cpu().numpy()
+    lo, hi = y.min(-1, keepdims=True), y.max(-1, keepdims=True)
+    step = np.where(hi > lo, (hi - lo) / np.float32(15), np.float32(1))
+    code = np.clip(np.floor((y - lo) / step + np.float32(0.5)), 0, 15).astype(np.float64)
+    return torch.from_numpy(code * step.astype(np.float16).astype(np.float64) + lo.astype(np.float16).astype(np.float64))
+
+
+def _exact_load(s):
+    rows = s["cache"].cpu().numpy().reshape(-1, *s["cache"].shape[2:])[s["slots"].cpu().numpy()]
+    d = rows.shape[-1] - 8
+    rulers = np.ascontiguousarray(rows[..., d:]).view(np.float16).astype(np.float64)
+    got = []
+    for i in (0, 1):
+        codes = np.empty(rows.shape[:2] + (d,))
+        half = rows[..., i * d // 2:(i + 1) * d // 2]
+        codes[..., 0::2], codes[..., 1::2] = half % 16, half // 16
+        got.append(torch.from_numpy(codes * rulers[..., 2 * i + 1, None] + rulers[..., 2 * i, None]))
+    return {"k": got[0], "v": got[1]}
+
+
+def _exact_plan(case, seed):
+    s = prepare(case, seed)
+    seq, new = _plan_host(case)
+    tables, free = s["block_tables"].cpu().numpy().copy(), s["free_blocks"].cpu().numpy()
+    at = int(s["cursor"][0])
+    slots, positions = [], []
+    for r, (n, m) in enumerate(zip(seq, new)):
+        for b in range(-(-(n - m) // BLOCK), -(-n // BLOCK)):
+            tables[r, b] = free[at]
+            at += 1
+        pos = np.arange(n - m, n, dtype=np.int64)
+        slots.append(tables[r, pos // BLOCK].astype(np.int64) * BLOCK + pos % BLOCK)
+        positions.append(pos)
+    slots.append(np.full(case["pad"], -1, np.int64))
+    positions.append(np.zeros(case["pad"], np.int64))
+    return {"block_tables": tables, "slot_mapping": np.concatenate(slots), "positions": np.concatenate(positions),
+            "cursor": torch.tensor(at, dtype=torch.int32)}
+
+
+def exact(case, seed):
+    op = case["op"]
+    if op == "plan":
+        return _exact_plan(case, seed)
+    if op == "prompt":
+        return _exact_prompt(case, seed)
+    s = prepare(case, seed)
+    if op == "load":
+        return _exact_load(s)
+    theta = s["positions"].double()[:, None] * s["inv_freq"].double()[None, :]
+    q = _exact_rotate(s["q"], theta, case["interleaved"], case["factor"])
+    k = _exact_rotate(s["k"], theta, case["interleaved"], case["factor"])
+    if op == "rotary":
+        return {"q": q, "k": k}
+    # the cache holds the rows of the 16-bit type
+    return {"q": q, "k": k, "k4": _exact_four_bits(k.to(s["k"].dtype)), "v4": _exact_four_bits(s["v"])}
