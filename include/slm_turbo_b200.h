@@ -63,6 +63,7 @@ extern "C" {
 #define SLMT_DEVERR_SEQ_LEN 8u  /* sequence length above the table capacity     */
 #define SLMT_DEVERR_PLACEMENT 16u /* a decode grid that should hold two CTAs per SM
                                      did not (its SM-aware chunk ranges are incomplete) */
+#define SLMT_DEVERR_FREE_BLOCKS 32u /* slmt_page_plan: the free list has too few blocks */
 
 /* Library version (major*10000 + minor*100 + patch). */
 int slmt_version(void);
@@ -361,6 +362,128 @@ int slmt_paged_decode_noalloc(const void* q, int q_dtype, int64_t q_seq_stride,
                               int out_dtype, int64_t out_seq_stride,
                               int64_t out_head_stride, int reset_scratch,
                               int32_t* err_flag, void* stream);
+
+/* ---- the serving step around the cache ------------------------------------
+ * The entries below have no counterpart in the reference.  They cover what a
+ * serving step needs next to the cache's own store and decode: where its new
+ * tokens go, their rotary positions, attention of fresh prompts, and reading
+ * tokens back.  All strides are in elements; the head dimension is contiguous.
+ */
+
+/*
+ * Block tables, slot ids and positions of one step, from request lengths.
+ * Request r brings rows [query_start_loc[r], query_start_loc[r+1]) of the
+ * step: the last n_r of its seq_lens[r] tokens (lengths AFTER the step; int32,
+ * device).  With free_blocks (int32 [num_free], device) the pages that the
+ * new tokens enter are taken from it in request order, from index
+ * *free_cursor on (NULL: 0), and written to block_tables (int32 [num_reqs,
+ * max_blocks_per_seq], row stride bt_seq_stride); without, the tables are
+ * complete already.  slot_mapping / positions: int64 [num_tokens]; row t of
+ * request r gets block_tables[r][pos / block_size] * block_size + pos %
+ * block_size and pos.  Rows of no request (padding) get slot -1 and position
+ * 0.  *cursor_out (optional, not free_cursor itself) becomes the next free
+ * index.  Only entries of new pages are written to block_tables.
+ * A free list that is too short gives -1 entries and slots and sets
+ * SLMT_DEVERR_FREE_BLOCKS (cursor_out: num_free); a negative table or
+ * free-list entry gives slot -1 and SLMT_DEVERR_BLOCK_ID; lengths beyond the
+ * table, below n_r, or rows outside [0, num_tokens) give slot -1 and
+ * SLMT_DEVERR_SEQ_LEN.  No workspace, no host sync, deterministic.
+ */
+int slmt_page_plan(const int32_t* query_start_loc, const int32_t* seq_lens,
+                   int64_t num_reqs, int32_t* block_tables,
+                   int64_t bt_seq_stride, int64_t max_blocks_per_seq,
+                   int64_t block_size, const int32_t* free_blocks,
+                   int64_t num_free, const int32_t* free_cursor,
+                   int64_t num_tokens, int64_t* slot_mapping,
+                   int64_t* positions, int32_t* cursor_out, int32_t* err_flag,
+                   void* stream);
+
+/*
+ * Rotary positions: pair i of the first rotary_dim dims of every q and k row
+ * (dims i and i + rotary_dim/2, or 2i and 2i+1 when interleaved) turns by
+ * theta = position * inv_freq[i], scaled by `scaling`:
+ *     y1 = x1 c - x2 s, y2 = x2 c + x1 s, c = scaling cos, s = scaling sin;
+ * the other dims are copied.  theta is taken in 64 bits, c and s rounded to
+ * fp32, each product and sum rounded in fp32, the result once to the row
+ * type.  q [num_tokens, num_q_heads, head_dim], k [num_tokens, num_kv_heads,
+ * head_dim], fp16 or bf16 (dtype), either with 0 heads; positions int32 or
+ * int64 [num_tokens] (negative ones turn back); inv_freq fp32 [rotary_dim/2],
+ * device.  q_out / k_out may be q / k themselves (same strides); other
+ * overlaps are not allowed.
+ */
+int slmt_rotary(const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                const void* k, int64_t k_token_stride, int64_t k_head_stride,
+                int dtype, const void* positions, int pos_dtype,
+                const float* inv_freq, int64_t rotary_dim, int interleaved,
+                float scaling, int64_t num_tokens, int64_t num_q_heads,
+                int64_t num_kv_heads, int64_t head_dim, void* q_out,
+                int64_t qo_token_stride, int64_t qo_head_stride, void* k_out,
+                int64_t ko_token_stride, int64_t ko_head_stride, void* stream);
+
+/*
+ * slmt_rotary followed by slmt_kv_quantize_store of the rotated k rows and
+ * the v rows [num_tokens, num_kv_heads, head_dim], as one launch: the same
+ * rows and the same cache bytes.  k_out may be NULL (the rotated k goes to
+ * the cache only).  slot_mapping as slmt_kv_quantize_store (negative: the
+ * row is rotated but not stored).
+ */
+int slmt_rotary_store(const void* q, int64_t q_token_stride,
+                      int64_t q_head_stride, const void* k,
+                      int64_t k_token_stride, int64_t k_head_stride,
+                      const void* v, int64_t v_token_stride,
+                      int64_t v_head_stride, int dtype, const void* positions,
+                      int pos_dtype, const float* inv_freq, int64_t rotary_dim,
+                      int interleaved, float scaling, int64_t num_tokens,
+                      int64_t num_q_heads, int64_t num_kv_heads,
+                      int64_t head_dim, void* q_out, int64_t qo_token_stride,
+                      int64_t qo_head_stride, void* k_out,
+                      int64_t ko_token_stride, int64_t ko_head_stride,
+                      uint8_t* kv_cache, int64_t num_blocks,
+                      int64_t block_size, const int64_t* slot_mapping,
+                      int32_t* err_flag, void* stream);
+
+/*
+ * Tokens read back out of the paged cache: key / value [num_tokens,
+ * num_kv_heads, head_dim] contiguous, 16-byte aligned, in out_dtype
+ * (f32/f16/bf16) get code * step + min of slot_mapping[t]'s rows (one fp32
+ * rounding, then one to out_dtype).  A negative slot gives a row of zeros,
+ * one beyond the cache too and sets SLMT_DEVERR_SLOT.
+ */
+int slmt_kv_dequantize_load(const uint8_t* kv_cache, int64_t num_blocks,
+                            int64_t block_size, int64_t num_kv_heads,
+                            int64_t head_dim, const int64_t* slot_mapping,
+                            int64_t num_tokens, void* key, void* value,
+                            int out_dtype, int32_t* err_flag, void* stream);
+
+/*
+ * Causal attention of packed prompts over their own K and V.  Request r owns
+ * rows [query_start_loc[r], query_start_loc[r+1]) of q [num_tokens,
+ * num_q_heads, head_dim] and k / v [num_tokens, num_kv_heads, head_dim] (fp16
+ * or bf16); row i of it attends to its rows 0..i, query head h to kv head
+ * h / (num_q_heads / num_kv_heads).  seq_lens (optional): requests whose
+ * seq_lens[r] is not their number of rows (those with a cached context) are
+ * skipped.  out in out_dtype (f32/f16/bf16); rows of no request, of skipped
+ * requests and behind the last one are left as they were.  max_query_len
+ * bounds the requests' rows; a request with more sets SLMT_DEVERR_SEQ_LEN and
+ * its rows beyond are not written.  Rows outside [0, num_tokens) set it too.
+ * A row sees nothing of the keys and values it does not attend to, NaN and
+ * infinities included.  sm_scale positive and finite.  Pointers 16-byte
+ * aligned, strides multiples of 16 bytes.  At most 128 query heads per kv
+ * head.  No workspace, no host sync.
+ */
+int slmt_prompt_attention(const void* q, int64_t q_token_stride,
+                          int64_t q_head_stride, const void* k,
+                          int64_t k_token_stride, int64_t k_head_stride,
+                          const void* v, int64_t v_token_stride,
+                          int64_t v_head_stride, int dtype,
+                          const int32_t* query_start_loc,
+                          const int32_t* seq_lens, int64_t num_reqs,
+                          int64_t max_query_len, int64_t num_tokens,
+                          int64_t num_q_heads, int64_t num_kv_heads,
+                          int64_t head_dim, float sm_scale, void* out,
+                          int out_dtype, int64_t out_token_stride,
+                          int64_t out_head_stride, int32_t* err_flag,
+                          void* stream);
 
 #ifdef __cplusplus
 } /* extern "C" */

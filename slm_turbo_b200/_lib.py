@@ -7,6 +7,7 @@ Non-zero statuses become ``RuntimeError`` (the reference surfaces its
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import threading
 from pathlib import Path
@@ -50,6 +51,16 @@ SIGNATURES = {
     "slmt_paged_prefill": (_i32, [_vp, _i32, _i64, _i64, _vp, _i64, _i64, _i64, _i64, _vp, _i32, _i64, _i64,
                                   _vp, _vp, _i64, _i64, _i64, _f32, _vp, _i32, _i64, _i64, _vp, _vp]),
     "slmt_per_channel_quantize": (_i32, [_vp, _i32, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp]),
+    "slmt_page_plan": (_i32, [_vp, _vp, _i64, _vp, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp,
+                              _vp]),
+    "slmt_rotary": (_i32, [_vp, _i64, _i64, _vp, _i64, _i64, _i32, _vp, _i32, _vp, _i64, _i32, _f32, _i64, _i64,
+                           _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp]),
+    "slmt_rotary_store": (_i32, [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i32, _vp, _i32, _vp, _i64,
+                                 _i32, _f32, _i64, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64,
+                                 _i64, _vp, _vp, _vp]),
+    "slmt_kv_dequantize_load": (_i32, [_vp, _i64, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _i32, _vp, _vp]),
+    "slmt_prompt_attention": (_i32, [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i32, _vp, _vp, _i64,
+                                     _i64, _i64, _i64, _i64, _i64, _f32, _vp, _i32, _i64, _i64, _vp, _vp]),
     "slmt_per_channel_append": (_i32, [_vp, _i32, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _i64, _i64,
                                        _vp]),
 }
@@ -93,6 +104,14 @@ def ptr(t) -> ctypes.c_void_p:
 
 def stream_of(device: torch.device) -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+
+
+def on_device(device: torch.device):
+    """Context in which launches go to `device`: the C entries launch on the
+    current CUDA device, which need not be the tensors' one."""
+    if device.index is None or torch.cuda.current_device() == device.index:
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
 
 
 def dtype_tag(dt: torch.dtype) -> int:

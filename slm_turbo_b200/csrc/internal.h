@@ -12,6 +12,12 @@ namespace slmt {
 
 inline bool valid_head_dim(int64_t d) { return d == 64 || d == 80 || d == 128; }
 
+// Whether output rows of [tokens, heads] share memory because a stride is 0
+// (an expanded tensor): writes to them would race.
+inline bool rows_overlap(int64_t tokens, int64_t heads, int64_t token_stride, int64_t head_stride) {
+  return (tokens > 1 && token_stride == 0) || (heads > 1 && head_stride == 0);
+}
+
 // Status of the launch just issued (clears the sticky-free launch error).
 inline int launch_status() {
   const cudaError_t e = cudaGetLastError();

@@ -1,0 +1,323 @@
+// page_ops.cu -- page bookkeeping around the 4-bit paged cache (sm_100a).
+//
+//  * page_plan_kernel: block tables, slot ids and positions of one serving
+//    step, from the requests' lengths alone.
+//  * load_kernel: packed slots back to 16- or 32-bit K and V rows.
+#include "internal.h"
+#include "ptx.cuh"
+
+namespace slmt {
+
+namespace {
+
+// ------------------------------------------------------------- page plan --
+// Request r brings the n_r = qsl[r+1] - qsl[r] last of its seq_lens[r]
+// tokens, the first of them at position ctx_r = seq_lens[r] - n_r.  It owns
+// have_r = ceil(ctx_r / bs) pages and needs need_r = ceil(seq_lens[r] / bs);
+// page have_r + i is free_blocks[cursor + off_r + i] with the exclusive sum
+// off_r = sum_{r' < r} (need_r' - have_r').  Every CTA sums the requests for
+// itself (a tile of kPlanTile at a time), so one launch does all of it with
+// no exchange between CTAs and no atomics: the plan is the same every time.
+// A new page's first token is always one of the step's new tokens
+// (have_r * bs >= ctx_r), so the thread of that token writes the table entry;
+// entries of new pages are never read here, only computed.
+constexpr int kPlanThreads = 256;
+constexpr int kPlanTile = 1024;              // requests summed at a time
+constexpr int kPlanTokens = 4 * kPlanThreads;  // tokens of one CTA
+
+struct PlanParams {
+  const int32_t* qsl;
+  const int32_t* seq_lens;
+  int32_t* tables;
+  int64_t table_stride;
+  const int32_t* free_blocks;  // null: the tables are complete already
+  int64_t num_free;
+  const int32_t* cursor_in;  // null: 0
+  int64_t* slots;
+  int64_t* positions;
+  int32_t* cursor_out;
+  int32_t* err;
+  int num_reqs, num_tokens, block_size, max_blocks;
+};
+
+__device__ __forceinline__ void set_error(int32_t* err, unsigned bit) {
+  if (err) atomicOr(reinterpret_cast<unsigned int*>(err), bit);
+}
+
+__global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const PlanParams p) {
+  __shared__ int s_start[kPlanTile + 1];  // query_start_loc of the tile
+  __shared__ int s_ctx[kPlanTile];        // tokens before the step's, -1: lengths that do not fit
+  __shared__ int64_t s_off[kPlanTile];    // place of the request's first new page in the free list
+  __shared__ int64_t s_warp[kPlanThreads / 32];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int t0 = blockIdx.x * kPlanTokens;
+  const int t1 = min(t0 + kPlanTokens, p.num_tokens);
+  unsigned bad = 0u;
+
+  // rows of no request: the padding behind the last token (and anything
+  // before the first request's rows)
+  const int first = p.num_reqs ? p.qsl[0] : 0, last = p.num_reqs ? p.qsl[p.num_reqs] : 0;
+  for (int t = t0 + tid; t < t1; t += kPlanThreads) {
+    if (t < first || t >= last) {
+      p.slots[t] = -1;
+      p.positions[t] = 0;
+    }
+  }
+  if (last > p.num_tokens || first < 0) bad |= SLMT_DEVERR_SEQ_LEN;
+
+  int64_t base = p.cursor_in ? (int64_t)*p.cursor_in : 0;
+  for (int r0 = 0; r0 < p.num_reqs; r0 += kPlanTile) {
+    const int nr = min(kPlanTile, p.num_reqs - r0);
+    constexpr int PER = kPlanTile / kPlanThreads;
+    // thread t sums the requests PER*t .. PER*t+PER-1 of the tile
+    int grow[PER];
+    int64_t sum = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int r = PER * tid + i;
+      grow[i] = 0;
+      if (r < nr) {
+        const int a = p.qsl[r0 + r], b = p.qsl[r0 + r + 1], len = p.seq_lens[r0 + r];
+        int ctx = len - (b - a);
+        if (b < a || ctx < 0 || a < 0) {
+          ctx = -1;
+          bad |= SLMT_DEVERR_SEQ_LEN;
+        } else {
+          const int need = min((int)(((int64_t)len + p.block_size - 1) / p.block_size), p.max_blocks);
+          const int have = min((int)(((int64_t)ctx + p.block_size - 1) / p.block_size), p.max_blocks);
+          grow[i] = p.free_blocks ? need - have : 0;
+        }
+        s_start[r] = a;
+        s_ctx[r] = ctx;
+        if (r == nr - 1) s_start[nr] = b;
+      }
+      sum += grow[i];
+    }
+    int64_t incl = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t x = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += x;
+    }
+    if (lane == 31) s_warp[warp] = incl;
+    __syncthreads();
+    int64_t before = base, total = 0;
+#pragma unroll
+    for (int w = 0; w < kPlanThreads / 32; ++w) {
+      if (w < warp) before += s_warp[w];
+      total += s_warp[w];
+    }
+    before += incl - sum;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int r = PER * tid + i;
+      if (r < nr) s_off[r] = before;
+      before += grow[i];
+    }
+    base += total;
+    __syncthreads();
+
+    const int lo_t = max(t0, s_start[0]), hi_t = min(t1, s_start[nr]);
+    for (int t = lo_t + tid; t < hi_t; t += kPlanThreads) {
+      // the last request of the tile that starts at or before t
+      int lo = 0, hi = nr - 1;
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (s_start[mid] <= t) lo = mid;
+        else hi = mid - 1;
+      }
+      int64_t slot = -1;
+      int pos = 0;
+      const int ctx = s_ctx[lo];
+      if (ctx >= 0 && t >= s_start[lo] && t < s_start[lo + 1]) {
+        pos = ctx + (t - s_start[lo]);
+        const int page = pos / p.block_size, in_page = pos - page * p.block_size;
+        if (page >= p.max_blocks) {
+          bad |= SLMT_DEVERR_SEQ_LEN;
+        } else {
+          int32_t* entry = p.tables + (int64_t)(r0 + lo) * p.table_stride + page;
+          const int have = (int)(((int64_t)ctx + p.block_size - 1) / p.block_size);
+          int block;
+          if (p.free_blocks && page >= have) {
+            const int64_t at = s_off[lo] + (page - have);
+            block = -1;
+            if (at >= 0 && at < p.num_free) {
+              block = p.free_blocks[at];
+              if (block < 0) bad |= SLMT_DEVERR_BLOCK_ID;
+            } else {
+              bad |= SLMT_DEVERR_FREE_BLOCKS;
+            }
+            if (in_page == 0) *entry = block;
+          } else {
+            block = *entry;
+            if (block < 0) bad |= SLMT_DEVERR_BLOCK_ID;
+          }
+          if (block >= 0) slot = (int64_t)block * p.block_size + in_page;
+        }
+      }
+      p.slots[t] = slot;
+      p.positions[t] = pos;
+    }
+    __syncthreads();  // the tile's arrays are filled again
+  }
+  if (blockIdx.x == 0 && tid == 0 && p.cursor_out) {
+    if (p.free_blocks && base > p.num_free) {
+      bad |= SLMT_DEVERR_FREE_BLOCKS;
+      base = p.num_free;
+    }
+    *p.cursor_out = (int32_t)base;
+  }
+  if (bad) set_error(p.err, bad);
+}
+
+// ------------------------------------------------------------------- load --
+// x = code * step + min in fp32 (code * step is exact: 4 by 11 bits), rounded
+// once.  A thread turns 4 code bytes into 8 values: D/8 threads for a row's
+// K, D/8 for its V, so a warp's reads and 16-byte writes are contiguous.
+template <typename T>
+struct Vec8;
+template <>
+struct Vec8<__half> {
+  static __device__ __forceinline__ void store(void* p, const float (&x)[8]) {
+    uint4 v;
+    v.x = pack_half2(x[0], x[1]), v.y = pack_half2(x[2], x[3]);
+    v.z = pack_half2(x[4], x[5]), v.w = pack_half2(x[6], x[7]);
+    *reinterpret_cast<uint4*>(p) = v;
+  }
+};
+__device__ __forceinline__ uint32_t pack_bf162(float lo, float hi) {
+  __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<uint32_t*>(&h);
+}
+template <>
+struct Vec8<__nv_bfloat16> {
+  static __device__ __forceinline__ void store(void* p, const float (&x)[8]) {
+    uint4 v;
+    v.x = pack_bf162(x[0], x[1]), v.y = pack_bf162(x[2], x[3]);
+    v.z = pack_bf162(x[4], x[5]), v.w = pack_bf162(x[6], x[7]);
+    *reinterpret_cast<uint4*>(p) = v;
+  }
+};
+template <>
+struct Vec8<float> {
+  static __device__ __forceinline__ void store(void* p, const float (&x)[8]) {
+    reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
+    reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
+  }
+};
+
+template <int D, typename T>
+__global__ void __launch_bounds__(256) load_kernel(const uint8_t* __restrict__ cache, int64_t num_slots,
+                                                   const int64_t* __restrict__ slot_mapping, int64_t rows, int kv,
+                                                   T* __restrict__ key, T* __restrict__ value, int32_t* err) {
+  constexpr int PIECES = D / 4;  // 8-value pieces of a row's K and V
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t row = i / PIECES;
+  if (row >= rows) return;
+  const int piece = (int)(i - row * PIECES);
+  const int64_t tok = row / kv;
+  const int h = (int)(row - tok * kv);
+  const int which = piece >= PIECES / 2, c = piece - which * (PIECES / 2);
+  const int64_t slot = slot_mapping[tok];
+  float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  if (slot >= 0 && slot < num_slots) {
+    const uint8_t* s = cache + (slot * kv + h) * (D + 8);
+    const uint32_t codes = *reinterpret_cast<const uint32_t*>(s + which * (D / 2) + 4 * c);
+    const uint32_t rulers = *reinterpret_cast<const uint32_t*>(s + D + 4 * which);
+    const float mn = half_bits_to_float((uint16_t)(rulers & 0xFFFFu)), st = half_bits_to_float((uint16_t)(rulers >> 16));
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = __fmaf_rn((float)((codes >> (4 * j)) & 15u), st, mn);
+  } else if (slot >= num_slots && piece == 0 && h == 0) {
+    set_error(err, SLMT_DEVERR_SLOT);
+  }
+  Vec8<T>::store((which ? value : key) + row * D + 8 * c, x);
+}
+
+template <int D>
+int load_launch(const uint8_t* cache, int64_t num_slots, const int64_t* slot_mapping, int64_t rows, int kv, void* key,
+                void* value, int dtype, int32_t* err, cudaStream_t st) {
+  const int64_t blocks = (rows * (D / 4) + 255) / 256;
+  if (blocks > INT32_MAX) return SLMT_ERR_UNSUPPORTED;
+  const dim3 grid((unsigned)blocks);
+  if (dtype == SLMT_DTYPE_F16)
+    load_kernel<D, __half><<<grid, 256, 0, st>>>(cache, num_slots, slot_mapping, rows, kv, (__half*)key,
+                                                 (__half*)value, err);
+  else if (dtype == SLMT_DTYPE_BF16)
+    load_kernel<D, __nv_bfloat16><<<grid, 256, 0, st>>>(cache, num_slots, slot_mapping, rows, kv,
+                                                        (__nv_bfloat16*)key, (__nv_bfloat16*)value, err);
+  else
+    load_kernel<D, float><<<grid, 256, 0, st>>>(cache, num_slots, slot_mapping, rows, kv, (float*)key, (float*)value,
+                                                err);
+  return launch_status();
+}
+
+}  // namespace
+}  // namespace slmt
+
+using namespace slmt;
+
+extern "C" int slmt_page_plan(const int32_t* query_start_loc, const int32_t* seq_lens, int64_t num_reqs,
+                              int32_t* block_tables, int64_t bt_seq_stride, int64_t max_blocks_per_seq,
+                              int64_t block_size, const int32_t* free_blocks, int64_t num_free,
+                              const int32_t* free_cursor, int64_t num_tokens, int64_t* slot_mapping,
+                              int64_t* positions, int32_t* cursor_out, int32_t* err_flag, void* stream) {
+  if (num_reqs < 0 || num_tokens < 0 || max_blocks_per_seq < 0 || block_size <= 0 || num_free < 0)
+    return SLMT_ERR_SHAPE;
+  if (num_reqs > 1 && bt_seq_stride < max_blocks_per_seq) return SLMT_ERR_SHAPE;
+  // positions, token and page numbers are 32-bit in the kernel
+  if (num_tokens > INT32_MAX / 2 || num_reqs > INT32_MAX / 2 || num_free > INT32_MAX || block_size > INT32_MAX / 2 ||
+      max_blocks_per_seq > INT32_MAX / 2)
+    return SLMT_ERR_SHAPE;
+  if (num_reqs > 0 && (!query_start_loc || !seq_lens || (!block_tables && max_blocks_per_seq > 0)))
+    return SLMT_ERR_NULL;
+  if (num_tokens > 0 && (!slot_mapping || !positions)) return SLMT_ERR_NULL;
+  if (cursor_out && cursor_out == free_cursor) return SLMT_ERR_SHAPE;  // every CTA reads one, CTA 0 writes the other
+  if (num_tokens == 0 && !cursor_out) return SLMT_OK;
+  PlanParams p;
+  p.qsl = query_start_loc;
+  p.seq_lens = seq_lens;
+  p.tables = block_tables;
+  p.table_stride = bt_seq_stride;
+  p.free_blocks = free_blocks;
+  p.num_free = free_blocks ? num_free : 0;
+  p.cursor_in = free_cursor;
+  p.slots = slot_mapping;
+  p.positions = positions;
+  p.cursor_out = cursor_out;
+  p.err = err_flag;
+  p.num_reqs = (int)num_reqs;
+  p.num_tokens = (int)num_tokens;
+  p.block_size = (int)block_size;
+  p.max_blocks = (int)max_blocks_per_seq;
+  const int64_t grid = std::max<int64_t>(1, (num_tokens + kPlanTokens - 1) / kPlanTokens);
+  page_plan_kernel<<<(unsigned)grid, kPlanThreads, 0, reinterpret_cast<cudaStream_t>(stream)>>>(p);
+  return launch_status();
+}
+
+extern "C" int slmt_kv_dequantize_load(const uint8_t* kv_cache, int64_t num_blocks, int64_t block_size,
+                                       int64_t num_kv_heads, int64_t head_dim, const int64_t* slot_mapping,
+                                       int64_t num_tokens, void* key, void* value, int out_dtype, int32_t* err_flag,
+                                       void* stream) {
+  if (!valid_head_dim(head_dim)) return SLMT_ERR_HEAD_DIM;
+  if (num_tokens < 0 || num_kv_heads <= 0 || num_kv_heads > INT32_MAX / 2 || num_blocks < 0 || block_size <= 0)
+    return SLMT_ERR_SHAPE;
+  if (out_dtype != SLMT_DTYPE_F32 && out_dtype != SLMT_DTYPE_F16 && out_dtype != SLMT_DTYPE_BF16)
+    return SLMT_ERR_DTYPE;
+  if (num_tokens == 0) return SLMT_OK;
+  if (!kv_cache || !slot_mapping || !key || !value) return SLMT_ERR_NULL;
+  // 4-byte code words and ruler pairs in, 16-byte pieces out
+  if (reinterpret_cast<uintptr_t>(kv_cache) % 8 != 0 || reinterpret_cast<uintptr_t>(key) % 16 != 0 ||
+      reinterpret_cast<uintptr_t>(value) % 16 != 0)
+    return SLMT_ERR_ALIGN;
+  const int64_t slots = num_blocks * block_size, rows = num_tokens * num_kv_heads;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  const int kv = (int)num_kv_heads;
+  switch (head_dim) {
+    case 64:
+      return load_launch<64>(kv_cache, slots, slot_mapping, rows, kv, key, value, out_dtype, err_flag, st);
+    case 80:
+      return load_launch<80>(kv_cache, slots, slot_mapping, rows, kv, key, value, out_dtype, err_flag, st);
+    default:
+      return load_launch<128>(kv_cache, slots, slot_mapping, rows, kv, key, value, out_dtype, err_flag, st);
+  }
+}

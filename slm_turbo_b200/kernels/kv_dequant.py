@@ -18,6 +18,14 @@ launch),
 dimension), ``kv_quantize_per_channel`` / ``kv_append_per_channel`` (the
 per-channel quantizer of kernels/benchmark/benchmark.py on the device), and
 bf16 query/key/value inputs (rulers stay fp16).
+
+The serving step around the cache: ``kv_page_plan`` (block tables, slot ids
+and positions from request lengths), ``kv_rotary`` / ``kv_rotary_store``
+(rotary positions, alone or with the quantize-on-write, frequencies from
+``kv_rotary_inv_freq``), ``kv_prompt_attention`` (causal attention of packed
+prompts over their own K/V) and ``kv_dequantize_load`` (tokens read back).
+These are for serving: they have no backward pass and refuse inputs that
+require a gradient while autograd records.
 """
 from __future__ import annotations
 
@@ -38,6 +46,12 @@ __all__ = [
     "kv_dequant_decode_attention_batched",
     "kv_quantize_per_channel",
     "kv_append_per_channel",
+    "kv_page_plan",
+    "kv_rotary_inv_freq",
+    "kv_rotary",
+    "kv_rotary_store",
+    "kv_dequantize_load",
+    "kv_prompt_attention",
     "read_device_errors",
 ]
 
@@ -479,3 +493,337 @@ def kv_append_per_channel(x_new, scale, zero, packed, pos):
                                    _lib.ptr(scale.contiguous()), _lib.ptr(zero.contiguous()),
                                    _lib.ptr(packed), packed.shape[1], int(pos), _lib.stream_of(x_new.device))
     _lib.check(rc, "per-channel append")
+
+
+# =============================================================================
+#  The serving step around the cache
+# =============================================================================
+def _same_device(what, dev, **tensors):
+    for name, t in tensors.items():
+        if t is not None and t.device != dev:
+            raise RuntimeError(f"{what}: {name} is on {t.device}, expected {dev}")
+
+
+def _no_autograd(what, *tensors):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{what}: has no backward pass; call it under torch.no_grad() or on detached tensors")
+
+
+def _int32(t):
+    return t if t.dtype == torch.int32 and t.is_contiguous() else t.to(torch.int32).contiguous()
+
+
+def kv_page_plan(query_start_loc, seq_lens, block_tables, block_size, num_tokens, free_blocks=None,
+                 free_cursor=None, slot_mapping=None, positions=None):
+    """Where the tokens of one serving step go, from the requests' lengths.
+
+    Request r brings rows query_start_loc[r] .. query_start_loc[r+1]-1 of the
+    step, the LAST of its seq_lens[r] tokens (lengths after the step; int32 on
+    the device, no host sync).  With ``free_blocks`` (int32 [F]) the pages that
+    the new tokens enter are taken from it, from index ``free_cursor`` (int32
+    [1]; 0 by default) on, in request order, and written to ``block_tables``
+    (int32 [R, max_blocks], in place); without it the tables are complete.
+    Returns (slot_mapping int64 [num_tokens] for ``kv_quantize_store`` /
+    ``kv_rotary_store``, positions int64 [num_tokens] for ``kv_rotary``, and
+    the next free index, int32 [1]); rows behind the last request get slot -1
+    and position 0.  ``slot_mapping`` / ``positions`` may be given to be
+    written in place.  A free list that is too short, entries below 0 and
+    lengths beyond the table give slot -1 and set a device error bit.
+    """
+    L = _lib.load()
+    _require_cuda(block_tables, "page plan: block_tables", (torch.int32,))
+    dev = block_tables.device
+    num_tokens = int(num_tokens)
+    R = seq_lens.numel()
+    if block_tables.dim() != 2 or block_tables.size(0) < R or (block_tables.size(1) > 1 and block_tables.stride(1) != 1):
+        raise RuntimeError(f"page plan: block_tables must be [{R}, max_blocks] with unit column stride")
+    if query_start_loc.numel() < R + 1:
+        raise RuntimeError(f"page plan: query_start_loc needs {R + 1} entries, has {query_start_loc.numel()}")
+    if num_tokens < 0:
+        raise RuntimeError(f"page plan: num_tokens must not be negative, got {num_tokens}")
+    for name, t, n in (("free_blocks", free_blocks, None), ("free_cursor", free_cursor, 1)):
+        if t is not None and (t.dtype != torch.int32 or not t.is_contiguous() or (n is not None and t.numel() != n)):
+            raise RuntimeError(f"page plan: {name} must be contiguous int32" + (f" of {n} entry" if n else ""))
+    for name, t in (("slot_mapping", slot_mapping), ("positions", positions)):
+        if t is not None and (t.dtype != torch.int64 or not t.is_contiguous() or t.numel() != num_tokens):
+            raise RuntimeError(f"page plan: {name} must be contiguous int64 of length {num_tokens}")
+    _same_device("page plan", dev, query_start_loc=query_start_loc, seq_lens=seq_lens, free_blocks=free_blocks,
+                 free_cursor=free_cursor, slot_mapping=slot_mapping, positions=positions)
+    qsl, sl = _int32(query_start_loc), _int32(seq_lens)
+    if slot_mapping is None:
+        slot_mapping = torch.empty(num_tokens, dtype=torch.int64, device=dev)
+    if positions is None:
+        positions = torch.empty(num_tokens, dtype=torch.int64, device=dev)
+    cursor = torch.empty(1, dtype=torch.int32, device=dev)
+    with _lib.on_device(dev):
+        rc = L.slmt_page_plan(
+            qsl.data_ptr(), sl.data_ptr(), R, block_tables.data_ptr(), block_tables.stride(0), block_tables.size(1),
+            int(block_size), None if free_blocks is None else free_blocks.data_ptr(),
+            0 if free_blocks is None else free_blocks.numel(), None if free_cursor is None else free_cursor.data_ptr(),
+            num_tokens, slot_mapping.data_ptr(), positions.data_ptr(), cursor.data_ptr(),
+            _lib.error_word(dev).data_ptr(), _lib.stream_of(dev))
+    _lib.check(rc, "page plan")
+    return slot_mapping, positions, cursor
+
+
+def kv_rotary_inv_freq(rotary_dim, base=10000.0, scaling=None, device=None):
+    """Frequencies of the rotary pairs, and the factor of their cos and sin.
+
+    Plain: inv_freq[i] = base^(-2i / rotary_dim).  ``scaling`` is a dict in the
+    form of a transformers ``rope_scaling`` entry ("rope_type", "factor", ...):
+
+    * "linear": inv_freq / factor (positions interpolated);
+    * "dynamic": base stretched for "seq_len" tokens beyond
+      "original_max_position_embeddings" (NTK-aware);
+    * "yarn": frequencies that turn more than beta_fast times over the original
+      length stay, those below beta_slow are divided by factor, a linear ramp
+      between; cos and sin are scaled by "attention_factor" (0.1 ln factor + 1);
+    * "llama3": as yarn with the ramp between low_freq_factor and
+      high_freq_factor turns, linear in the number of turns.
+
+    Returns (fp32 [rotary_dim / 2] on ``device``, attention scaling); computed
+    in 64 bits, rounded once.
+    """
+    if rotary_dim < 2 or rotary_dim % 2:
+        raise RuntimeError(f"rotary_dim must be even and positive, got {rotary_dim}")
+    if not base > 0:
+        raise RuntimeError(f"rotary base must be positive, got {base}")
+    kind = "default" if scaling is None else scaling.get("rope_type", scaling.get("type", "default"))
+    exponent = torch.arange(0, rotary_dim, 2, dtype=torch.float64) / rotary_dim
+    freq = float(base) ** -exponent
+    factor_out = 1.0
+
+    def need(name):
+        if name not in scaling or scaling[name] is None:
+            raise RuntimeError(f"rotary scaling {kind!r} needs {name!r}")
+        return float(scaling[name])
+
+    if kind == "default":
+        pass
+    elif kind == "linear":
+        freq = freq / need("factor")
+    elif kind == "dynamic":
+        factor, orig = need("factor"), need("original_max_position_embeddings")
+        seq = max(need("seq_len"), orig)
+        if rotary_dim <= 2:
+            raise RuntimeError("rotary scaling 'dynamic' needs rotary_dim > 2")
+        stretched = float(base) * (factor * seq / orig - (factor - 1.0)) ** (rotary_dim / (rotary_dim - 2.0))
+        freq = stretched ** -exponent
+    elif kind in ("yarn", "llama3"):
+        factor, orig = need("factor"), need("original_max_position_embeddings")
+        if kind == "llama3":
+            low, high = need("low_freq_factor"), need("high_freq_factor")
+            turns = orig * freq / (2.0 * math.pi)  # over the original length
+            keep = ((turns - low) / (high - low)).clamp(0.0, 1.0)
+        else:
+            fast, slow = float(scaling.get("beta_fast") or 32.0), float(scaling.get("beta_slow") or 1.0)
+
+            def index_of(turns):  # the pair that makes this many turns over the original length
+                return rotary_dim * math.log(orig / (turns * 2.0 * math.pi)) / (2.0 * math.log(base))
+
+            first, last = index_of(fast), index_of(slow)
+            if scaling.get("truncate", True):
+                first, last = math.floor(first), math.ceil(last)
+            first, last = max(first, 0), min(last, rotary_dim - 1)
+            if first == last:
+                last += 0.001
+            i = torch.arange(rotary_dim // 2, dtype=torch.float64)
+            keep = 1.0 - ((i - first) / (last - first)).clamp(0.0, 1.0)
+            given = scaling.get("attention_factor")
+            factor_out = float(given) if given is not None else (0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0)
+        freq = keep * freq + (1.0 - keep) * freq / factor
+    else:
+        raise RuntimeError(f"rotary scaling {kind!r} is not one of default/linear/dynamic/yarn/llama3")
+    return freq.to(torch.float32).to(device or "cpu"), factor_out
+
+
+def _rotary_args(what, query, key, positions, inv_freq, query_out, key_out):
+    """Checks of kv_rotary / kv_rotary_store; returns the tensors to pass."""
+    _require_cuda(query, f"{what}: query", _QDT)
+    _require_cuda(key, f"{what}: key", _QDT)
+    if query.dtype != key.dtype:
+        raise RuntimeError(f"{what}: query/key dtypes differ")
+    if query.dim() != 3 or key.dim() != 3 or query.size(0) != key.size(0) or query.size(2) != key.size(2):
+        raise RuntimeError(f"{what}: query/key must be [N, H, D] and [N, KV, D], got {tuple(query.shape)} and "
+                           f"{tuple(key.shape)}")
+    N, _, D = query.shape
+    if positions.dtype not in (torch.int32, torch.int64) or positions.dim() != 1 or positions.numel() != N:
+        raise RuntimeError(f"{what}: positions must be int32/int64 of length {N}")
+    if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 or 2 * inv_freq.numel() > D:
+        raise RuntimeError(f"{what}: inv_freq must be float32 with at most head_dim/2 entries")
+    for name, o, t in (("query_out", query_out, query), ("key_out", key_out, key)):
+        if o is not None and (o.shape != t.shape or o.dtype != t.dtype or o.stride(2) != 1):
+            raise RuntimeError(f"{what}: {name} must be {tuple(t.shape)} {t.dtype} with unit head-dim stride")
+    _same_device(what, query.device, key=key, positions=positions, inv_freq=inv_freq, query_out=query_out,
+                 key_out=key_out)
+    _no_autograd(what, query, key, inv_freq, query_out, key_out)
+    # an in-place call reads the caller's own rows, whatever their strides
+    query = query if query.stride(2) == 1 else query.contiguous()
+    key = key if key.stride(2) == 1 else key.contiguous()
+    return query, key, positions.contiguous(), inv_freq.contiguous()
+
+
+def kv_rotary(query, key, positions, inv_freq, interleaved=False, attention_scaling=1.0, query_out=None,
+              key_out=None):
+    """Rotary positions of query [N, Hq, D] and key [N, KV, D] (fp16/bf16).
+
+    Pair i of the first 2 * len(inv_freq) dims -- (i, i + len(inv_freq)), or
+    (2i, 2i + 1) with ``interleaved`` -- of row n turns by positions[n] *
+    inv_freq[i] (int32/int64 and fp32, on the device; the angle is taken in 64
+    bits), its cos and sin times ``attention_scaling``; the other dims are
+    copied.  Negative positions turn back.  Returns (query, key) rotated: new
+    tensors, or ``query_out`` / ``key_out``, which may be the inputs themselves.
+    """
+    L = _lib.load()
+    q, k, pos, freq = _rotary_args("rotary", query, key, positions, inv_freq, query_out, key_out)
+    dev = q.device
+    qo = torch.empty(q.shape, dtype=q.dtype, device=dev) if query_out is None else query_out
+    ko = torch.empty(k.shape, dtype=k.dtype, device=dev) if key_out is None else key_out
+    with _lib.on_device(dev):
+        rc = L.slmt_rotary(
+            q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), _lib.dtype_tag(q.dtype),
+            pos.data_ptr(), _lib.dtype_tag(pos.dtype), freq.data_ptr(), 2 * freq.numel(), int(bool(interleaved)),
+            float(attention_scaling), q.size(0), q.size(1), k.size(1), q.size(2), qo.data_ptr(), qo.stride(0),
+            qo.stride(1), ko.data_ptr(), ko.stride(0), ko.stride(1), _lib.stream_of(dev))
+    _lib.check(rc, "rotary")
+    return qo, ko
+
+
+def kv_rotary_store(query, key, value, positions, inv_freq, kv_cache, slot_mapping, interleaved=False,
+                    attention_scaling=1.0, query_out=None, key_out=None, return_key=True):
+    """``kv_rotary`` of query and key and ``kv_quantize_store`` of the rotated
+    key and of value [N, KV, D], as one launch: the same rows, the same cache
+    bytes.
+
+    kv_cache [num_blocks, block_size, KV, D+8] uint8 (in place); slot_mapping
+    [N] int64 (negative: rotated, not stored).  Returns (query, key) rotated;
+    with ``return_key=False`` (a decode step, whose key is read from the cache)
+    the rotated key goes to the cache only and None is returned for it.
+    """
+    L = _lib.load()
+    q, k, pos, freq = _rotary_args("rotary store", query, key, positions, inv_freq, query_out, key_out)
+    N, KV, D = k.shape
+    _require_cuda(value, "rotary store: value", _QDT)
+    if value.dtype != key.dtype or value.shape != key.shape:
+        raise RuntimeError(f"rotary store: value must be {tuple(key.shape)} {key.dtype}")
+    if kv_cache.dtype != torch.uint8 or not kv_cache.is_contiguous() or kv_cache.dim() != 4:
+        raise RuntimeError("rotary store: kv_cache must be contiguous uint8 [num_blocks, block_size, KV, D+8]")
+    if kv_cache.size(2) != KV or kv_cache.size(3) != D + 8:
+        raise RuntimeError(f"rotary store: cache rows are {tuple(kv_cache.shape[2:])}, expected {(KV, D + 8)}")
+    if slot_mapping.dtype != torch.int64 or slot_mapping.numel() != N:
+        raise RuntimeError(f"rotary store: slot_mapping must be int64 of length {N}")
+    if key_out is not None and not return_key:
+        raise RuntimeError("rotary store: key_out is given but return_key is False")
+    dev = q.device
+    _same_device("rotary store", dev, value=value, kv_cache=kv_cache, slot_mapping=slot_mapping)
+    _no_autograd("rotary store", value)
+    v = value if value.stride(2) == 1 else value.contiguous()
+    sm = slot_mapping.contiguous()
+    qo = torch.empty(q.shape, dtype=q.dtype, device=dev) if query_out is None else query_out
+    ko = key_out
+    if ko is None and return_key:
+        ko = torch.empty(k.shape, dtype=k.dtype, device=dev)
+    with _lib.on_device(dev):
+        rc = L.slmt_rotary_store(
+            q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
+            v.stride(0), v.stride(1), _lib.dtype_tag(q.dtype), pos.data_ptr(), _lib.dtype_tag(pos.dtype),
+            freq.data_ptr(), 2 * freq.numel(), int(bool(interleaved)), float(attention_scaling), N, q.size(1), KV, D,
+            qo.data_ptr(), qo.stride(0), qo.stride(1), None if ko is None else ko.data_ptr(),
+            0 if ko is None else ko.stride(0), 0 if ko is None else ko.stride(1), kv_cache.data_ptr(),
+            kv_cache.size(0), kv_cache.size(1), sm.data_ptr(), _lib.error_word(dev).data_ptr(),
+            _lib.stream_of(dev))
+    _lib.check(rc, "rotary store")
+    return qo, ko
+
+
+def kv_dequantize_load(kv_cache, slot_mapping, dtype=torch.float16, key_out=None, value_out=None):
+    """Tokens read back out of the packed cache: (key, value) [N, KV, D] in
+    ``dtype`` (fp16/bf16/fp32), code * step + min of the rows at slot_mapping
+    [N] (int64).  Negative slots give zeros; slots beyond the cache too, and
+    set a device error bit.  ``key_out`` / ``value_out``: contiguous tensors to
+    write instead of new ones.
+    """
+    L = _lib.load()
+    _require_cuda(kv_cache, "load: kv_cache", (torch.uint8,))
+    if kv_cache.dim() != 4 or not kv_cache.is_contiguous():
+        raise RuntimeError("load: kv_cache must be contiguous [num_blocks, block_size, KV, D+8]")
+    if slot_mapping.dtype != torch.int64 or slot_mapping.dim() != 1:
+        raise RuntimeError("load: slot_mapping must be int64 [N]")
+    NB, bs, KV, row = kv_cache.shape
+    N, D, dev = slot_mapping.numel(), row - 8, kv_cache.device
+    for name, t in (("key_out", key_out), ("value_out", value_out)):
+        if t is not None and (tuple(t.shape) != (N, KV, D) or t.dtype != dtype or not t.is_contiguous()):
+            raise RuntimeError(f"load: {name} must be contiguous {(N, KV, D)} {dtype}")
+    _same_device("load", dev, slot_mapping=slot_mapping, key_out=key_out, value_out=value_out)
+    _no_autograd("load", key_out, value_out)
+    sm = slot_mapping.contiguous()
+    k = torch.empty(N, KV, D, dtype=dtype, device=dev) if key_out is None else key_out
+    v = torch.empty(N, KV, D, dtype=dtype, device=dev) if value_out is None else value_out
+    with _lib.on_device(dev):
+        rc = L.slmt_kv_dequantize_load(
+            kv_cache.data_ptr(), NB, bs, KV, D, sm.data_ptr(), N, k.data_ptr(), v.data_ptr(), _lib.dtype_tag(dtype),
+            _lib.error_word(dev).data_ptr(), _lib.stream_of(dev))
+    _lib.check(rc, "load")
+    return k, v
+
+
+def _tile_ready(t):
+    """`t` itself where 16-byte rows can be copied from it, else a dense copy."""
+    if t.stride(2) == 1 and t.stride(0) % 8 == 0 and t.stride(1) % 8 == 0 and t.data_ptr() % 16 == 0 \
+            and t.stride(0) > 0 and t.stride(1) > 0:
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def kv_prompt_attention(query, key, value, query_start_loc, max_query_len, seq_lens=None, out=None, sm_scale=None):
+    """Causal attention of packed prompts over their own K and V, one launch.
+
+    query [N, Hq, D], key/value [N, KV, D] (fp16/bf16): request r owns rows
+    query_start_loc[r] .. query_start_loc[r+1]-1 (int32 [R+1] on the device),
+    and row i of it attends to its rows 0..i; query head h reads kv head
+    h // (Hq // KV).  max_query_len (host int) bounds the requests' rows.  With
+    ``seq_lens`` (int32 [R]) only requests whose tokens are all in this step
+    (seq_lens[r] equal to their rows) are attended: the other half of a mixed
+    batch is ``kv_prefill_paged``'s.  Returns out [N, Hq, D] (fp32 by default,
+    or the given ``out`` in fp32/fp16/bf16); rows of no request and of skipped
+    ones are not written.  A row sees nothing of what it does not attend to,
+    NaN and infinities included.
+    """
+    L = _lib.load()
+    _require_cuda(query, "prompt attention: query", _QDT)
+    if query.dim() != 3 or key.dim() != 3 or key.shape != value.shape or key.size(0) != query.size(0) \
+            or key.size(2) != query.size(2):
+        raise RuntimeError(f"prompt attention: query [N, Hq, D] and key/value [N, KV, D] expected, got "
+                           f"{tuple(query.shape)}, {tuple(key.shape)}, {tuple(value.shape)}")
+    if key.dtype != query.dtype or value.dtype != query.dtype:
+        raise RuntimeError("prompt attention: query/key/value dtypes differ")
+    N, H, D = query.shape
+    KV = key.size(1)
+    if KV == 0 or H % KV:
+        raise RuntimeError(f"prompt attention: {H} query heads do not divide over {KV} kv heads")
+    R = query_start_loc.numel() - 1
+    if R < 0 or (seq_lens is not None and seq_lens.numel() != R):
+        raise RuntimeError("prompt attention: query_start_loc must have one entry more than there are requests"
+                           + ("" if seq_lens is None else f" (seq_lens has {seq_lens.numel()})"))
+    if out is not None and (out.shape != query.shape or (N > 0 and out.stride(2) != 1)):
+        raise RuntimeError(f"prompt attention: out must be {tuple(query.shape)} with unit head-dim stride")
+    dev = query.device
+    _same_device("prompt attention", dev, key=key, value=value, query_start_loc=query_start_loc, seq_lens=seq_lens,
+                 out=out)
+    _no_autograd("prompt attention", query, key, value, out)
+    if out is None:
+        out = torch.empty(N, H, D, dtype=torch.float32, device=dev)
+    if N == 0:
+        return out
+    q, k, v = _tile_ready(query), _tile_ready(key), _tile_ready(value)
+    qsl = _int32(query_start_loc)
+    sl = None if seq_lens is None else _int32(seq_lens)
+    with _lib.on_device(dev):
+        rc = L.slmt_prompt_attention(
+            q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
+            v.stride(0), v.stride(1), _lib.dtype_tag(q.dtype), qsl.data_ptr(), None if sl is None else sl.data_ptr(),
+            R, int(max_query_len), N, H, KV, D, float(1.0 / math.sqrt(D) if sm_scale is None else sm_scale),
+            out.data_ptr(), _lib.dtype_tag(out.dtype), out.stride(0), out.stride(1),
+            _lib.error_word(dev).data_ptr(), _lib.stream_of(dev))
+    _lib.check(rc, "prompt attention")
+    return out
