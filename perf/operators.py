@@ -271,7 +271,7 @@ def _own(s):
         slots, positions, cursor = kd.kv_page_plan(s["query_start_loc"], s["seq_lens"], s["block_tables"], BLOCK,
                                                    s["num_tokens"], free_blocks=s["free_blocks"],
                                                    free_cursor=s["cursor"])
-        return {"block_tables": s["block_tables"], "slot_mapping": slots, "positions": positions, "cursor": cursor[0]}
+        return {"block_tables": s["block_tables"], "slot_mapping": slots, "positions": positions, "cursor": cursor}
     if op == "prompt":
         out = torch.empty_like(s["q"])
         kd.kv_prompt_attention(s["q"], s["k"], s["v"], s["query_start_loc"], s["max_query_len"], out=out)
