@@ -26,7 +26,7 @@ SOURCES = ["decode.cu", "store.cu", "decode_noalloc.cu",
            "decode_d128_paged.cu", "decode_d128_contig.cu", "prefill.cu",
            "page_ops.cu", "rotary.cu", "prompt.cu"]
 HEADERS = ["ptx.cuh", "decode_common.cuh", "decode_kernels.cuh", "decode_dispatch.cuh", "quant_store.cuh",
-           "internal.h"]
+           "internal.h", "tcgen05.cuh"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

@@ -90,8 +90,6 @@ int current_device_sms(int* device_out) {
   return n;
 }
 
-namespace {
-
 // cuTensorMapEncodeTiled from the driver, looked up once through the runtime
 // (the library links the runtime only).
 PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
@@ -106,6 +104,10 @@ PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
   });
   return fn;
 }
+
+uint64_t wait_limit_ns() { return g_wait_limit_ns.load(std::memory_order_relaxed); }
+
+namespace {
 
 // Tensor map of packed codes [num_seqs, kv, s_cap, half bytes] (sequence
 // stride seq_stride_rows rows) viewed as 8-byte elements [num_seqs, kv,

@@ -2,86 +2,560 @@
 // (sm_100a): o_i = sum_{j <= i} softmax_j(scale q_i k_j) v_j within each
 // request, grouped heads.
 //
-// Simple form: one warp per (row, query head) with the online softmax's
-// running maximum, sum and output in registers.
+// One persistent CTA per SM, tiles of 128 query rows by 128 keys.  The rows of
+// a tile are (token, query head of one kv head's group), token by token, so a
+// group shares its K and V tiles and a prompt of a few tokens still fills
+// rows.  A work item is two such tiles of consecutive tokens (A and B) of one
+// request and kv head.
+//
+//   S = Q K^T   tcgen05.mma, both operands in shared memory, S in TMEM
+//   P = exp2((S - m) scale log2 e)   rounded to the inputs' type, over S in TMEM
+//   O += P V    tcgen05.mma, P from TMEM, V in shared memory as it was copied
+//
+// Warps 0-3 and 4-7 are the softmax of tile A and of tile B, a row per thread;
+// while one of them works on its scores, the tensor core computes the other
+// tile's products.  Warp 8 issues the products, warp 9 the tiled copies into
+// a ring of K and V tiles, warps 10 and 11 look at the V tiles on the
+// diagonal (below).  Every role walks the same list of items by itself.
+//
+// Running maximum: the reference m of a row moves only when a score passes it
+// by more than 2^8 in weight; until then old weights stay on their scale, and
+// O is rescaled in TMEM only then.  Sums are fp32, of the unrounded weights.
+//
+// What is not attended to is not seen: hidden scores are replaced, not added
+// to.  For V that is not enough -- a hidden key's weight is 0, but 0 times a
+// NaN or an infinity is a NaN -- so V tiles with a hidden key are searched for
+// such values; where there are some they are taken out of the tile, and added
+// to the rows that do attend to them at the end, read from global memory.
 #include "internal.h"
-#include "ptx.cuh"
+#include "tcgen05.cuh"
 
 namespace slmt {
 
 namespace {
 
+constexpr int kThreads = 384;
+constexpr int kMaxReqs = 2048;    // requests of one launch (sorted in shared memory)
+constexpr int kReqBits = 11;
+constexpr uint32_t kTmemCols = 512;
+constexpr int kMaxStages = 6;
+
 struct PromptParams {
-  const void* q;
-  const void* k;
   const void* v;
   void* out;
   const int32_t* qsl;
   const int32_t* seq_lens;
   int32_t* err;
-  int64_t q_tok, q_head, k_tok, k_head, v_tok, v_head, o_tok, o_head;
-  float scale;
-  int num_tokens, num_reqs, max_query, hq, kv, bf16, out_dtype;
+  int64_t v_tok, v_head, o_tok, o_head;
+  uint64_t wait_limit_ns;
+  float scale_log2;
+  int num_tokens, num_reqs, max_query, kv, group, tile_tokens, out_dtype;
 };
 
-__device__ __forceinline__ float get16(const void* p, int64_t i, int bf16) {
-  return bf16 ? __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p)[i])
-              : __half2float(reinterpret_cast<const __half*>(p)[i]);
-}
+struct PromptCtl {
+  uint64_t q_full[2], q_empty[2], s_full[2], p_ready[2], o_full[2], drain;
+  uint64_t kv_full[kMaxStages], kv_empty[kMaxStages], v_ok[kMaxStages];
+  uint32_t tmem;
+  uint32_t tile_bad[2];
+  uint32_t slot_bad[kMaxStages][2];
+  uint32_t sort_key[kMaxReqs];  // (pairs of tiles << kReqBits) | request, descending
+  int start[kMaxReqs], rows[kMaxReqs];
+};
 
 template <int D>
-__global__ void __launch_bounds__(128) prompt_simple_kernel(const PromptParams p) {
-  constexpr int VEC = (D + 31) / 32;
-  const int lane = threadIdx.x & 31;
-  const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  const int i = (int)(item / p.hq), h = (int)(item % p.hq);
-  const int r = blockIdx.y;
-  const int a = p.qsl[r], b = p.qsl[r + 1];
-  if (a < 0 || b < a || b > p.num_tokens || b - a > p.max_query) {
-    if (item == 0 && lane == 0 && p.err) atomicOr(reinterpret_cast<unsigned int*>(p.err), SLMT_DEVERR_SEQ_LEN);
+struct PromptGeom {
+  static constexpr int PANELS = (D + 63) / 64;        // 128-byte wide panels of a tile
+  static constexpr int TILE = PANELS * 128 * 128;     // bytes
+  static constexpr int STAGES = D == 64 ? 6 : 4;      // K and V take turns: an even number
+  static constexpr int SMEM = 1024 + (2 + STAGES) * TILE + (int)sizeof(PromptCtl);
+  static_assert(SMEM <= 227 * 1024 && STAGES % 2 == 0 && STAGES <= kMaxStages, "");
+};
+
+// One work item, as every role sees it.
+struct Item {
+  int req, head;     // request of this launch, kv head
+  int start, rows;   // the request's first row and its number of rows
+  int tok[2];        // first token of tile A and B
+  int steps[2];      // key tiles of each (0: no rows in tile B)
+  int nk;            // key tiles loaded
+  int guard;         // first key tile that some row of A or B does not see whole
+};
+
+// The items in the order of falling cost -- requests' last tiles first -- dealt
+// to the CTAs back and forth, so that their sums stay within about one small
+// item of each other.  Level t holds the items of tile pair t of every request
+// that has one: those are the first `count` of the requests sorted by length.
+struct Walk {
+  int k, level, count;
+  int64_t base;
+  __device__ __forceinline__ void begin(const PromptCtl* c) {
+    k = 0, count = 0, base = 0;
+    level = (int)(c->sort_key[0] >> kReqBits);
   }
-  const int lo = max(a, 0), hi = min(b, p.num_tokens);
-  if (i >= hi - lo || i >= p.max_query) return;
-  if (p.seq_lens && p.seq_lens[r] != b - a) return;
-  const int hk = h / (p.hq / p.kv);
-  float q[VEC], o[VEC], m = -INFINITY, l = 0.f;
-#pragma unroll
-  for (int d = 0; d < VEC; ++d) {
-    const int c = lane + 32 * d;
-    q[d] = c < D ? get16(p.q, (int64_t)(lo + i) * p.q_tok + (int64_t)h * p.q_head + c, p.bf16) : 0.f;
-    o[d] = 0.f;
-  }
-  for (int j = 0; j <= i; ++j) {
-    float s = 0.f;
-#pragma unroll
-    for (int d = 0; d < VEC; ++d) {
-      const int c = lane + 32 * d;
-      if (c < D) s += q[d] * get16(p.k, (int64_t)(lo + j) * p.k_tok + (int64_t)hk * p.k_head + c, p.bf16);
+  __device__ __forceinline__ bool next(const PromptCtl* c, const PromptParams& p, Item& it) {
+    const int nc = gridDim.x;
+    const int64_t at = (int64_t)k * nc + ((k & 1) ? nc - 1 - (int)blockIdx.x : (int)blockIdx.x);
+    ++k;
+    while (at >= base + (int64_t)count * p.kv) {
+      base += (int64_t)count * p.kv;
+      if (--level < 0) return false;
+      while (count < p.num_reqs && (int)(c->sort_key[count] >> kReqBits) > level) ++count;
     }
+    const int rem = (int)(at - base);
+    it.head = rem % p.kv;
+    it.req = (int)(c->sort_key[rem / p.kv] & ((1u << kReqBits) - 1));
+    it.start = c->start[it.req];
+    it.rows = c->rows[it.req];
+    it.tok[0] = level * 2 * p.tile_tokens;
+    it.tok[1] = it.tok[0] + p.tile_tokens;
+    it.steps[0] = (min(it.tok[1], it.rows) + 127) >> 7;
+    it.steps[1] = it.tok[1] < it.rows ? (min(it.tok[1] + p.tile_tokens, it.rows) + 127) >> 7 : 0;
+    it.nk = max(it.steps[0], it.steps[1]);
+    it.guard = (it.tok[0] + 1) >> 7;
+    return true;
+  }
+};
+
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack16(float lo, float hi) {
+  if constexpr (BF16) {
+    __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<uint32_t*>(&h);
+  } else {
+    return pack_half2(lo, hi);
+  }
+}
+
+// Write 16 finished columns of an output row.
+__device__ __forceinline__ void store16(void* out, int out_dtype, int64_t at, const float* x) {
+  if (out_dtype == SLMT_DTYPE_F32) {
+    float4* o = reinterpret_cast<float4*>(reinterpret_cast<float*>(out) + at);
 #pragma unroll
-    for (int w = 16; w > 0; w >>= 1) s += __shfl_xor_sync(0xffffffffu, s, w);
-    s *= p.scale;
-    const float mn = fmaxf(m, s);
-    const float base = mn == -INFINITY ? 0.f : mn;
-    const float f = expf(m - base), e = expf(s - base);
-    l = l * f + e;
+    for (int i = 0; i < 4; ++i) o[i] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+    return;
+  }
+  uint4* o = reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(out) + at);
 #pragma unroll
-    for (int d = 0; d < VEC; ++d) {
-      const int c = lane + 32 * d;
-      if (c < D) o[d] = o[d] * f + e * get16(p.v, (int64_t)(lo + j) * p.v_tok + (int64_t)hk * p.v_head + c, p.bf16);
+  for (int i = 0; i < 2; ++i) {
+    uint4 w;
+    if (out_dtype == SLMT_DTYPE_F16)
+      w = make_uint4(pack_half2(x[8 * i], x[8 * i + 1]), pack_half2(x[8 * i + 2], x[8 * i + 3]),
+                     pack_half2(x[8 * i + 4], x[8 * i + 5]), pack_half2(x[8 * i + 6], x[8 * i + 7]));
+    else
+      w = make_uint4(pack16<true>(x[8 * i], x[8 * i + 1]), pack16<true>(x[8 * i + 2], x[8 * i + 3]),
+                     pack16<true>(x[8 * i + 4], x[8 * i + 5]), pack16<true>(x[8 * i + 6], x[8 * i + 7]));
+    o[i] = w;
+  }
+}
+
+template <int D, bool BF16>
+__global__ void __launch_bounds__(kThreads, 1)
+    prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                  const __grid_constant__ CUtensorMap map_v, const PromptParams p) {
+  using G = PromptGeom<D>;
+  constexpr int TILE = G::TILE, STAGES = G::STAGES, PANELS = G::PANELS;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  PromptCtl* c = reinterpret_cast<PromptCtl*>(smem + (2 + STAGES) * TILE);
+  uint8_t* ring = smem + 2 * TILE;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const uint64_t limit = p.wait_limit_ns;
+
+  // ---- set-up: barriers, tensor memory, the requests sorted by length
+  if (tid == 0) {
+    for (int x = 0; x < 2; ++x) {
+      mbar_init(&c->q_full[x], 1), mbar_init(&c->q_empty[x], 1);
+      mbar_init(&c->s_full[x], 1), mbar_init(&c->p_ready[x], 128);
+      mbar_init(&c->o_full[x], 2);  // the commit, and the thread that set tile_bad
     }
-    m = mn;
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&c->kv_full[s], 1);
+      mbar_init(&c->kv_empty[s], s & 1 ? 3 : 1);  // V tiles: the commit and both guard warps
+      mbar_init(&c->v_ok[s], 2);
+    }
+    mbar_init(&c->drain, 1);
+    fence_mbar_init();
   }
+  if (warp == 8) tmem_alloc(&c->tmem, kTmemCols);
+  int n2 = 1;
+  while (n2 < p.num_reqs) n2 <<= 1;
+  unsigned bad_len = 0u;
+  for (int r = tid; r < n2; r += kThreads) {
+    int n = 0, a = 0;
+    if (r < p.num_reqs) {
+      const int qa = p.qsl[r], qb = p.qsl[r + 1];
+      if (!(p.seq_lens && p.seq_lens[r] != qb - qa)) {
+        a = max(qa, 0);
+        n = max(min(qb, p.num_tokens) - a, 0);
+        if (qa < 0 || qb < qa || qb > p.num_tokens || n > p.max_query) bad_len = SLMT_DEVERR_SEQ_LEN;
+        n = min(n, p.max_query);
+      }
+      c->start[r] = a;
+      c->rows[r] = n;
+    }
+    const int pairs = (n + 2 * p.tile_tokens - 1) / (2 * p.tile_tokens);
+    c->sort_key[r] = ((uint32_t)pairs << kReqBits) | (uint32_t)r;
+  }
+  if (bad_len && blockIdx.x == 0 && p.err) atomicOr(reinterpret_cast<unsigned int*>(p.err), bad_len);
+  __syncthreads();
+  for (int k = 2; k <= n2; k <<= 1)
+    for (int j = k >> 1; j > 0; j >>= 1) {
+      for (int i = tid; i < n2; i += kThreads) {
+        const int o = i ^ j;
+        if (o > i) {
+          const uint32_t x = c->sort_key[i], y = c->sort_key[o];
+          if ((x < y) == ((i & k) == 0)) c->sort_key[i] = y, c->sort_key[o] = x;
+        }
+      }
+      __syncthreads();
+    }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = c->tmem;
+  // columns: S of A and B (128 each; P takes the first 64 of each), O of A and B
+  const uint32_t col_s = 0, col_o = 256;
+
+  bool failed = false;
+  if (warp >= 8) {
+    regs_lower<88>();
+    if (warp == 9) {
+      // ------------------------------------------------------------ copies
+      if (lane == 0) {
+        uint32_t fill = 0, nq[2] = {0, 0};
+        auto load_q = [&](const Item& it, int x) {
+          if (!mbar_wait(&c->q_empty[x], (nq[x] & 1u) ^ 1u, limit)) return false;
+          ++nq[x];
+          mbar_arrive_expect_tx(&c->q_full[x], (uint32_t)(PANELS * 128 * p.tile_tokens * p.group));
+          for (int d = 0; d < PANELS; ++d)
+            tma_load_3d(smem + x * TILE + d * 16384, &map_q, d * 64, it.head * p.group, it.start + it.tok[x],
+                        &c->q_full[x]);
+          return true;
+        };
+        auto load_kv = [&](const Item& it, int j, const CUtensorMap* map) {
+          const uint32_t s = fill % STAGES;
+          if (!mbar_wait(&c->kv_empty[s], ((fill / STAGES) & 1u) ^ 1u, limit)) return false;
+          ++fill;
+          mbar_arrive_expect_tx(&c->kv_full[s], TILE);
+          for (int d = 0; d < PANELS; ++d)
+            tma_load_3d(ring + s * TILE + d * 16384, map, d * 64, it.head, it.start + 128 * j, &c->kv_full[s]);
+          return true;
+        };
+        Walk w;
+        Item it;
+        w.begin(c);
+        while (!failed && w.next(c, p, it)) {
+          bool ok = load_kv(it, 0, &map_k) && load_q(it, 0) && (it.steps[1] == 0 || load_q(it, 1));
+          ok = ok && load_kv(it, 0, &map_v);
+          for (int j = 1; ok && j < it.nk; ++j) ok = load_kv(it, j, &map_k) && load_kv(it, j, &map_v);
+          failed = !ok;
+        }
+        // no copy is in flight when this thread is done, whatever happened
+        for (uint32_t f = fill > (uint32_t)STAGES ? fill - STAGES : 0; f < fill; ++f)
+          if (!mbar_wait(&c->kv_full[f % STAGES], (f / STAGES) & 1u, limit)) failed = true;
+        for (int x = 0; x < 2; ++x)
+          if (nq[x] && !mbar_wait(&c->q_full[x], (nq[x] - 1) & 1u, limit)) failed = true;
+      }
+    } else if (warp == 8) {
+      // ----------------------------------------------------------- products
+      if (lane == 0) {
+        constexpr uint32_t idesc_s = mma_idesc(BF16, 128, 128, false), idesc_o = mma_idesc(BF16, 128, D, true);
+        const uint32_t q_addr = smem_addr(smem), ring_addr = smem_addr(ring);
+        uint32_t fill = 0, nq[2] = {0, 0}, np[2] = {0, 0}, ok_phase = 0;
+        auto full = [&](uint32_t f) { return mbar_wait(&c->kv_full[f % STAGES], (f / STAGES) & 1u, limit); };
+        auto scores = [&](int x, uint32_t f) {
+          const uint32_t a = q_addr + x * TILE, b = ring_addr + (f % STAGES) * TILE;
 #pragma unroll
-  for (int d = 0; d < VEC; ++d) {
-    const int c = lane + 32 * d;
-    if (c >= D) continue;
-    const int64_t at = (int64_t)(lo + i) * p.o_tok + (int64_t)h * p.o_head + c;
-    const float x = o[d] / l;
-    if (p.out_dtype == SLMT_DTYPE_F32) reinterpret_cast<float*>(p.out)[at] = x;
-    else if (p.out_dtype == SLMT_DTYPE_F16) reinterpret_cast<__half*>(p.out)[at] = __float2half_rn(x);
-    else reinterpret_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(x);
+          for (int u = 0; u < D / 16; ++u) {
+            const uint32_t off = (u >> 2) * 16384 + (u & 3) * 32;
+            mma_ss(tmem + col_s + 128 * x, smem_desc(a + off, 16, 1024), smem_desc(b + off, 16, 1024), idesc_s, u > 0);
+          }
+          mma_commit(&c->s_full[x]);
+        };
+        auto weigh = [&](int x, uint32_t f, bool first) {
+          const uint32_t b = ring_addr + (f % STAGES) * TILE;
+#pragma unroll
+          for (int u = 0; u < 8; ++u)
+            mma_ts(tmem + col_o + D * x, tmem + col_s + 128 * x + 8 * u, smem_desc(b + u * 2048, 16384, 1024), idesc_o,
+                   !first || u > 0);
+        };
+        auto wait_q = [&](int x) { return mbar_wait(&c->q_full[x], nq[x]++ & 1u, limit); };
+        auto wait_p = [&](int x) {
+          const bool ok = mbar_wait(&c->p_ready[x], np[x]++ & 1u, limit);
+          tc_fence_after();
+          return ok;
+        };
+        Walk w;
+        Item it;
+        w.begin(c);
+        while (!failed && w.next(c, p, it)) {
+          uint32_t bad = 0;
+          bool ok = full(fill) && wait_q(0);
+          if (!ok) {
+            failed = true;
+            break;
+          }
+          scores(0, fill);
+          if (it.steps[0] == 1) mma_commit(&c->q_empty[0]);
+          if (it.steps[1]) {
+            if (!wait_q(1)) {
+              failed = true;
+              break;
+            }
+            scores(1, fill);
+            if (it.steps[1] == 1) mma_commit(&c->q_empty[1]);
+          }
+          mma_commit(&c->kv_empty[fill % STAGES]);
+          for (int j = 0; j < it.nk; ++j) {
+            const uint32_t fv = fill + 2 * j + 1, fk = fv + 1;
+            if (!full(fv)) {
+              failed = true;
+              break;
+            }
+            if (j >= it.guard) {
+              const uint32_t s = fv % STAGES;
+              if (!mbar_wait(&c->v_ok[s], (ok_phase >> s) & 1u, limit)) {
+                failed = true;
+                break;
+              }
+              ok_phase ^= 1u << s;
+              bad |= c->slot_bad[s][0] | c->slot_bad[s][1];
+            }
+            bool have_k = j + 1 >= it.nk;  // nothing to wait for
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              if (j >= it.steps[x]) continue;
+              if (!wait_p(x)) {
+                failed = true;
+                break;
+              }
+              weigh(x, fv, j == 0);
+              if (j + 1 < it.steps[x]) {
+                if (!have_k && !full(fk)) {
+                  failed = true;
+                  break;
+                }
+                have_k = true;
+                scores(x, fk);
+                if (j + 2 == it.steps[x]) mma_commit(&c->q_empty[x]);
+              } else {
+                c->tile_bad[x] = bad;
+                mbar_arrive(&c->o_full[x]);
+                mma_commit(&c->o_full[x]);
+              }
+            }
+            if (failed) break;
+            mma_commit(&c->kv_empty[fv % STAGES]);
+            if (j + 1 < it.nk) mma_commit(&c->kv_empty[fk % STAGES]);
+          }
+          fill += 2 * it.nk;
+        }
+        if (failed) {  // products in flight read shared and tensor memory
+          mma_commit(&c->drain);
+          mbar_wait(&c->drain, 0, limit);
+        }
+      }
+    } else {
+      // ------------------------------------------- non-finite values in V
+      constexpr uint32_t EXP = BF16 ? 0x7F80u : 0x7C00u;
+      const int half = warp - 10;
+      uint32_t fill = 0;
+      Walk w;
+      Item it;
+      w.begin(c);
+      while (!failed && w.next(c, p, it)) {
+        for (int j = 0; j < it.nk; ++j) {
+          const uint32_t f = fill + 2 * j + 1, s = f % STAGES;
+          if (!__all_sync(0xffffffffu, mbar_wait(&c->kv_full[s], (f / STAGES) & 1u, limit))) {
+            failed = true;
+            break;
+          }
+          if (j >= it.guard) {
+            uint4* tile = reinterpret_cast<uint4*>(ring + s * TILE + half * (TILE / 2));
+            uint32_t top = 0;
+#pragma unroll 8
+            for (int i = lane; i < TILE / 32; i += 32) {
+              const uint4 x = tile[i];
+              top = __vmaxu2(top, x.x & 0x7FFF7FFFu);
+              top = __vmaxu2(top, x.y & 0x7FFF7FFFu);
+              top = __vmaxu2(top, x.z & 0x7FFF7FFFu);
+              top = __vmaxu2(top, x.w & 0x7FFF7FFFu);
+            }
+            const bool found = __any_sync(0xffffffffu, (top & 0xFFFFu) >= EXP || (top >> 16) >= EXP);
+            if (found) {
+              uint16_t* v = reinterpret_cast<uint16_t*>(tile);
+              for (int i = lane; i < TILE / 4; i += 32)
+                if ((v[i] & EXP) == EXP) v[i] = 0;
+              fence_proxy_async_shared();  // before the tensor core reads them
+            }
+            __syncwarp();
+            if (lane == 0) {
+              c->slot_bad[s][half] = found;
+              mbar_arrive(&c->v_ok[s]);
+            }
+          }
+          if (lane == 0) mbar_arrive(&c->kv_empty[s]);
+        }
+        fill += 2 * it.nk;
+      }
+    }
+  } else {
+    // ---------------------------------------------------------------- softmax
+    regs_raise<208>();
+    constexpr float SHIFT = BF16 ? 0.f : 6.f;  // fp16 weights lie in [2^-24, 2^14]: a row's largest is 2^6 or more
+    constexpr float MOVE = 8.f;
+    const int x = warp >> 2, row = tid & 127;
+    const int row_tok = row / p.group, row_head = row - row_tok * p.group;
+    const uint32_t lane_base = (uint32_t)(warp & 3) << 21;
+    const uint32_t ts = tmem + lane_base + col_s + 128 * x, to = tmem + lane_base + col_o + D * x;
+    const float sc = p.scale_log2;
+    uint32_t ns = 0, no = 0;
+    Walk w;
+    Item it;
+    w.begin(c);
+    while (!failed && w.next(c, p, it)) {
+      const int steps = it.steps[x];
+      if (steps == 0) continue;
+      const int tok = min(it.tok[x] + row_tok, it.rows - 1);
+      const int first_hidden = (it.tok[x] + 1) >> 7;  // first key tile that a row of this tile does not see whole
+      float m = -INFINITY, ref = 0.f, sum = 0.f;
+      for (int j = 0; j < steps; ++j) {
+        if (!__all_sync(0xffffffffu, mbar_wait(&c->s_full[x], ns++ & 1u, limit))) {
+          failed = true;
+          break;
+        }
+        tc_fence_after();
+        float s[128];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) tmem_ld32(s + 32 * i, ts + 32 * i);
+        tmem_wait_ld();
+        if (j >= first_hidden) {
+          const int seen = tok - 128 * j;  // columns 0..seen are attended to
+#pragma unroll
+          for (int i = 0; i < 128; ++i) s[i] = i <= seen ? s[i] : -INFINITY;
+        }
+        float mx[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+        for (int i = 4; i < 128; i += 4) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) mx[k] = fmaxf(mx[k], s[i + k]);
+        }
+        const float top = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
+        if (j == 0) {
+          m = top;
+        } else {
+          const bool move = (top - m) * sc > MOVE;
+          if (__any_sync(0xffffffffu, move)) {
+            // products up to the last step's are done: this step's scores, issued after them, are
+            const float f = move ? exp2_approx((m - top) * sc) : 1.f;
+            if (move) m = top;
+            sum *= f;
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) {
+              float o[16];
+              tmem_ld16(o, to + 16 * i);
+              tmem_wait_ld();
+#pragma unroll
+              for (int k = 0; k < 16; ++k) o[k] *= f;
+              tmem_st16(to + 16 * i, reinterpret_cast<uint32_t*>(o));
+            }
+          }
+        }
+        ref = m == -INFINITY ? 0.f : m;
+        const uint64_t neg = f2_pack(-ref, -ref), scale2 = f2_pack(sc, sc), shift2 = f2_pack(SHIFT, SHIFT);
+        uint64_t acc = f2_pack(0.f, 0.f);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          uint32_t w16[16];
+#pragma unroll
+          for (int k = 0; k < 16; ++k) {
+            // the difference first: exact near the maximum, whatever its size
+            const uint64_t e = f2_fma(f2_add(f2_pack(s[32 * i + 2 * k], s[32 * i + 2 * k + 1]), neg), scale2, shift2);
+            float lo, hi;
+            f2_unpack(e, lo, hi);
+            lo = exp2_approx(lo), hi = exp2_approx(hi);
+            acc = f2_add(acc, f2_pack(lo, hi));
+            w16[k] = pack16<BF16>(lo, hi);
+          }
+          tmem_st16(ts + 16 * i, w16);
+        }
+        float a0, a1;
+        f2_unpack(acc, a0, a1);
+        sum += a0 + a1;
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(&c->p_ready[x]);
+      }
+      if (failed) break;
+      if (!__all_sync(0xffffffffu, mbar_wait(&c->o_full[x], no++ & 1u, limit))) {
+        failed = true;
+        break;
+      }
+      tc_fence_after();
+      const bool valid = row_tok < p.tile_tokens && it.tok[x] + row_tok < it.rows;
+      const float inv = 1.f / sum;
+      const int h = it.head * p.group + row_head;
+      const int64_t at = (int64_t)(it.start + tok) * p.o_tok + (int64_t)h * p.o_head;
+      const bool bad = c->tile_bad[x] != 0;
+#pragma unroll 1
+      for (int i = 0; i < D / 16; ++i) {
+        float o[16];
+        tmem_ld16(o, to + 16 * i);
+        tmem_wait_ld();
+#pragma unroll
+        for (int k = 0; k < 16; ++k) o[k] *= inv;
+        if (bad && valid) {
+          // the values taken out of the V tiles, for the rows that attend to them
+          for (int j = 128 * it.guard; j <= tok; ++j) {
+            const uint16_t* v = reinterpret_cast<const uint16_t*>(p.v) + (int64_t)(it.start + j) * p.v_tok +
+                                (int64_t)it.head * p.v_head + 16 * i;
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+              const float y = BF16 ? __bfloat162float(__ushort_as_bfloat16(v[k])) : __half2float(__ushort_as_half(v[k]));
+              if (!(y - y == 0.f)) o[k] += y;
+            }
+          }
+        }
+        if (valid) store16(p.out, p.out_dtype, at + 16 * i, o);
+      }
+      tc_fence_before();  // O is read before the next item's first product overwrites it
+    }
   }
+  if (failed && p.err) atomicOr(reinterpret_cast<unsigned int*>(p.err), SLMT_DEVERR_TIMEOUT);
+  __syncthreads();
+  if (warp == 8) tmem_dealloc(tmem, kTmemCols);
+}
+
+// Tensor map of rows [tokens, heads, D] of a 16-bit type: the box is 64 dims
+// (a 128-byte swizzled panel; dims past D read as zero) of box_heads heads of
+// box_tokens tokens.
+bool encode_rows(CUtensorMap* m, const void* base, bool bf16, int64_t d, int64_t heads, int64_t tokens,
+                 int64_t head_stride, int64_t token_stride, int box_heads, int box_tokens) {
+  auto enc = tensor_map_encoder();
+  if (!enc) return false;
+  if (heads == 1) head_stride = d;  // not used
+  if (tokens == 1) token_stride = d;
+  const cuuint64_t dims[3] = {(cuuint64_t)d, (cuuint64_t)heads, (cuuint64_t)tokens};
+  const cuuint64_t strides[2] = {(cuuint64_t)(2 * head_stride), (cuuint64_t)(2 * token_stride)};
+  const cuuint32_t box[3] = {64, (cuuint32_t)box_heads, (cuuint32_t)box_tokens};
+  const cuuint32_t one[3] = {1, 1, 1};
+  return enc(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(base),
+             dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int D, bool BF16>
+int prompt_launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const PromptParams& p, int grid,
+                  cudaStream_t st) {
+  // per device: the attribute belongs to the device's context
+  if (cudaFuncSetAttribute(prompt_kernel<D, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           PromptGeom<D>::SMEM) != cudaSuccess)
+    {
+    launch_status();  // clears it
+    return SLMT_ERR_CUDA;
+  }
+  prompt_kernel<D, BF16><<<grid, kThreads, PromptGeom<D>::SMEM, st>>>(mq, mk, mv, p);
+  return launch_status();
 }
 
 }  // namespace
@@ -108,20 +582,67 @@ extern "C" int slmt_prompt_attention(const void* q, int64_t q_token_stride, int6
   if (num_reqs == 0 || max_query_len == 0 || num_tokens == 0) return SLMT_OK;
   if (!q || !k || !v || !out || !query_start_loc) return SLMT_ERR_NULL;
   if (rows_overlap(num_tokens, num_q_heads, out_token_stride, out_head_stride)) return SLMT_ERR_SHAPE;
+  // the tiled copies: 16-byte aligned rows, strides positive and below 2^40 bytes
   const uintptr_t any = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) |
                         reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(out);
   if (any % 16 != 0) return SLMT_ERR_ALIGN;
-  if ((q_token_stride | q_head_stride | k_token_stride | k_head_stride | v_token_stride | v_head_stride) % 8 != 0)
+  for (const int64_t s : {q_token_stride, k_token_stride, v_token_stride})
+    if (num_tokens > 1 && (s % 8 != 0 || s <= 0 || s >= (1ll << 39))) return SLMT_ERR_ALIGN;
+  if (num_q_heads > 1 && (q_head_stride % 8 != 0 || q_head_stride <= 0 || q_head_stride >= (1ll << 39)))
     return SLMT_ERR_ALIGN;
-  if ((out_token_stride | out_head_stride) % (out_dtype == SLMT_DTYPE_F32 ? 4 : 8) != 0) return SLMT_ERR_ALIGN;
-  PromptParams p = {q, k, v, out, query_start_loc, seq_lens, err_flag, q_token_stride, q_head_stride,
-                    k_token_stride, k_head_stride, v_token_stride, v_head_stride, out_token_stride, out_head_stride,
-                    sm_scale, (int)num_tokens, (int)num_reqs, (int)std::min<int64_t>(max_query_len, num_tokens),
-                    (int)num_q_heads, (int)num_kv_heads, dtype == SLMT_DTYPE_BF16, out_dtype};
-  const dim3 grid((unsigned)(((int64_t)p.max_query * p.hq + 3) / 4), (unsigned)num_reqs);
+  for (const int64_t s : {k_head_stride, v_head_stride})
+    if (num_kv_heads > 1 && (s % 8 != 0 || s <= 0 || s >= (1ll << 39))) return SLMT_ERR_ALIGN;
+  const int out_unit = out_dtype == SLMT_DTYPE_F32 ? 4 : 8;
+  if ((num_tokens > 1 && out_token_stride % out_unit != 0) || (num_q_heads > 1 && out_head_stride % out_unit != 0))
+    return SLMT_ERR_ALIGN;
+
+  const bool bf16 = dtype == SLMT_DTYPE_BF16;
+  const int group = (int)(num_q_heads / num_kv_heads);
+  const int tile_tokens = 128 / group;
+  const int64_t max_query = std::min(max_query_len, num_tokens);
+  if ((max_query + 2 * tile_tokens - 1) / (2 * tile_tokens) >= (1 << (32 - kReqBits))) return SLMT_ERR_UNSUPPORTED;
+  CUtensorMap mq, mk, mv;
+  if (!encode_rows(&mq, q, bf16, head_dim, num_q_heads, num_tokens, q_head_stride, q_token_stride, group,
+                   tile_tokens) ||
+      !encode_rows(&mk, k, bf16, head_dim, num_kv_heads, num_tokens, k_head_stride, k_token_stride, 1, 128) ||
+      !encode_rows(&mv, v, bf16, head_dim, num_kv_heads, num_tokens, v_head_stride, v_token_stride, 1, 128))
+    return SLMT_ERR_CUDA;
+  PromptParams p;
+  p.v = v;
+  p.out = out;
+  p.err = err_flag;
+  p.v_tok = v_token_stride, p.v_head = v_head_stride;
+  p.o_tok = out_token_stride, p.o_head = out_head_stride;
+  p.wait_limit_ns = wait_limit_ns();
+  p.scale_log2 = sm_scale * 1.4426950408889634f;
+  p.num_tokens = (int)num_tokens;
+  p.max_query = (int)max_query;
+  p.kv = (int)num_kv_heads;
+  p.group = group;
+  p.tile_tokens = tile_tokens;
+  p.out_dtype = out_dtype;
+  int dev = 0;
+  const int sms = current_device_sms(&dev);
+  if (sms <= 0) return SLMT_ERR_CUDA;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (head_dim == 64) prompt_simple_kernel<64><<<grid, 128, 0, st>>>(p);
-  else if (head_dim == 80) prompt_simple_kernel<80><<<grid, 128, 0, st>>>(p);
-  else prompt_simple_kernel<128><<<grid, 128, 0, st>>>(p);
-  return launch_status();
+  for (int64_t r = 0; r < num_reqs; r += kMaxReqs) {
+    const int64_t nr = std::min<int64_t>(kMaxReqs, num_reqs - r);
+    p.qsl = query_start_loc + r;
+    p.seq_lens = seq_lens ? seq_lens + r : nullptr;
+    p.num_reqs = (int)nr;
+    // no more CTAs than there can be items
+    const int64_t pairs = std::min(nr * ((max_query + 2 * tile_tokens - 1) / (2 * tile_tokens)),
+                                   num_tokens / (2 * tile_tokens) + nr);
+    const int grid = (int)std::min<int64_t>(sms, pairs * num_kv_heads);
+    int rc;
+    if (head_dim == 64)
+      rc = bf16 ? prompt_launch<64, true>(mq, mk, mv, p, grid, st) : prompt_launch<64, false>(mq, mk, mv, p, grid, st);
+    else if (head_dim == 80)
+      rc = bf16 ? prompt_launch<80, true>(mq, mk, mv, p, grid, st) : prompt_launch<80, false>(mq, mk, mv, p, grid, st);
+    else
+      rc = bf16 ? prompt_launch<128, true>(mq, mk, mv, p, grid, st)
+                : prompt_launch<128, false>(mq, mk, mv, p, grid, st);
+    if (rc != SLMT_OK) return rc;
+  }
+  return SLMT_OK;
 }
