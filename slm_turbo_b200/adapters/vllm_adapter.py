@@ -22,10 +22,11 @@ What changes:
   across requests, and a continuation chunk (chunked prefill, prefix cache)
   or a decode row in a mixed batch never sees its cached prefix.  Here each
   request is handled on its own: a request whose tokens are all new (no
-  cached context) gets causal attention over its own raw K/V, exactly the
-  reference's first-chunk computation; every other query token attends to
-  its request's packed cache through the block table (positions 0..its
-  own), with the same kernel as decode.  All of it stays on the device.
+  cached context) gets causal attention over its own raw K/V, the
+  reference's first-chunk computation, all such requests of the step in one
+  ``kv_prompt_attention`` launch; every other query token attends to its
+  request's packed cache through the block table (positions 0..its own).
+  All of it stays on the device.
 * The impl's ``scale`` is honoured in decode too (the reference kernel hard
   codes 1/sqrt(head_size), kernels/kv_dequant_kernels.cuh:703; the two agree
   for the usual models).
@@ -138,7 +139,8 @@ class _ErrorWatch:
                 logger.error("slm-turbo kernels set device error bits 0x%x", bits)
                 raise RuntimeError(f"slm-turbo kernels reported device error bits 0x{bits:x} "
                                    "(1 bad block id, 2 slot beyond the cache, 4 wait timeout, "
-                                   "8 length above the block table, 16 unexpected CTA placement)")
+                                   "8 length above the block table, 16 unexpected CTA placement, "
+                                   "32 too few free blocks)")
         self.host.copy_(_lib.error_word(self.device), non_blocking=True)
         if self.event is None:
             self.event = torch.cuda.Event()
@@ -203,6 +205,13 @@ def _register_custom_backend() -> bool:
             raise RuntimeError(f"slm-turbo 4-bit KV kernels unavailable in this process: "
                                f"{self._slm_kernel_err}")
 
+        def _prompt_kernel_takes(self, query, key):
+            """Whether fresh prompts go to kv_prompt_attention (the packed cache
+            takes the same types); anything else is left to SDPA."""
+            return (self._slm_kernel and query.is_cuda and query.dtype in (torch.float16, torch.bfloat16)
+                    and key.dtype == query.dtype and self.scale > 0 and query.shape[1] <= 128 * key.shape[1]
+                    and not (torch.is_grad_enabled() and query.requires_grad))
+
         def do_kv_cache_update(self, layer, key, value, kv_cache, slot_mapping):
             """Quantize the batch's K/V into their packed slots (ref :185-203)."""
             if kv_cache is None or kv_cache.numel() == 0:
@@ -250,26 +259,37 @@ def _register_custom_backend() -> bool:
             qsl = [min(x, n) for x in attn_metadata.query_start_loc[:nreq + 1].tolist()]
             seq_lens = attn_metadata.seq_lens[:nreq].tolist()
             hk = key.shape[1]
-            kernel_lens, longest = [], 0
+            kernel_lens, longest = [], 0  # requests with cached tokens: lengths, and the most rows
+            fresh_lens, longest_fresh = [], 0  # the others: rows
             for r in range(nreq):
                 a, b = qsl[r], qsl[r + 1]
                 ctx = seq_lens[r] - (b - a)
-                if b > a and ctx > 0:  # rows a..b-1 are the last b-a of seq_lens[r] cached tokens
-                    kernel_lens.append(seq_lens[r])
+                cached = b > a and ctx > 0  # rows a..b-1 are the last b-a of seq_lens[r] cached tokens
+                kernel_lens.append(seq_lens[r] if cached else 0)  # length 0: the paged kernel skips it
+                fresh_lens.append(-1 if cached else b - a)        # not its rows: the prompt kernel skips it
+                if cached:
                     longest = max(longest, b - a)
-                else:  # nothing cached before this chunk (or no rows): length 0, the kernel skips it
-                    kernel_lens.append(0)
+                else:
+                    longest_fresh = max(longest_fresh, b - a)
+            own = longest_fresh > 0 and self._prompt_kernel_takes(query, key)
+            if longest or own:
+                meta = torch.tensor(qsl + kernel_lens + fresh_lens, dtype=torch.int32).to(query.device,
+                                                                                          non_blocking=True)
+                starts, cached_lens, own_lens = meta[:nreq + 1], meta[nreq + 1:2 * nreq + 1], meta[2 * nreq + 1:]
             if longest:
-                dev = query.device
                 self._slm_prefill(
-                    query, kv_cache, attn_metadata.block_table[:nreq],
-                    torch.tensor(qsl, dtype=torch.int32).to(dev, non_blocking=True),
-                    torch.tensor(kernel_lens, dtype=torch.int32).to(dev, non_blocking=True), longest,
+                    query, kv_cache, attn_metadata.block_table[:nreq], starts, cached_lens, longest,
                     block_size=kv_cache.shape[1], num_kv_heads=kv_cache.shape[2], out=out, sm_scale=self.scale)
                 _KERNEL_CALLS += 1
+            if own:  # all requests whose tokens are all new: causal over their own rows
+                from slm_turbo_b200.kernels.kv_dequant import kv_prompt_attention
+                kv_prompt_attention(query, key, value, starts, longest_fresh, seq_lens=own_lens, out=out,
+                                    sm_scale=self.scale)
+                _KERNEL_CALLS += 1
+                return out
             for r in range(nreq):
                 a, b = qsl[r], qsl[r + 1]
-                if b > a and kernel_lens[r] == 0:  # all of this request's tokens are new: causal over them
+                if b > a and kernel_lens[r] == 0:
                     o = torch.nn.functional.scaled_dot_product_attention(
                         query[a:b].transpose(0, 1).unsqueeze(0), key[a:b].transpose(0, 1).unsqueeze(0),
                         value[a:b].transpose(0, 1).unsqueeze(0), is_causal=True, scale=self.scale,
@@ -280,8 +300,8 @@ def _register_custom_backend() -> bool:
         def _prefill_attention_device(self, query, key, value, kv_cache, attn_metadata, out):
             """The same computation with no host read (used under CUDA graph
             capture): every token is a pseudo-sequence of the packed-cache
-            kernel (length 0 for requests without cached context), and a
-            block-diagonal causal SDPA over the raw K/V covers the others."""
+            kernel (length 0 for requests without cached context), and the
+            prompt kernel covers the others over their raw K/V."""
             global _KERNEL_CALLS
             n, hq, d = query.shape
             dev = query.device
@@ -300,6 +320,14 @@ def _register_custom_backend() -> bool:
                 query, kv_cache, bt, vlen, block_size=kv_cache.shape[1], num_kv_heads=kv_cache.shape[2],
                 out=out, sm_scale=self.scale, max_seq_len=None)
             _KERNEL_CALLS += 1
+            if self._prompt_kernel_takes(query, key):
+                from slm_turbo_b200.kernels.kv_dequant import kv_prompt_attention
+                rows = qsl[1:] - qsl[:-1]
+                own_lens = torch.where(ctx <= 0, rows, torch.full_like(rows, -1))
+                kv_prompt_attention(query, key, value, qsl.clamp(max=n), n, seq_lens=own_lens, out=out,
+                                    sm_scale=self.scale)
+                _KERNEL_CALLS += 1
+                return out
             raw = self._first_chunk_attention(query, key, value, req)
             out.copy_(torch.where(first.view(n, 1, 1), raw.to(out.dtype), out))
             return out
