@@ -206,49 +206,88 @@ struct Vec8<float> {
   }
 };
 
+// A thread keeps its place in a token's slots (head, K or V, piece) and walks
+// over tokens, four at a time so that their slot ids and code words are in
+// flight together; places are found once, with 32-bit arithmetic.
+constexpr int kLoadThreads = 256;
+constexpr int kLoadUnroll = 4;
+
 template <int D, typename T>
-__global__ void __launch_bounds__(256) load_kernel(const uint8_t* __restrict__ cache, int64_t num_slots,
-                                                   const int64_t* __restrict__ slot_mapping, int64_t rows, int kv,
-                                                   T* __restrict__ key, T* __restrict__ value, int32_t* err) {
+__global__ void __launch_bounds__(kLoadThreads)
+    load_kernel(const uint8_t* __restrict__ cache, int64_t num_slots, const int64_t* __restrict__ slot_mapping,
+                int64_t num_tokens, int kv, int places, int sub_tokens, T* __restrict__ key, T* __restrict__ value,
+                int32_t* err) {
   constexpr int PIECES = D / 4;  // 8-value pieces of a row's K and V
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t row = i / PIECES;
-  if (row >= rows) return;
-  const int piece = (int)(i - row * PIECES);
-  const int64_t tok = row / kv;
-  const int h = (int)(row - tok * kv);
+  // `places` pieces of a token in this block's pass (kv * PIECES when a block
+  // holds whole tokens, sub_tokens of them; else a part, by blockIdx.y)
+  const int sub = threadIdx.x / places;
+  const int place = threadIdx.x - sub * places + blockIdx.y * kLoadThreads;
+  if (sub >= sub_tokens || place >= kv * PIECES) return;
+  const int h = place / PIECES, piece = place - h * PIECES;
   const int which = piece >= PIECES / 2, c = piece - which * (PIECES / 2);
-  const int64_t slot = slot_mapping[tok];
-  float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  if (slot >= 0 && slot < num_slots) {
-    const uint8_t* s = cache + (slot * kv + h) * (D + 8);
-    const uint32_t codes = *reinterpret_cast<const uint32_t*>(s + which * (D / 2) + 4 * c);
-    const uint32_t rulers = *reinterpret_cast<const uint32_t*>(s + D + 4 * which);
-    const float mn = half_bits_to_float((uint16_t)(rulers & 0xFFFFu)), st = half_bits_to_float((uint16_t)(rulers >> 16));
+  const int64_t slot_bytes = (int64_t)kv * (D + 8);
+  const uint8_t* base = cache + (int64_t)h * (D + 8);
+  const int code_at = which * (D / 2) + 4 * c, ruler_at = D + 4 * which;
+  T* out = (which ? value : key) + (int64_t)h * D + 8 * c;
+  const int64_t t0 = (int64_t)blockIdx.x * (sub_tokens * kLoadUnroll) + sub;
+  int64_t slot[kLoadUnroll];
+  uint32_t codes[kLoadUnroll], rulers[kLoadUnroll];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = __fmaf_rn((float)((codes >> (4 * j)) & 15u), st, mn);
-  } else if (slot >= num_slots && piece == 0 && h == 0) {
-    set_error(err, SLMT_DEVERR_SLOT);
+  for (int u = 0; u < kLoadUnroll; ++u) {
+    const int64_t t = t0 + u * sub_tokens;
+    slot[u] = t < num_tokens ? slot_mapping[t] : -1;
   }
-  Vec8<T>::store((which ? value : key) + row * D + 8 * c, x);
+#pragma unroll
+  for (int u = 0; u < kLoadUnroll; ++u) {
+    codes[u] = rulers[u] = 0u;  // code 0, min 0: a row of zeros
+    if (slot[u] >= 0 && slot[u] < num_slots) {
+      const uint8_t* s = base + slot[u] * slot_bytes;
+      codes[u] = *reinterpret_cast<const uint32_t*>(s + code_at);
+      rulers[u] = *reinterpret_cast<const uint32_t*>(s + ruler_at);
+    } else if (slot[u] >= num_slots && place == 0) {
+      set_error(err, SLMT_DEVERR_SLOT);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kLoadUnroll; ++u) {
+    const int64_t t = t0 + u * sub_tokens;
+    if (t >= num_tokens) return;
+    const float mn = half_bits_to_float((uint16_t)(rulers[u] & 0xFFFFu));
+    const float st = half_bits_to_float((uint16_t)(rulers[u] >> 16));
+    float x[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      // 2^23 + code has the code in its low mantissa bits: code as a float
+      // without the slower integer conversion
+      const float code = __uint_as_float(((codes[u] >> (4 * j)) & 15u) | 0x4B000000u) - 8388608.f;
+      x[j] = __fmaf_rn(code, st, mn);
+    }
+    Vec8<T>::store(out + t * kv * D, x);
+  }
+}
+
+template <int D, typename T>
+int load_launch_typed(const uint8_t* cache, int64_t num_slots, const int64_t* slot_mapping, int64_t tokens, int kv,
+                      void* key, void* value, int32_t* err, cudaStream_t st) {
+  const int64_t all = (int64_t)kv * (D / 4);  // pieces of a token
+  const int places = (int)std::min<int64_t>(all, kLoadThreads);
+  const int sub_tokens = kLoadThreads / places;
+  const int64_t parts = (all + kLoadThreads - 1) / kLoadThreads;
+  const int64_t per_block = (int64_t)sub_tokens * kLoadUnroll, blocks = (tokens + per_block - 1) / per_block;
+  if (blocks > INT32_MAX || parts > 65535) return SLMT_ERR_UNSUPPORTED;
+  load_kernel<D, T><<<dim3((unsigned)blocks, (unsigned)parts), kLoadThreads, 0, st>>>(
+      cache, num_slots, slot_mapping, tokens, kv, places, sub_tokens, (T*)key, (T*)value, err);
+  return launch_status();
 }
 
 template <int D>
-int load_launch(const uint8_t* cache, int64_t num_slots, const int64_t* slot_mapping, int64_t rows, int kv, void* key,
-                void* value, int dtype, int32_t* err, cudaStream_t st) {
-  const int64_t blocks = (rows * (D / 4) + 255) / 256;
-  if (blocks > INT32_MAX) return SLMT_ERR_UNSUPPORTED;
-  const dim3 grid((unsigned)blocks);
+int load_launch(const uint8_t* cache, int64_t num_slots, const int64_t* slot_mapping, int64_t tokens, int kv,
+                void* key, void* value, int dtype, int32_t* err, cudaStream_t st) {
   if (dtype == SLMT_DTYPE_F16)
-    load_kernel<D, __half><<<grid, 256, 0, st>>>(cache, num_slots, slot_mapping, rows, kv, (__half*)key,
-                                                 (__half*)value, err);
-  else if (dtype == SLMT_DTYPE_BF16)
-    load_kernel<D, __nv_bfloat16><<<grid, 256, 0, st>>>(cache, num_slots, slot_mapping, rows, kv,
-                                                        (__nv_bfloat16*)key, (__nv_bfloat16*)value, err);
-  else
-    load_kernel<D, float><<<grid, 256, 0, st>>>(cache, num_slots, slot_mapping, rows, kv, (float*)key, (float*)value,
-                                                err);
-  return launch_status();
+    return load_launch_typed<D, __half>(cache, num_slots, slot_mapping, tokens, kv, key, value, err, st);
+  if (dtype == SLMT_DTYPE_BF16)
+    return load_launch_typed<D, __nv_bfloat16>(cache, num_slots, slot_mapping, tokens, kv, key, value, err, st);
+  return load_launch_typed<D, float>(cache, num_slots, slot_mapping, tokens, kv, key, value, err, st);
 }
 
 }  // namespace
@@ -309,15 +348,15 @@ extern "C" int slmt_kv_dequantize_load(const uint8_t* kv_cache, int64_t num_bloc
   if (reinterpret_cast<uintptr_t>(kv_cache) % 8 != 0 || reinterpret_cast<uintptr_t>(key) % 16 != 0 ||
       reinterpret_cast<uintptr_t>(value) % 16 != 0)
     return SLMT_ERR_ALIGN;
-  const int64_t slots = num_blocks * block_size, rows = num_tokens * num_kv_heads;
+  const int64_t slots = num_blocks * block_size;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const int kv = (int)num_kv_heads;
   switch (head_dim) {
     case 64:
-      return load_launch<64>(kv_cache, slots, slot_mapping, rows, kv, key, value, out_dtype, err_flag, st);
+      return load_launch<64>(kv_cache, slots, slot_mapping, num_tokens, kv, key, value, out_dtype, err_flag, st);
     case 80:
-      return load_launch<80>(kv_cache, slots, slot_mapping, rows, kv, key, value, out_dtype, err_flag, st);
+      return load_launch<80>(kv_cache, slots, slot_mapping, num_tokens, kv, key, value, out_dtype, err_flag, st);
     default:
-      return load_launch<128>(kv_cache, slots, slot_mapping, rows, kv, key, value, out_dtype, err_flag, st);
+      return load_launch<128>(kv_cache, slots, slot_mapping, num_tokens, kv, key, value, out_dtype, err_flag, st);
   }
 }

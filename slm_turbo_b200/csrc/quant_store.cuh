@@ -26,6 +26,27 @@ struct SlotRow {
   uint2 rulers;     // (k_min | k_step << 16, v_min | v_step << 16), fp16 bits
 };
 
+// The parts of the quantizer, for rows that lie across lanes in another way:
+// minimum and step of a row, a value's code, and the two fp16 rulers.
+struct SlotScale {
+  float mn, step;
+};
+__device__ __forceinline__ SlotScale slot_scale(float mn, float mx) {
+  SlotScale s;
+  s.mn = mn;
+  s.step = __fdiv_rn(mx - mn, 15.0f);
+  if (!(s.step > 0.0f)) s.step = 1.0f;  // constant row guard (ref .cuh:854)
+  return s;
+}
+__device__ __forceinline__ uint32_t slot_code(float x, const SlotScale& s) {
+  const int q = (int)__fadd_rn(__fdiv_rn(__fsub_rn(x, s.mn), s.step), 0.5f);
+  return (uint32_t)(q < 0 ? 0 : (q > 15 ? 15 : q));
+}
+__device__ __forceinline__ uint32_t slot_rulers(const SlotScale& s) {
+  return (uint32_t)__half_as_ushort(__float2half_rn(s.mn)) |
+         ((uint32_t)__half_as_ushort(__float2half_rn(s.step)) << 16);
+}
+
 // Quantize a row whose VEC values per lane are in xk / xv (lanes >= LANES
 // hold zeros and take no part in the min/max).
 template <int D>

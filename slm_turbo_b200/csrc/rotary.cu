@@ -20,7 +20,7 @@ namespace slmt {
 namespace {
 
 constexpr int kRotThreads = 256;
-constexpr int kRotTokens = 4;  // tokens of one CTA
+constexpr int kRotRows = 4;  // rows of a thread in flight
 
 struct RotaryParams {
   const void* q;
@@ -39,11 +39,6 @@ struct RotaryParams {
   int num_tokens, hq, kv, half, interleaved, pos_i64, bf16;
 };
 
-__device__ __forceinline__ float load16(const void* p, int64_t i, int bf16) {
-  return bf16 ? __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p)[i])
-              : __half2float(reinterpret_cast<const __half*>(p)[i]);
-}
-
 // cos and sin of p * f, in turns: the product is exact in 64 bits, its whole
 // turns are taken off with the rest of the multiplication by 1/(2 pi) kept.
 __device__ __forceinline__ float2 turn(int64_t pos, float f) {
@@ -56,92 +51,252 @@ __device__ __forceinline__ float2 turn(int64_t pos, float f) {
   return make_float2((float)c, (float)s);
 }
 
-template <int D>
+// How a thread's 8 dims of a row lie.
+enum RotaryLayout {
+  ROT_HALF = 0,         // 4 pairs as dims 4i.. and rot/2 + 4i.., or 8 dims past rot: half % 4 == 0, aligned rows
+  ROT_INTERLEAVED = 1,  // 4 pairs, 8 dims next to one another, aligned rows
+  ROT_ANY = 2           // 8 dims next to one another, partners fetched one by one
+};
+
+__device__ __forceinline__ float from16(uint32_t bits, int bf16) {
+  return bf16 ? __bfloat162float(__ushort_as_bfloat16((uint16_t)bits)) : __half2float(__ushort_as_half((uint16_t)bits));
+}
+__device__ __forceinline__ uint32_t to16(float x, int bf16) {
+  return bf16 ? (uint32_t)__bfloat16_as_ushort(__float2bfloat16_rn(x)) : (uint32_t)__half_as_ushort(__float2half_rn(x));
+}
+
+// One CTA per token: D / 8 lanes to a row (D 80: 10 of 16), so a thread's
+// pairs are the same in every row and their cos and sin stay in registers.
+// The rows' loads are issued before the CTA works out the token's angles (64
+// double-precision sincos at most, a thread each), which hides one behind the
+// other.
+template <int D, int LAYOUT, bool STORE>
 __global__ void __launch_bounds__(kRotThreads) rotary_kernel(const RotaryParams p) {
-  constexpr int VEC = SlotGeom<D>::VEC;
-  __shared__ float2 s_cs[kRotTokens][D / 2];
-  const int t0 = blockIdx.x * kRotTokens;
-  const int nt = min(kRotTokens, p.num_tokens - t0);
-  for (int i = threadIdx.x; i < nt * p.half; i += kRotThreads) {
-    const int t = i / p.half, f = i - t * p.half;
-    const int64_t pos = p.pos_i64 ? reinterpret_cast<const int64_t*>(p.positions)[t0 + t]
-                                  : (int64_t) reinterpret_cast<const int32_t*>(p.positions)[t0 + t];
-    const float2 cs = turn(pos, p.inv_freq[f]);
-    s_cs[t][f] = make_float2(__fmul_rn(cs.x, p.scaling), __fmul_rn(cs.y, p.scaling));
+  constexpr int ACTIVE = D / 8, LANES = D == 64 ? 8 : 16, SLOTS = kRotThreads / LANES;
+  constexpr int ROWS = LAYOUT == ROT_ANY ? 1 : kRotRows;
+  __shared__ float2 s_cs[D / 2];
+  const int64_t tok = blockIdx.x;
+  const int li = threadIdx.x % LANES, slot0 = threadIdx.x / LANES;
+  const bool act = li < ACTIVE;
+  const int heads = p.hq + p.kv, half = p.half;
+  // dims of the thread: 4 from d0 on and 4 from d1 on; pairs from pair0 on
+  int d0 = 8 * li, d1 = d0 + 4, pair0 = 4 * li;
+  bool turns = false;  // HALF: all 4 pairs turn, or none
+  if (LAYOUT == ROT_HALF) {
+    turns = li < half / 4;
+    d0 = turns ? 4 * li : 2 * half + 8 * (li - half / 4);
+    d1 = turns ? half + 4 * li : d0 + 4;
   }
-  __syncthreads();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int heads = p.hq + p.kv;
-  for (int row = warp; row < nt * heads; row += kRotThreads / 32) {
-    const int t = row / heads, h = row - t * heads;
-    const int64_t tok = t0 + t;
-    const bool is_k = h >= p.hq;
-    const int hh = is_k ? h - p.hq : h;
-    const int64_t in = is_k ? tok * p.k_tok + hh * p.k_head : tok * p.q_tok + hh * p.q_head;
-    const void* src = is_k ? p.k : p.q;
-    float y[VEC];
-    const bool act = lane < SlotGeom<D>::LANES;
+  float2 cs[4];
+  const uint16_t* q = reinterpret_cast<const uint16_t*>(p.q);
+  const uint16_t* k = reinterpret_cast<const uint16_t*>(p.k);
+  const uint16_t* v = reinterpret_cast<const uint16_t*>(p.v);
+  int64_t cache_slot = -1;
+  if (STORE) {
+    cache_slot = p.slot_mapping[tok];
+    if (cache_slot >= p.num_slots) {
+      if (threadIdx.x == 0 && p.err) atomicOr(reinterpret_cast<unsigned int*>(p.err), SLMT_DEVERR_SLOT);
+      cache_slot = -1;
+    }
+  }
+  bool first = true;
+  for (int h0 = 0; h0 < heads; h0 += SLOTS * ROWS) {
+    uint2 lo[ROWS], hi[ROWS], vlo[ROWS], vhi[ROWS];
+    float other[8];  // ROT_ANY: the partners
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      const int i = lane * VEC + j;
-      y[j] = 0.f;
-      if (act) {
-        const float x = load16(src, in + i, p.bf16);
-        y[j] = x;
-        if (i < 2 * p.half) {
-          bool second;
-          int pair, other;
-          if (p.interleaved) {
-            second = i & 1, pair = i >> 1, other = i ^ 1;
-          } else {
-            second = i >= p.half, pair = second ? i - p.half : i, other = second ? i - p.half : i + p.half;
-          }
-          const float o = load16(src, in + other, p.bf16);
-          const float2 cs = s_cs[t][pair];
-          const float a = __fmul_rn(x, cs.x), b = __fmul_rn(o, cs.y);
-          y[j] = second ? __fadd_rn(a, b) : __fsub_rn(a, b);
+    for (int r = 0; r < ROWS; ++r) {
+      const int h = h0 + slot0 + r * SLOTS;
+      lo[r] = hi[r] = vlo[r] = vhi[r] = make_uint2(0u, 0u);
+      if (!act || h >= heads) continue;
+      const bool is_k = h >= p.hq;
+      const uint16_t* row = is_k ? k + tok * p.k_tok + (int64_t)(h - p.hq) * p.k_head
+                                 : q + tok * p.q_tok + (int64_t)h * p.q_head;
+      if (LAYOUT == ROT_HALF) {
+        lo[r] = *reinterpret_cast<const uint2*>(row + d0);
+        hi[r] = *reinterpret_cast<const uint2*>(row + d1);
+      } else if (LAYOUT == ROT_INTERLEAVED) {
+        const uint4 x = *reinterpret_cast<const uint4*>(row + d0);
+        lo[r] = make_uint2(x.x, x.y), hi[r] = make_uint2(x.z, x.w);
+      } else {
+        uint32_t e[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int i = d0 + j;
+          e[j] = row[i];
+          int o = i;
+          if (i < 2 * half) o = p.interleaved ? i ^ 1 : (i < half ? i + half : i - half);
+          other[j] = from16(row[o], p.bf16);
         }
-        y[j] = p.bf16 ? __bfloat162float(__float2bfloat16_rn(y[j])) : __half2float(__float2half_rn(y[j]));
+        lo[r] = make_uint2(e[0] | e[1] << 16, e[2] | e[3] << 16);
+        hi[r] = make_uint2(e[4] | e[5] << 16, e[6] | e[7] << 16);
+      }
+      if (STORE && is_k && cache_slot >= 0) {
+        const uint16_t* vr = v + tok * p.v_tok + (int64_t)(h - p.hq) * p.v_head;
+        if (LAYOUT == ROT_HALF) {
+          vlo[r] = *reinterpret_cast<const uint2*>(vr + d0);
+          vhi[r] = *reinterpret_cast<const uint2*>(vr + d1);
+        } else if (LAYOUT == ROT_INTERLEAVED) {
+          const uint4 x = *reinterpret_cast<const uint4*>(vr + d0);
+          vlo[r] = make_uint2(x.x, x.y), vhi[r] = make_uint2(x.z, x.w);
+        } else {
+          vlo[r] = make_uint2(vr[d0] | (uint32_t)vr[d0 + 1] << 16, vr[d0 + 2] | (uint32_t)vr[d0 + 3] << 16);
+          vhi[r] = make_uint2(vr[d1] | (uint32_t)vr[d1 + 1] << 16, vr[d1 + 2] | (uint32_t)vr[d1 + 3] << 16);
+        }
       }
     }
-    __syncwarp();  // in place: the whole row is read before any of it is written
-    void* dst = is_k ? p.k_out : p.q_out;
-    if (dst && act) {
-      const int64_t out = is_k ? tok * p.ko_tok + hh * p.ko_head : tok * p.qo_tok + hh * p.qo_head;
+    if (first) {
+      for (int i = threadIdx.x; i < half; i += kRotThreads) {
+        const int64_t pos = p.pos_i64 ? reinterpret_cast<const int64_t*>(p.positions)[tok]
+                                      : (int64_t) reinterpret_cast<const int32_t*>(p.positions)[tok];
+        const float2 t = turn(pos, p.inv_freq[i]);
+        s_cs[i] = make_float2(__fmul_rn(t.x, p.scaling), __fmul_rn(t.y, p.scaling));
+      }
+    }
+    // the angles; and, where partners are other threads' dims, every row is
+    // read before any of it is written (in-place calls)
+    if (first || LAYOUT == ROT_ANY) __syncthreads();
+    if (first && LAYOUT != ROT_ANY) {
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        if (p.bf16) reinterpret_cast<__nv_bfloat16*>(dst)[out + lane * VEC + j] = __float2bfloat16_rn(y[j]);
-        else reinterpret_cast<__half*>(dst)[out + lane * VEC + j] = __float2half_rn(y[j]);
+      for (int j = 0; j < 4; ++j) {
+        const bool on = act && (LAYOUT == ROT_HALF ? turns : pair0 + j < half);
+        cs[j] = on ? s_cs[pair0 + j] : make_float2(0.f, 0.f);
       }
     }
-    if (is_k && p.cache) {
-      const int64_t slot = p.slot_mapping[tok];
-      if (slot >= p.num_slots) {
-        if (lane == 0 && p.err) atomicOr(reinterpret_cast<unsigned int*>(p.err), SLMT_DEVERR_SLOT);
-      } else if (slot >= 0) {
-        float xv[VEC];
-        const size_t esz = 2;
-        load_row_vals<D>(reinterpret_cast<const uint8_t*>(p.v) + (tok * p.v_tok + hh * p.v_head) * esz, p.bf16, xv);
-        const SlotRow r = quantize_slot_vals<D>(y, xv);
-        write_slot_row<D>(p.cache + (slot * p.kv + hh) * (D + 8), r);
+    first = false;
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+      const int h = h0 + slot0 + r * SLOTS;
+      const bool live = act && h < heads;
+      const bool is_k = h >= p.hq;
+      // x: dims d0..d0+3, d1..d1+3
+      float x[8];
+      const uint32_t w[4] = {lo[r].x, lo[r].y, hi[r].x, hi[r].y};
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = from16(j & 1 ? w[j >> 1] >> 16 : w[j >> 1] & 0xFFFFu, p.bf16);
+      uint32_t y[8];
+      if (LAYOUT == ROT_HALF) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float a = x[j], b = x[4 + j];
+          y[j] = to16(turns ? __fsub_rn(__fmul_rn(a, cs[j].x), __fmul_rn(b, cs[j].y)) : a, p.bf16);
+          y[4 + j] = to16(turns ? __fadd_rn(__fmul_rn(b, cs[j].x), __fmul_rn(a, cs[j].y)) : b, p.bf16);
+        }
+      } else if (LAYOUT == ROT_INTERLEAVED) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float a = x[2 * j], b = x[2 * j + 1];
+          const bool on = pair0 + j < half;
+          y[2 * j] = to16(on ? __fsub_rn(__fmul_rn(a, cs[j].x), __fmul_rn(b, cs[j].y)) : a, p.bf16);
+          y[2 * j + 1] = to16(on ? __fadd_rn(__fmul_rn(b, cs[j].x), __fmul_rn(a, cs[j].y)) : b, p.bf16);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int i = d0 + j;
+          float z = x[j];
+          if (live && i < 2 * half) {
+            const bool second = p.interleaved ? i & 1 : i >= half;
+            const float2 t = s_cs[p.interleaved ? i >> 1 : second ? i - half : i];
+            const float a = __fmul_rn(z, t.x), b = __fmul_rn(other[j], t.y);
+            z = second ? __fadd_rn(a, b) : __fsub_rn(a, b);
+          }
+          y[j] = to16(z, p.bf16);
+        }
+      }
+      uint16_t* dst = reinterpret_cast<uint16_t*>(is_k ? p.k_out : p.q_out);
+      if (live && dst) {
+        dst += is_k ? tok * p.ko_tok + (int64_t)(h - p.hq) * p.ko_head : tok * p.qo_tok + (int64_t)h * p.qo_head;
+        const uint2 a = make_uint2(y[0] | y[1] << 16, y[2] | y[3] << 16);
+        const uint2 b = make_uint2(y[4] | y[5] << 16, y[6] | y[7] << 16);
+        if (LAYOUT == ROT_HALF) {
+          *reinterpret_cast<uint2*>(dst + d0) = a;
+          *reinterpret_cast<uint2*>(dst + d1) = b;
+        } else if (LAYOUT == ROT_INTERLEAVED) {
+          *reinterpret_cast<uint4*>(dst + d0) = make_uint4(a.x, a.y, b.x, b.y);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) dst[d0 + j] = (uint16_t)y[j];
+        }
+      }
+      // the cache: the whole warp takes part where a row of it is a k row
+      if (STORE && cache_slot >= 0 && __any_sync(0xffffffffu, h < heads && is_k)) {
+        float mn[2] = {INFINITY, INFINITY}, mx[2] = {-INFINITY, -INFINITY}, vx[8], kx[8];
+        const uint32_t vw[4] = {vlo[r].x, vlo[r].y, vhi[r].x, vhi[r].y};
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          vx[j] = from16(j & 1 ? vw[j >> 1] >> 16 : vw[j >> 1] & 0xFFFFu, p.bf16);
+          kx[j] = from16(y[j], p.bf16);
+          if (act) {
+            mn[0] = fminf(mn[0], kx[j]), mx[0] = fmaxf(mx[0], kx[j]);
+            mn[1] = fminf(mn[1], vx[j]), mx[1] = fmaxf(mx[1], vx[j]);
+          }
+        }
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            mn[i] = fminf(mn[i], __shfl_xor_sync(0xffffffffu, mn[i], o));
+            mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], o));
+          }
+        }
+        if (live && is_k) {
+          const SlotScale ks = slot_scale(mn[0], mx[0]), vs = slot_scale(mn[1], mx[1]);
+          uint32_t kc = 0u, vc = 0u;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            kc |= slot_code(kx[j], ks) << (4 * j);
+            vc |= slot_code(vx[j], vs) << (4 * j);
+          }
+          uint8_t* row = p.cache + (cache_slot * p.kv + (h - p.hq)) * (D + 8);
+          if (LAYOUT == ROT_HALF) {
+            *reinterpret_cast<uint16_t*>(row + d0 / 2) = (uint16_t)kc;
+            *reinterpret_cast<uint16_t*>(row + d1 / 2) = (uint16_t)(kc >> 16);
+            *reinterpret_cast<uint16_t*>(row + D / 2 + d0 / 2) = (uint16_t)vc;
+            *reinterpret_cast<uint16_t*>(row + D / 2 + d1 / 2) = (uint16_t)(vc >> 16);
+          } else {
+            *reinterpret_cast<uint32_t*>(row + d0 / 2) = kc;
+            *reinterpret_cast<uint32_t*>(row + D / 2 + d0 / 2) = vc;
+          }
+          if (li == 0) *reinterpret_cast<uint2*>(row + D) = make_uint2(slot_rulers(ks), slot_rulers(vs));
+        }
       }
     }
+    if (LAYOUT == ROT_ANY && h0 + SLOTS * ROWS < heads) __syncthreads();
   }
 }
 
+template <int D, bool STORE>
+int rotary_launch_d(const RotaryParams& p, int layout, cudaStream_t st) {
+  const dim3 grid((unsigned)p.num_tokens);
+  if (layout == ROT_HALF)
+    rotary_kernel<D, ROT_HALF, STORE><<<grid, kRotThreads, 0, st>>>(p);
+  else if (layout == ROT_INTERLEAVED)
+    rotary_kernel<D, ROT_INTERLEAVED, STORE><<<grid, kRotThreads, 0, st>>>(p);
+  else
+    rotary_kernel<D, ROT_ANY, STORE><<<grid, kRotThreads, 0, st>>>(p);
+  return launch_status();
+}
+
+// Whether rows at these strides can be read and written `bytes` at a time.
+bool rows_aligned(const void* base, int64_t tok, int64_t head, int64_t bytes) {
+  return reinterpret_cast<uintptr_t>(base) % bytes == 0 && (2 * tok) % bytes == 0 && (2 * head) % bytes == 0;
+}
+
 int rotary_launch(const RotaryParams& p, int64_t head_dim, cudaStream_t st) {
-  const dim3 grid((unsigned)((p.num_tokens + kRotTokens - 1) / kRotTokens));
+  const int64_t bytes = p.interleaved ? 16 : 8;
+  const bool aligned = rows_aligned(p.q, p.q_tok, p.q_head, bytes) && rows_aligned(p.k, p.k_tok, p.k_head, bytes) &&
+                       rows_aligned(p.v, p.v_tok, p.v_head, bytes) && rows_aligned(p.q_out, p.qo_tok, p.qo_head, bytes) &&
+                       rows_aligned(p.k_out, p.ko_tok, p.ko_head, bytes);
+  const int layout = !aligned ? ROT_ANY : p.interleaved ? ROT_INTERLEAVED : p.half % 4 == 0 ? ROT_HALF : ROT_ANY;
+  const bool store = p.cache != nullptr;
   switch (head_dim) {
     case 64:
-      rotary_kernel<64><<<grid, kRotThreads, 0, st>>>(p);
-      break;
+      return store ? rotary_launch_d<64, true>(p, layout, st) : rotary_launch_d<64, false>(p, layout, st);
     case 80:
-      rotary_kernel<80><<<grid, kRotThreads, 0, st>>>(p);
-      break;
+      return store ? rotary_launch_d<80, true>(p, layout, st) : rotary_launch_d<80, false>(p, layout, st);
     default:
-      rotary_kernel<128><<<grid, kRotThreads, 0, st>>>(p);
+      return store ? rotary_launch_d<128, true>(p, layout, st) : rotary_launch_d<128, false>(p, layout, st);
   }
-  return launch_status();
 }
 
 // Checks shared by both entries; SLMT_OK and *empty for a call with no rows.
