@@ -7,7 +7,6 @@ Non-zero statuses become ``RuntimeError`` (the reference surfaces its
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import threading
 from pathlib import Path
@@ -106,17 +105,12 @@ def stream_of(device: torch.device) -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
-def on_device(device: torch.device):
-    """Context in which launches go to `device`: the C entries launch on the
-    current CUDA device, which need not be the tensors' one."""
-    if device.index is None or torch.cuda.current_device() == device.index:
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
+_TAGS = {torch.float16: DT_F16, torch.bfloat16: DT_BF16, torch.float32: DT_F32,
+         torch.int32: DT_I32, torch.int64: DT_I64}
 
 
 def dtype_tag(dt: torch.dtype) -> int:
-    return {torch.float16: DT_F16, torch.bfloat16: DT_BF16, torch.float32: DT_F32,
-            torch.int32: DT_I32, torch.int64: DT_I64}.get(dt, -1)
+    return _TAGS.get(dt, -1)
 
 
 # ------------------------------------------------------------ device state
@@ -143,6 +137,8 @@ def device_state(device: torch.device) -> _DeviceState:
         _states[key] = st
     return st
 
+
+_err_ptrs: dict = {}  # device index -> address of its error word (lives as long as the process)
 
 _ws_need: dict = {}
 
@@ -171,6 +167,24 @@ def workspace(device: torch.device, num_seqs: int, hq: int, kv: int, d: int) -> 
         ws = torch.zeros(size, dtype=torch.uint8, device=st.device)
         st.workspaces[stream] = ws
     return ws
+
+
+def call_on(index: int, fn, *args) -> int:
+    """Status of the C entry ``fn(*args, stream)`` on device `index` and its
+    current stream.  The entries launch on the current CUDA device, which need
+    not be `index`."""
+    if torch._C._cuda_getDevice() == index:
+        return fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    with torch.cuda.device(index):
+        return fn(*args, torch._C._cuda_getCurrentRawStream(index))
+
+
+def error_ptr(index: int) -> int:
+    """Address of device `index`'s error word (allocated once, never freed)."""
+    p = _err_ptrs.get(index)
+    if p is None:
+        p = _err_ptrs[index] = device_state(torch.device("cuda", index)).err.data_ptr()
+    return p
 
 
 def error_word(device: torch.device) -> torch.Tensor:

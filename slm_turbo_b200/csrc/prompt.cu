@@ -27,6 +27,8 @@
 // NaN or an infinity is a NaN -- so V tiles with a hidden key are searched for
 // such values; where there are some they are taken out of the tile, and added
 // to the rows that do attend to them at the end, read from global memory.
+#include <atomic>
+
 #include "internal.h"
 #include "tcgen05.cuh"
 
@@ -546,13 +548,17 @@ bool encode_rows(CUtensorMap* m, const void* base, bool bf16, int64_t d, int64_t
 
 template <int D, bool BF16>
 int prompt_launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const PromptParams& p, int grid,
-                  cudaStream_t st) {
-  // per device: the attribute belongs to the device's context
-  if (cudaFuncSetAttribute(prompt_kernel<D, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           PromptGeom<D>::SMEM) != cudaSuccess)
-    {
-    launch_status();  // clears it
-    return SLMT_ERR_CUDA;
+                  int device, cudaStream_t st) {
+  // once per device: the attribute belongs to the device's context
+  static std::atomic<uint64_t> ready{0};
+  const uint64_t bit = device < 64 ? 1ull << device : 0ull;
+  if (!(ready.load(std::memory_order_relaxed) & bit)) {
+    if (cudaFuncSetAttribute(prompt_kernel<D, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             PromptGeom<D>::SMEM) != cudaSuccess) {
+      launch_status();  // clears it
+      return SLMT_ERR_CUDA;
+    }
+    ready.fetch_or(bit, std::memory_order_relaxed);
   }
   prompt_kernel<D, BF16><<<grid, kThreads, PromptGeom<D>::SMEM, st>>>(mq, mk, mv, p);
   return launch_status();
@@ -636,12 +642,12 @@ extern "C" int slmt_prompt_attention(const void* q, int64_t q_token_stride, int6
     const int grid = (int)std::min<int64_t>(sms, pairs * num_kv_heads);
     int rc;
     if (head_dim == 64)
-      rc = bf16 ? prompt_launch<64, true>(mq, mk, mv, p, grid, st) : prompt_launch<64, false>(mq, mk, mv, p, grid, st);
+      rc = bf16 ? prompt_launch<64, true>(mq, mk, mv, p, grid, dev, st) : prompt_launch<64, false>(mq, mk, mv, p, grid, dev, st);
     else if (head_dim == 80)
-      rc = bf16 ? prompt_launch<80, true>(mq, mk, mv, p, grid, st) : prompt_launch<80, false>(mq, mk, mv, p, grid, st);
+      rc = bf16 ? prompt_launch<80, true>(mq, mk, mv, p, grid, dev, st) : prompt_launch<80, false>(mq, mk, mv, p, grid, dev, st);
     else
-      rc = bf16 ? prompt_launch<128, true>(mq, mk, mv, p, grid, st)
-                : prompt_launch<128, false>(mq, mk, mv, p, grid, st);
+      rc = bf16 ? prompt_launch<128, true>(mq, mk, mv, p, grid, dev, st)
+                : prompt_launch<128, false>(mq, mk, mv, p, grid, dev, st);
     if (rc != SLMT_OK) return rc;
   }
   return SLMT_OK;

@@ -498,19 +498,26 @@ def kv_append_per_channel(x_new, scale, zero, packed, pos):
 # =============================================================================
 #  The serving step around the cache
 # =============================================================================
-def _same_device(what, dev, **tensors):
+def _same_device(what, index, **tensors):
     for name, t in tensors.items():
-        if t is not None and t.device != dev:
-            raise RuntimeError(f"{what}: {name} is on {t.device}, expected {dev}")
+        if t is not None and t.get_device() != index:
+            raise RuntimeError(f"{what}: {name} is on {t.device}, expected cuda:{index}")
 
 
 def _no_autograd(what, *tensors):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError(f"{what}: has no backward pass; call it under torch.no_grad() or on detached tensors")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError(f"{what}: has no backward pass; call it under torch.no_grad() or on detached "
+                                   "tensors")
 
 
 def _int32(t):
     return t if t.dtype == torch.int32 and t.is_contiguous() else t.to(torch.int32).contiguous()
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
 
 
 def kv_page_plan(query_start_loc, seq_lens, block_tables, block_size, num_tokens, free_blocks=None,
@@ -532,7 +539,7 @@ def kv_page_plan(query_start_loc, seq_lens, block_tables, block_size, num_tokens
     """
     L = _lib.load()
     _require_cuda(block_tables, "page plan: block_tables", (torch.int32,))
-    dev = block_tables.device
+    index = block_tables.get_device()
     num_tokens = int(num_tokens)
     R = seq_lens.numel()
     if block_tables.dim() != 2 or block_tables.size(0) < R or (block_tables.size(1) > 1 and block_tables.stride(1) != 1):
@@ -541,27 +548,26 @@ def kv_page_plan(query_start_loc, seq_lens, block_tables, block_size, num_tokens
         raise RuntimeError(f"page plan: query_start_loc needs {R + 1} entries, has {query_start_loc.numel()}")
     if num_tokens < 0:
         raise RuntimeError(f"page plan: num_tokens must not be negative, got {num_tokens}")
-    for name, t, n in (("free_blocks", free_blocks, None), ("free_cursor", free_cursor, 1)):
-        if t is not None and (t.dtype != torch.int32 or not t.is_contiguous() or (n is not None and t.numel() != n)):
-            raise RuntimeError(f"page plan: {name} must be contiguous int32" + (f" of {n} entry" if n else ""))
+    if free_blocks is not None and (free_blocks.dtype != torch.int32 or not free_blocks.is_contiguous()):
+        raise RuntimeError("page plan: free_blocks must be contiguous int32")
+    if free_cursor is not None and (free_cursor.dtype != torch.int32 or free_cursor.numel() != 1):
+        raise RuntimeError("page plan: free_cursor must be one int32")
     for name, t in (("slot_mapping", slot_mapping), ("positions", positions)):
         if t is not None and (t.dtype != torch.int64 or not t.is_contiguous() or t.numel() != num_tokens):
             raise RuntimeError(f"page plan: {name} must be contiguous int64 of length {num_tokens}")
-    _same_device("page plan", dev, query_start_loc=query_start_loc, seq_lens=seq_lens, free_blocks=free_blocks,
+    _same_device("page plan", index, query_start_loc=query_start_loc, seq_lens=seq_lens, free_blocks=free_blocks,
                  free_cursor=free_cursor, slot_mapping=slot_mapping, positions=positions)
     qsl, sl = _int32(query_start_loc), _int32(seq_lens)
     if slot_mapping is None:
-        slot_mapping = torch.empty(num_tokens, dtype=torch.int64, device=dev)
+        slot_mapping = block_tables.new_empty(num_tokens, dtype=torch.int64)
     if positions is None:
-        positions = torch.empty(num_tokens, dtype=torch.int64, device=dev)
-    cursor = torch.empty(1, dtype=torch.int32, device=dev)
-    with _lib.on_device(dev):
-        rc = L.slmt_page_plan(
-            qsl.data_ptr(), sl.data_ptr(), R, block_tables.data_ptr(), block_tables.stride(0), block_tables.size(1),
-            int(block_size), None if free_blocks is None else free_blocks.data_ptr(),
-            0 if free_blocks is None else free_blocks.numel(), None if free_cursor is None else free_cursor.data_ptr(),
-            num_tokens, slot_mapping.data_ptr(), positions.data_ptr(), cursor.data_ptr(),
-            _lib.error_word(dev).data_ptr(), _lib.stream_of(dev))
+        positions = block_tables.new_empty(num_tokens, dtype=torch.int64)
+    cursor = block_tables.new_empty(1)
+    rc = _lib.call_on(
+        index, L.slmt_page_plan, qsl.data_ptr(), sl.data_ptr(), R, block_tables.data_ptr(), block_tables.stride(0),
+        block_tables.size(1), int(block_size), _ptr(free_blocks), 0 if free_blocks is None else free_blocks.numel(),
+        _ptr(free_cursor), num_tokens, slot_mapping.data_ptr(), positions.data_ptr(), cursor.data_ptr(),
+        _lib.error_ptr(index))
     _lib.check(rc, "page plan")
     return slot_mapping, positions, cursor
 
@@ -654,7 +660,7 @@ def _rotary_args(what, query, key, positions, inv_freq, query_out, key_out):
     for name, o, t in (("query_out", query_out, query), ("key_out", key_out, key)):
         if o is not None and (o.shape != t.shape or o.dtype != t.dtype or o.stride(2) != 1):
             raise RuntimeError(f"{what}: {name} must be {tuple(t.shape)} {t.dtype} with unit head-dim stride")
-    _same_device(what, query.device, key=key, positions=positions, inv_freq=inv_freq, query_out=query_out,
+    _same_device(what, query.get_device(), key=key, positions=positions, inv_freq=inv_freq, query_out=query_out,
                  key_out=key_out)
     _no_autograd(what, query, key, inv_freq, query_out, key_out)
     # an in-place call reads the caller's own rows, whatever their strides
@@ -676,15 +682,14 @@ def kv_rotary(query, key, positions, inv_freq, interleaved=False, attention_scal
     """
     L = _lib.load()
     q, k, pos, freq = _rotary_args("rotary", query, key, positions, inv_freq, query_out, key_out)
-    dev = q.device
-    qo = torch.empty(q.shape, dtype=q.dtype, device=dev) if query_out is None else query_out
-    ko = torch.empty(k.shape, dtype=k.dtype, device=dev) if key_out is None else key_out
-    with _lib.on_device(dev):
-        rc = L.slmt_rotary(
-            q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), _lib.dtype_tag(q.dtype),
-            pos.data_ptr(), _lib.dtype_tag(pos.dtype), freq.data_ptr(), 2 * freq.numel(), int(bool(interleaved)),
-            float(attention_scaling), q.size(0), q.size(1), k.size(1), q.size(2), qo.data_ptr(), qo.stride(0),
-            qo.stride(1), ko.data_ptr(), ko.stride(0), ko.stride(1), _lib.stream_of(dev))
+    N, H, D = q.shape
+    qo = q.new_empty((N, H, D)) if query_out is None else query_out
+    ko = k.new_empty(k.shape) if key_out is None else key_out
+    rc = _lib.call_on(
+        q.get_device(), L.slmt_rotary, q.data_ptr(), *q.stride()[:2], k.data_ptr(), *k.stride()[:2],
+        _lib.dtype_tag(q.dtype), pos.data_ptr(), _lib.dtype_tag(pos.dtype), freq.data_ptr(), 2 * freq.numel(),
+        int(bool(interleaved)), float(attention_scaling), N, H, k.size(1), D, qo.data_ptr(), *qo.stride()[:2],
+        ko.data_ptr(), *ko.stride()[:2])
     _lib.check(rc, "rotary")
     return qo, ko
 
@@ -714,24 +719,19 @@ def kv_rotary_store(query, key, value, positions, inv_freq, kv_cache, slot_mappi
         raise RuntimeError(f"rotary store: slot_mapping must be int64 of length {N}")
     if key_out is not None and not return_key:
         raise RuntimeError("rotary store: key_out is given but return_key is False")
-    dev = q.device
-    _same_device("rotary store", dev, value=value, kv_cache=kv_cache, slot_mapping=slot_mapping)
+    index = q.get_device()
+    _same_device("rotary store", index, value=value, kv_cache=kv_cache, slot_mapping=slot_mapping)
     _no_autograd("rotary store", value)
     v = value if value.stride(2) == 1 else value.contiguous()
     sm = slot_mapping.contiguous()
-    qo = torch.empty(q.shape, dtype=q.dtype, device=dev) if query_out is None else query_out
-    ko = key_out
-    if ko is None and return_key:
-        ko = torch.empty(k.shape, dtype=k.dtype, device=dev)
-    with _lib.on_device(dev):
-        rc = L.slmt_rotary_store(
-            q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
-            v.stride(0), v.stride(1), _lib.dtype_tag(q.dtype), pos.data_ptr(), _lib.dtype_tag(pos.dtype),
-            freq.data_ptr(), 2 * freq.numel(), int(bool(interleaved)), float(attention_scaling), N, q.size(1), KV, D,
-            qo.data_ptr(), qo.stride(0), qo.stride(1), None if ko is None else ko.data_ptr(),
-            0 if ko is None else ko.stride(0), 0 if ko is None else ko.stride(1), kv_cache.data_ptr(),
-            kv_cache.size(0), kv_cache.size(1), sm.data_ptr(), _lib.error_word(dev).data_ptr(),
-            _lib.stream_of(dev))
+    qo = q.new_empty(q.shape) if query_out is None else query_out
+    ko = k.new_empty(k.shape) if key_out is None and return_key else key_out
+    rc = _lib.call_on(
+        index, L.slmt_rotary_store, q.data_ptr(), *q.stride()[:2], k.data_ptr(), *k.stride()[:2], v.data_ptr(),
+        *v.stride()[:2], _lib.dtype_tag(q.dtype), pos.data_ptr(), _lib.dtype_tag(pos.dtype), freq.data_ptr(),
+        2 * freq.numel(), int(bool(interleaved)), float(attention_scaling), N, q.size(1), KV, D, qo.data_ptr(),
+        *qo.stride()[:2], _ptr(ko), *((0, 0) if ko is None else ko.stride()[:2]), kv_cache.data_ptr(),
+        kv_cache.size(0), kv_cache.size(1), sm.data_ptr(), _lib.error_ptr(index))
     _lib.check(rc, "rotary store")
     return qo, ko
 
@@ -750,27 +750,25 @@ def kv_dequantize_load(kv_cache, slot_mapping, dtype=torch.float16, key_out=None
     if slot_mapping.dtype != torch.int64 or slot_mapping.dim() != 1:
         raise RuntimeError("load: slot_mapping must be int64 [N]")
     NB, bs, KV, row = kv_cache.shape
-    N, D, dev = slot_mapping.numel(), row - 8, kv_cache.device
+    N, D, index = slot_mapping.numel(), row - 8, kv_cache.get_device()
     for name, t in (("key_out", key_out), ("value_out", value_out)):
-        if t is not None and (tuple(t.shape) != (N, KV, D) or t.dtype != dtype or not t.is_contiguous()):
+        if t is not None and (t.shape != (N, KV, D) or t.dtype != dtype or not t.is_contiguous()):
             raise RuntimeError(f"load: {name} must be contiguous {(N, KV, D)} {dtype}")
-    _same_device("load", dev, slot_mapping=slot_mapping, key_out=key_out, value_out=value_out)
+    _same_device("load", index, slot_mapping=slot_mapping, key_out=key_out, value_out=value_out)
     _no_autograd("load", key_out, value_out)
     sm = slot_mapping.contiguous()
-    k = torch.empty(N, KV, D, dtype=dtype, device=dev) if key_out is None else key_out
-    v = torch.empty(N, KV, D, dtype=dtype, device=dev) if value_out is None else value_out
-    with _lib.on_device(dev):
-        rc = L.slmt_kv_dequantize_load(
-            kv_cache.data_ptr(), NB, bs, KV, D, sm.data_ptr(), N, k.data_ptr(), v.data_ptr(), _lib.dtype_tag(dtype),
-            _lib.error_word(dev).data_ptr(), _lib.stream_of(dev))
+    k = kv_cache.new_empty((N, KV, D), dtype=dtype) if key_out is None else key_out
+    v = kv_cache.new_empty((N, KV, D), dtype=dtype) if value_out is None else value_out
+    rc = _lib.call_on(index, L.slmt_kv_dequantize_load, kv_cache.data_ptr(), NB, bs, KV, D, sm.data_ptr(), N,
+                      k.data_ptr(), v.data_ptr(), _lib.dtype_tag(dtype), _lib.error_ptr(index))
     _lib.check(rc, "load")
     return k, v
 
 
 def _tile_ready(t):
     """`t` itself where 16-byte rows can be copied from it, else a dense copy."""
-    if t.stride(2) == 1 and t.stride(0) % 8 == 0 and t.stride(1) % 8 == 0 and t.data_ptr() % 16 == 0 \
-            and t.stride(0) > 0 and t.stride(1) > 0:
+    token, head, dim = t.stride()
+    if dim == 1 and token > 0 and head > 0 and (token | head) % 8 == 0 and t.data_ptr() % 16 == 0:
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
@@ -807,23 +805,21 @@ def kv_prompt_attention(query, key, value, query_start_loc, max_query_len, seq_l
                            + ("" if seq_lens is None else f" (seq_lens has {seq_lens.numel()})"))
     if out is not None and (out.shape != query.shape or (N > 0 and out.stride(2) != 1)):
         raise RuntimeError(f"prompt attention: out must be {tuple(query.shape)} with unit head-dim stride")
-    dev = query.device
-    _same_device("prompt attention", dev, key=key, value=value, query_start_loc=query_start_loc, seq_lens=seq_lens,
+    index = query.get_device()
+    _same_device("prompt attention", index, key=key, value=value, query_start_loc=query_start_loc, seq_lens=seq_lens,
                  out=out)
     _no_autograd("prompt attention", query, key, value, out)
     if out is None:
-        out = torch.empty(N, H, D, dtype=torch.float32, device=dev)
+        out = query.new_empty((N, H, D), dtype=torch.float32)
     if N == 0:
         return out
     q, k, v = _tile_ready(query), _tile_ready(key), _tile_ready(value)
     qsl = _int32(query_start_loc)
     sl = None if seq_lens is None else _int32(seq_lens)
-    with _lib.on_device(dev):
-        rc = L.slmt_prompt_attention(
-            q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
-            v.stride(0), v.stride(1), _lib.dtype_tag(q.dtype), qsl.data_ptr(), None if sl is None else sl.data_ptr(),
-            R, int(max_query_len), N, H, KV, D, float(1.0 / math.sqrt(D) if sm_scale is None else sm_scale),
-            out.data_ptr(), _lib.dtype_tag(out.dtype), out.stride(0), out.stride(1),
-            _lib.error_word(dev).data_ptr(), _lib.stream_of(dev))
+    rc = _lib.call_on(
+        index, L.slmt_prompt_attention, q.data_ptr(), *q.stride()[:2], k.data_ptr(), *k.stride()[:2], v.data_ptr(),
+        *v.stride()[:2], _lib.dtype_tag(q.dtype), qsl.data_ptr(), _ptr(sl), R, int(max_query_len), N, H, KV, D,
+        float(1.0 / math.sqrt(D) if sm_scale is None else sm_scale), out.data_ptr(), _lib.dtype_tag(out.dtype),
+        *out.stride()[:2], _lib.error_ptr(index))
     _lib.check(rc, "prompt attention")
     return out
