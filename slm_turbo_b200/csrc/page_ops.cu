@@ -210,7 +210,10 @@ struct Vec8<float> {
 // over tokens, four at a time so that their slot ids and code words are in
 // flight together; places are found once, with 32-bit arithmetic.
 constexpr int kLoadThreads = 256;
-constexpr int kLoadUnroll = 4;
+#ifndef LOAD_U
+#define LOAD_U 4
+#endif
+constexpr int kLoadUnroll = LOAD_U;
 
 template <int D, typename T>
 __global__ void __launch_bounds__(kLoadThreads)

@@ -28,19 +28,38 @@ struct SlotRow {
 
 // The parts of the quantizer, for rows that lie across lanes in another way:
 // minimum and step of a row, a value's code, and the two fp16 rulers.
+// A code needs fl((x - mn) / step), correctly rounded.  Instead of a division
+// per value, slot_code multiplies by the row's rounded reciprocal and corrects
+// the quotient twice with its exact remainder: after the first correction it
+// is within an ulp, and by P. Markstein's theorem (IBM J. R&D 34-1, 1990) the
+// second then gives the correctly rounded quotient, for every divisor but one
+// whose mantissa is all ones.  Such steps, and those so large or small that a
+// remainder could leave the normal range, take the division.
 struct SlotScale {
-  float mn, step;
+  float mn, step, recip;
+  bool divide;
 };
 __device__ __forceinline__ SlotScale slot_scale(float mn, float mx) {
   SlotScale s;
   s.mn = mn;
   s.step = __fdiv_rn(mx - mn, 15.0f);
   if (!(s.step > 0.0f)) s.step = 1.0f;  // constant row guard (ref .cuh:854)
+  s.recip = __frcp_rn(s.step);
+  s.divide = !(s.step > 0x1p-60f && s.step < 0x1p60f) || (__float_as_uint(s.step) & 0x7FFFFFu) == 0x7FFFFFu;
   return s;
 }
 __device__ __forceinline__ uint32_t slot_code(float x, const SlotScale& s) {
-  const int q = (int)__fadd_rn(__fdiv_rn(__fsub_rn(x, s.mn), s.step), 0.5f);
-  return (uint32_t)(q < 0 ? 0 : (q > 15 ? 15 : q));
+  const float d = __fsub_rn(x, s.mn);
+  float q;
+  if (s.divide) {
+    q = __fdiv_rn(d, s.step);
+  } else {
+    q = __fmul_rn(d, s.recip);
+    q = __fmaf_rn(__fmaf_rn(-q, s.step, d), s.recip, q);
+    q = __fmaf_rn(__fmaf_rn(-q, s.step, d), s.recip, q);
+  }
+  const int c = (int)__fadd_rn(q, 0.5f);
+  return (uint32_t)(c < 0 ? 0 : (c > 15 ? 15 : c));
 }
 __device__ __forceinline__ uint32_t slot_rulers(const SlotScale& s) {
   return (uint32_t)__half_as_ushort(__float2half_rn(s.mn)) |

@@ -20,7 +20,8 @@ namespace slmt {
 namespace {
 
 constexpr int kRotThreads = 256;
-constexpr int kRotRows = 4;  // rows of a thread in flight
+constexpr int kRotRows = 4;   // q rows of a thread in flight
+constexpr int kRotKRows = 2;  // k rows of a thread in flight, with their v rows
 
 struct RotaryParams {
   const void* q;
@@ -58,223 +59,334 @@ enum RotaryLayout {
   ROT_ANY = 2           // 8 dims next to one another, partners fetched one by one
 };
 
-__device__ __forceinline__ float from16(uint32_t bits, int bf16) {
-  return bf16 ? __bfloat162float(__ushort_as_bfloat16((uint16_t)bits)) : __half2float(__ushort_as_half((uint16_t)bits));
+template <bool BF16>
+__device__ __forceinline__ float from16(uint32_t bits) {
+  return BF16 ? __bfloat162float(__ushort_as_bfloat16((uint16_t)bits)) : __half2float(__ushort_as_half((uint16_t)bits));
 }
-__device__ __forceinline__ uint32_t to16(float x, int bf16) {
-  return bf16 ? (uint32_t)__bfloat16_as_ushort(__float2bfloat16_rn(x)) : (uint32_t)__half_as_ushort(__float2half_rn(x));
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if constexpr (BF16) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  return pack_half2(lo, hi);
+}
+__device__ __forceinline__ int64_t position_of(const RotaryParams& p, int64_t tok) {
+  return p.pos_i64 ? reinterpret_cast<const int64_t*>(p.positions)[tok]
+                   : (int64_t) reinterpret_cast<const int32_t*>(p.positions)[tok];
 }
 
-// One CTA per token: D / 8 lanes to a row (D 80: 10 of 16), so a thread's
-// pairs are the same in every row and their cos and sin stay in registers.
-// The rows' loads are issued before the CTA works out the token's angles (64
-// double-precision sincos at most, a thread each), which hides one behind the
-// other.
-template <int D, int LAYOUT, bool STORE>
-__global__ void __launch_bounds__(kRotThreads) rotary_kernel(const RotaryParams p) {
-  constexpr int ACTIVE = D / 8, LANES = D == 64 ? 8 : 16, SLOTS = kRotThreads / LANES;
-  constexpr int ROWS = LAYOUT == ROT_ANY ? 1 : kRotRows;
-  __shared__ float2 s_cs[D / 2];
-  const int64_t tok = blockIdx.x;
-  const int li = threadIdx.x % LANES, slot0 = threadIdx.x / LANES;
-  const bool act = li < ACTIVE;
-  const int heads = p.hq + p.kv, half = p.half;
-  // dims of the thread: 4 from d0 on and 4 from d1 on; pairs from pair0 on
-  int d0 = 8 * li, d1 = d0 + 4, pair0 = 4 * li;
-  bool turns = false;  // HALF: all 4 pairs turn, or none
-  if (LAYOUT == ROT_HALF) {
-    turns = li < half / 4;
-    d0 = turns ? 4 * li : 2 * half + 8 * (li - half / 4);
-    d1 = turns ? half + 4 * li : d0 + 4;
+// D / 8 lanes to a row; D 80: 10 of 16.
+template <int D>
+struct RotGeom {
+  static constexpr int ACTIVE = D / 8, LANES = D == 64 ? 8 : 16, SLOTS = kRotThreads / LANES;
+};
+
+// 8 of a row's values, dims d0..d0+3 and d1..d1+3, two to a word.
+template <int LAYOUT>
+__device__ __forceinline__ uint4 load8(const uint16_t* row, int d0, int d1) {
+  if (LAYOUT == ROT_INTERLEAVED) return *reinterpret_cast<const uint4*>(row + d0);
+  if (LAYOUT == ROT_ANY)
+    return make_uint4(row[d0] | (uint32_t)row[d0 + 1] << 16, row[d0 + 2] | (uint32_t)row[d0 + 3] << 16,
+                      row[d1] | (uint32_t)row[d1 + 1] << 16, row[d1 + 2] | (uint32_t)row[d1 + 3] << 16);
+  const uint2 a = *reinterpret_cast<const uint2*>(row + d0), b = *reinterpret_cast<const uint2*>(row + d1);
+  return make_uint4(a.x, a.y, b.x, b.y);
+}
+template <int LAYOUT>
+__device__ __forceinline__ void store8(uint16_t* row, int d0, int d1, const uint4& w) {
+  if (LAYOUT == ROT_INTERLEAVED) {
+    *reinterpret_cast<uint4*>(row + d0) = w;
+  } else if (LAYOUT == ROT_HALF) {
+    *reinterpret_cast<uint2*>(row + d0) = make_uint2(w.x, w.y);
+    *reinterpret_cast<uint2*>(row + d1) = make_uint2(w.z, w.w);
+  } else {
+    const uint32_t a[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int j = 0; j < 8; ++j) row[d0 + j] = (uint16_t)(j & 1 ? a[j >> 1] >> 16 : a[j >> 1]);
   }
-  float2 cs[4];
+}
+template <bool BF16>
+__device__ __forceinline__ void unpack8(const uint4& w, float (&x)[8]) {
+  const uint32_t a[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int j = 0; j < 8; ++j) x[j] = from16<BF16>(j & 1 ? a[j >> 1] >> 16 : a[j >> 1] & 0xFFFFu);
+}
+template <bool BF16>
+__device__ __forceinline__ uint4 pack8(const float (&y)[8]) {
+  return make_uint4(pack2<BF16>(y[0], y[1]), pack2<BF16>(y[2], y[3]), pack2<BF16>(y[4], y[5]), pack2<BF16>(y[6], y[7]));
+}
+
+// The turned row's 8 values.  cs: cos and sin of pairs pair0..pair0+3, of
+// which the first `on` turn.
+template <int LAYOUT, bool BF16>
+__device__ __forceinline__ uint4 turn8(const uint4& w, const float2* cs, int on) {
+  float x[8], y[8];
+  unpack8<BF16>(w, x);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int i1 = LAYOUT == ROT_HALF ? j : 2 * j, i2 = LAYOUT == ROT_HALF ? 4 + j : 2 * j + 1;
+    const float a = x[i1], b = x[i2];
+    y[i1] = j < on ? __fsub_rn(__fmul_rn(a, cs[j].x), __fmul_rn(b, cs[j].y)) : a;
+    y[i2] = j < on ? __fadd_rn(__fmul_rn(b, cs[j].x), __fmul_rn(a, cs[j].y)) : b;
+  }
+  return pack8<BF16>(y);
+}
+
+// One row of k (turned) and v into its slot: the lanes of the row are
+// neighbours in the warp, and the whole warp takes part in the exchange.
+template <int D, int LAYOUT, bool BF16>
+__device__ __forceinline__ void quantize8(const uint4& kw, const uint4& vw, uint8_t* row, bool act, bool write, int li,
+                                          int d0, int d1) {
+  float mn[2] = {INFINITY, INFINITY}, mx[2] = {-INFINITY, -INFINITY}, vx[8], kx[8];
+  unpack8<BF16>(vw, vx);
+  unpack8<BF16>(kw, kx);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    if (act) {
+      mn[0] = fminf(mn[0], kx[j]), mx[0] = fmaxf(mx[0], kx[j]);
+      mn[1] = fminf(mn[1], vx[j]), mx[1] = fmaxf(mx[1], vx[j]);
+    }
+  }
+#pragma unroll
+  for (int o = RotGeom<D>::LANES / 2; o > 0; o >>= 1) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      mn[i] = fminf(mn[i], __shfl_xor_sync(0xffffffffu, mn[i], o));
+      mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], o));
+    }
+  }
+  if (!write) return;
+  const SlotScale ks = slot_scale(mn[0], mx[0]), vs = slot_scale(mn[1], mx[1]);
+  uint32_t kc = 0u, vc = 0u;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    kc |= slot_code(kx[j], ks) << (4 * j);
+    vc |= slot_code(vx[j], vs) << (4 * j);
+  }
+  if (LAYOUT == ROT_HALF) {
+    *reinterpret_cast<uint16_t*>(row + d0 / 2) = (uint16_t)kc;
+    *reinterpret_cast<uint16_t*>(row + d1 / 2) = (uint16_t)(kc >> 16);
+    *reinterpret_cast<uint16_t*>(row + D / 2 + d0 / 2) = (uint16_t)vc;
+    *reinterpret_cast<uint16_t*>(row + D / 2 + d1 / 2) = (uint16_t)(vc >> 16);
+  } else {
+    *reinterpret_cast<uint32_t*>(row + d0 / 2) = kc;
+    *reinterpret_cast<uint32_t*>(row + D / 2 + d0 / 2) = vc;
+  }
+  if (li == 0) *reinterpret_cast<uint2*>(row + D) = make_uint2(slot_rulers(ks), slot_rulers(vs));
+}
+
+// A token's slot in the cache, -1 if it has none.
+__device__ __forceinline__ int64_t slot_of(const RotaryParams& p, int64_t tok, bool report) {
+  const int64_t s = p.slot_mapping[tok];
+  if (s < p.num_slots) return s;
+  if (report && p.err) atomicOr(reinterpret_cast<unsigned int*>(p.err), SLMT_DEVERR_SLOT);
+  return -1;
+}
+
+// TOKENS tokens per CTA.  The k rows come first (they are stored and
+// quantized, which takes longest), then the q rows, kRotRows of a thread in
+// flight.  The first rows' loads are issued before the CTA works out its
+// tokens' angles -- double-precision sincos, a long chain -- which hides one
+// behind the other; four tokens share that wait when there are enough of them
+// to fill the GPU, and one token per CTA spreads few tokens over more SMs.
+template <int D, int LAYOUT, bool STORE, bool BF16, int TOKENS>
+__global__ void __launch_bounds__(kRotThreads, 4) rotary_kernel(const RotaryParams p) {
+  using G = RotGeom<D>;
+  constexpr int SLOTS = G::SLOTS;
+  __shared__ float4 s_cs4[TOKENS][D / 4];  // pairs of (cos, sin): read two at a time
+  const int64_t tok0 = (int64_t)blockIdx.x * TOKENS;
+  const int nt = (int)min((int64_t)TOKENS, p.num_tokens - tok0);
+  const int li = threadIdx.x % G::LANES, slot0 = threadIdx.x / G::LANES;
+  const bool act = li < G::ACTIVE;
+  const int half = p.half;
+  // dims of the thread: 4 from d0 on and 4 from d1 on; pairs from pair0 on
+  int d0 = 8 * li, d1 = d0 + 4, on;
+  const int pair0 = 4 * li;
+  if (LAYOUT == ROT_HALF) {
+    on = li < half / 4 ? 4 : 0;
+    d0 = on ? 4 * li : 2 * half + 8 * (li - half / 4);
+    d1 = on ? half + 4 * li : d0 + 4;
+  } else {
+    on = half - pair0;
+  }
   const uint16_t* q = reinterpret_cast<const uint16_t*>(p.q);
   const uint16_t* k = reinterpret_cast<const uint16_t*>(p.k);
   const uint16_t* v = reinterpret_cast<const uint16_t*>(p.v);
-  int64_t cache_slot = -1;
-  if (STORE) {
-    cache_slot = p.slot_mapping[tok];
-    if (cache_slot >= p.num_slots) {
-      if (threadIdx.x == 0 && p.err) atomicOr(reinterpret_cast<unsigned int*>(p.err), SLMT_DEVERR_SLOT);
-      cache_slot = -1;
+  uint16_t* q_out = reinterpret_cast<uint16_t*>(p.q_out);
+  uint16_t* k_out = reinterpret_cast<uint16_t*>(p.k_out);
+
+  auto angles = [&] {
+    float2* s_cs = reinterpret_cast<float2*>(s_cs4);
+    for (int i = threadIdx.x; i < nt * half; i += kRotThreads) {
+      const int t = TOKENS == 1 ? 0 : i / half, f = TOKENS == 1 ? i : i - t * half;
+      const float2 c = turn(position_of(p, tok0 + t), p.inv_freq[f]);
+      s_cs[t * (D / 2) + f] = make_float2(__fmul_rn(c.x, p.scaling), __fmul_rn(c.y, p.scaling));
     }
-  }
+    __syncthreads();
+  };
+  auto pairs_of = [&](int t, float2 (&cs)[4]) {
+    const float4 a = act ? s_cs4[t][pair0 / 2] : make_float4(0.f, 0.f, 0.f, 0.f);
+    const float4 b = act ? s_cs4[t][pair0 / 2 + 1] : a;
+    cs[0] = make_float2(a.x, a.y), cs[1] = make_float2(a.z, a.w);
+    cs[2] = make_float2(b.x, b.y), cs[3] = make_float2(b.z, b.w);
+  };
+
   bool first = true;
-  for (int h0 = 0; h0 < heads; h0 += SLOTS * ROWS) {
-    uint2 lo[ROWS], hi[ROWS], vlo[ROWS], vhi[ROWS];
-    float other[8];  // ROT_ANY: the partners
+  if (STORE) {  // k rows, two of a thread in flight
+    constexpr int ROWS = kRotKRows;
+    const int rows = nt * p.kv;
+    int t = slot0 / p.kv, h = slot0 - t * p.kv;
+    for (int base = 0; base < rows; base += SLOTS * ROWS) {
+      uint4 x[ROWS], vx[ROWS];
+      int tt[ROWS], hh[ROWS];
+      int64_t slot[ROWS];
 #pragma unroll
-    for (int r = 0; r < ROWS; ++r) {
-      const int h = h0 + slot0 + r * SLOTS;
-      lo[r] = hi[r] = vlo[r] = vhi[r] = make_uint2(0u, 0u);
-      if (!act || h >= heads) continue;
-      const bool is_k = h >= p.hq;
-      const uint16_t* row = is_k ? k + tok * p.k_tok + (int64_t)(h - p.hq) * p.k_head
-                                 : q + tok * p.q_tok + (int64_t)h * p.q_head;
-      if (LAYOUT == ROT_HALF) {
-        lo[r] = *reinterpret_cast<const uint2*>(row + d0);
-        hi[r] = *reinterpret_cast<const uint2*>(row + d1);
-      } else if (LAYOUT == ROT_INTERLEAVED) {
-        const uint4 x = *reinterpret_cast<const uint4*>(row + d0);
-        lo[r] = make_uint2(x.x, x.y), hi[r] = make_uint2(x.z, x.w);
-      } else {
-        uint32_t e[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int i = d0 + j;
-          e[j] = row[i];
-          int o = i;
-          if (i < 2 * half) o = p.interleaved ? i ^ 1 : (i < half ? i + half : i - half);
-          other[j] = from16(row[o], p.bf16);
-        }
-        lo[r] = make_uint2(e[0] | e[1] << 16, e[2] | e[3] << 16);
-        hi[r] = make_uint2(e[4] | e[5] << 16, e[6] | e[7] << 16);
-      }
-      if (STORE && is_k && cache_slot >= 0) {
-        const uint16_t* vr = v + tok * p.v_tok + (int64_t)(h - p.hq) * p.v_head;
-        if (LAYOUT == ROT_HALF) {
-          vlo[r] = *reinterpret_cast<const uint2*>(vr + d0);
-          vhi[r] = *reinterpret_cast<const uint2*>(vr + d1);
-        } else if (LAYOUT == ROT_INTERLEAVED) {
-          const uint4 x = *reinterpret_cast<const uint4*>(vr + d0);
-          vlo[r] = make_uint2(x.x, x.y), vhi[r] = make_uint2(x.z, x.w);
-        } else {
-          vlo[r] = make_uint2(vr[d0] | (uint32_t)vr[d0 + 1] << 16, vr[d0 + 2] | (uint32_t)vr[d0 + 3] << 16);
-          vhi[r] = make_uint2(vr[d1] | (uint32_t)vr[d1 + 1] << 16, vr[d1 + 2] | (uint32_t)vr[d1 + 3] << 16);
-        }
-      }
-    }
-    if (first) {
-      for (int i = threadIdx.x; i < half; i += kRotThreads) {
-        const int64_t pos = p.pos_i64 ? reinterpret_cast<const int64_t*>(p.positions)[tok]
-                                      : (int64_t) reinterpret_cast<const int32_t*>(p.positions)[tok];
-        const float2 t = turn(pos, p.inv_freq[i]);
-        s_cs[i] = make_float2(__fmul_rn(t.x, p.scaling), __fmul_rn(t.y, p.scaling));
-      }
-    }
-    // the angles; and, where partners are other threads' dims, every row is
-    // read before any of it is written (in-place calls)
-    if (first || LAYOUT == ROT_ANY) __syncthreads();
-    if (first && LAYOUT != ROT_ANY) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const bool on = act && (LAYOUT == ROT_HALF ? turns : pair0 + j < half);
-        cs[j] = on ? s_cs[pair0 + j] : make_float2(0.f, 0.f);
-      }
-    }
-    first = false;
-#pragma unroll
-    for (int r = 0; r < ROWS; ++r) {
-      const int h = h0 + slot0 + r * SLOTS;
-      const bool live = act && h < heads;
-      const bool is_k = h >= p.hq;
-      // x: dims d0..d0+3, d1..d1+3
-      float x[8];
-      const uint32_t w[4] = {lo[r].x, lo[r].y, hi[r].x, hi[r].y};
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = from16(j & 1 ? w[j >> 1] >> 16 : w[j >> 1] & 0xFFFFu, p.bf16);
-      uint32_t y[8];
-      if (LAYOUT == ROT_HALF) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float a = x[j], b = x[4 + j];
-          y[j] = to16(turns ? __fsub_rn(__fmul_rn(a, cs[j].x), __fmul_rn(b, cs[j].y)) : a, p.bf16);
-          y[4 + j] = to16(turns ? __fadd_rn(__fmul_rn(b, cs[j].x), __fmul_rn(a, cs[j].y)) : b, p.bf16);
-        }
-      } else if (LAYOUT == ROT_INTERLEAVED) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float a = x[2 * j], b = x[2 * j + 1];
-          const bool on = pair0 + j < half;
-          y[2 * j] = to16(on ? __fsub_rn(__fmul_rn(a, cs[j].x), __fmul_rn(b, cs[j].y)) : a, p.bf16);
-          y[2 * j + 1] = to16(on ? __fadd_rn(__fmul_rn(b, cs[j].x), __fmul_rn(a, cs[j].y)) : b, p.bf16);
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int i = d0 + j;
-          float z = x[j];
-          if (live && i < 2 * half) {
-            const bool second = p.interleaved ? i & 1 : i >= half;
-            const float2 t = s_cs[p.interleaved ? i >> 1 : second ? i - half : i];
-            const float a = __fmul_rn(z, t.x), b = __fmul_rn(other[j], t.y);
-            z = second ? __fadd_rn(a, b) : __fsub_rn(a, b);
-          }
-          y[j] = to16(z, p.bf16);
-        }
-      }
-      uint16_t* dst = reinterpret_cast<uint16_t*>(is_k ? p.k_out : p.q_out);
-      if (live && dst) {
-        dst += is_k ? tok * p.ko_tok + (int64_t)(h - p.hq) * p.ko_head : tok * p.qo_tok + (int64_t)h * p.qo_head;
-        const uint2 a = make_uint2(y[0] | y[1] << 16, y[2] | y[3] << 16);
-        const uint2 b = make_uint2(y[4] | y[5] << 16, y[6] | y[7] << 16);
-        if (LAYOUT == ROT_HALF) {
-          *reinterpret_cast<uint2*>(dst + d0) = a;
-          *reinterpret_cast<uint2*>(dst + d1) = b;
-        } else if (LAYOUT == ROT_INTERLEAVED) {
-          *reinterpret_cast<uint4*>(dst + d0) = make_uint4(a.x, a.y, b.x, b.y);
-        } else {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) dst[d0 + j] = (uint16_t)y[j];
-        }
-      }
-      // the cache: the whole warp takes part where a row of it is a k row
-      if (STORE && cache_slot >= 0 && __any_sync(0xffffffffu, h < heads && is_k)) {
-        float mn[2] = {INFINITY, INFINITY}, mx[2] = {-INFINITY, -INFINITY}, vx[8], kx[8];
-        const uint32_t vw[4] = {vlo[r].x, vlo[r].y, vhi[r].x, vhi[r].y};
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          vx[j] = from16(j & 1 ? vw[j >> 1] >> 16 : vw[j >> 1] & 0xFFFFu, p.bf16);
-          kx[j] = from16(y[j], p.bf16);
+      for (int r = 0; r < ROWS; ++r) {
+        tt[r] = t, hh[r] = h;
+        x[r] = vx[r] = make_uint4(0u, 0u, 0u, 0u);
+        slot[r] = -1;
+        if (t < nt) {
+          const int64_t tok = tok0 + t;
+          if (STORE) slot[r] = slot_of(p, tok, li == 0 && h == 0);
           if (act) {
-            mn[0] = fminf(mn[0], kx[j]), mx[0] = fmaxf(mx[0], kx[j]);
-            mn[1] = fminf(mn[1], vx[j]), mx[1] = fmaxf(mx[1], vx[j]);
+            x[r] = load8<LAYOUT>(k + tok * p.k_tok + (int64_t)h * p.k_head, d0, d1);
+            if (STORE && slot[r] >= 0) vx[r] = load8<LAYOUT>(v + tok * p.v_tok + (int64_t)h * p.v_head, d0, d1);
           }
         }
+        h += SLOTS;
+        while (h >= p.kv && t < nt) h -= p.kv, ++t;
+      }
+      if (first) angles();
+      first = false;
 #pragma unroll
-        for (int o = LANES / 2; o > 0; o >>= 1) {
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            mn[i] = fminf(mn[i], __shfl_xor_sync(0xffffffffu, mn[i], o));
-            mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], o));
-          }
-        }
-        if (live && is_k) {
-          const SlotScale ks = slot_scale(mn[0], mx[0]), vs = slot_scale(mn[1], mx[1]);
-          uint32_t kc = 0u, vc = 0u;
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            kc |= slot_code(kx[j], ks) << (4 * j);
-            vc |= slot_code(vx[j], vs) << (4 * j);
-          }
-          uint8_t* row = p.cache + (cache_slot * p.kv + (h - p.hq)) * (D + 8);
-          if (LAYOUT == ROT_HALF) {
-            *reinterpret_cast<uint16_t*>(row + d0 / 2) = (uint16_t)kc;
-            *reinterpret_cast<uint16_t*>(row + d1 / 2) = (uint16_t)(kc >> 16);
-            *reinterpret_cast<uint16_t*>(row + D / 2 + d0 / 2) = (uint16_t)vc;
-            *reinterpret_cast<uint16_t*>(row + D / 2 + d1 / 2) = (uint16_t)(vc >> 16);
-          } else {
-            *reinterpret_cast<uint32_t*>(row + d0 / 2) = kc;
-            *reinterpret_cast<uint32_t*>(row + D / 2 + d0 / 2) = vc;
-          }
-          if (li == 0) *reinterpret_cast<uint2*>(row + D) = make_uint2(slot_rulers(ks), slot_rulers(vs));
-        }
+      for (int r = 0; r < ROWS; ++r) {
+        const bool live = tt[r] < nt;
+        float2 cs[4];
+        pairs_of(live ? tt[r] : 0, cs);
+        const uint4 y = turn8<LAYOUT, BF16>(x[r], cs, on);
+        if (live && act && k_out)
+          store8<LAYOUT>(k_out + (tok0 + tt[r]) * p.ko_tok + (int64_t)hh[r] * p.ko_head, d0, d1, y);
+        if (STORE && __any_sync(0xffffffffu, slot[r] >= 0))
+          quantize8<D, LAYOUT, BF16>(y, vx[r], p.cache + (slot[r] * p.kv + hh[r]) * (D + 8), act, act && slot[r] >= 0,
+                                     li, d0, d1);
       }
     }
-    if (LAYOUT == ROT_ANY && h0 + SLOTS * ROWS < heads) __syncthreads();
   }
+  {  // q rows, and k rows that are not stored
+    const int heads = STORE ? p.hq : p.hq + p.kv, rows = nt * heads;
+    int t = heads ? slot0 / heads : 0, h = slot0 - t * heads;
+    for (int base = 0; base < rows; base += SLOTS * kRotRows) {
+      uint4 x[kRotRows];
+      uint16_t* out[kRotRows];
+      int tt[kRotRows];
+#pragma unroll
+      for (int r = 0; r < kRotRows; ++r) {
+        tt[r] = t;
+        x[r] = make_uint4(0u, 0u, 0u, 0u);
+        if (act && t < nt) {
+          const int64_t tok = tok0 + t;
+          if (STORE || h < p.hq) {
+            x[r] = load8<LAYOUT>(q + tok * p.q_tok + (int64_t)h * p.q_head, d0, d1);
+            out[r] = q_out + tok * p.qo_tok + (int64_t)h * p.qo_head;
+          } else {
+            x[r] = load8<LAYOUT>(k + tok * p.k_tok + (int64_t)(h - p.hq) * p.k_head, d0, d1);
+            out[r] = k_out + tok * p.ko_tok + (int64_t)(h - p.hq) * p.ko_head;
+          }
+        }
+        h += SLOTS;
+        while (h >= heads && t < nt) h -= heads, ++t;
+      }
+      if (first) angles();
+      first = false;
+#pragma unroll
+      for (int r = 0; r < kRotRows; ++r) {
+        if (!act || tt[r] >= nt) continue;
+        float2 cs[4];
+        pairs_of(tt[r], cs);
+        store8<LAYOUT>(out[r], d0, d1, turn8<LAYOUT, BF16>(x[r], cs, on));
+      }
+    }
+  }
+}
+
+// Rows at any alignment and any rot: a CTA per token, partners fetched one by
+// one, a row of a thread at a time.  Partners are other threads' dims, so
+// every row of a pass is read before any of it is written (in-place calls).
+template <int D, bool STORE, bool BF16>
+__global__ void __launch_bounds__(kRotThreads) rotary_any_kernel(const RotaryParams p) {
+  using G = RotGeom<D>;
+  __shared__ float2 s_cs[D / 2];
+  const int64_t tok = blockIdx.x;
+  const int li = threadIdx.x % G::LANES, slot0 = threadIdx.x / G::LANES;
+  const bool act = li < G::ACTIVE;
+  const int heads = p.hq + p.kv, half = p.half, d0 = 8 * li;
+  for (int i = threadIdx.x; i < half; i += kRotThreads) {
+    const float2 c = turn(position_of(p, tok), p.inv_freq[i]);
+    s_cs[i] = make_float2(__fmul_rn(c.x, p.scaling), __fmul_rn(c.y, p.scaling));
+  }
+  const int64_t slot = STORE ? slot_of(p, tok, threadIdx.x == 0) : -1;
+  for (int h0 = 0; h0 < heads; h0 += G::SLOTS) {
+    const int h = h0 + slot0;
+    const bool live = act && h < heads, is_k = h >= p.hq;
+    const uint16_t* row = reinterpret_cast<const uint16_t*>(is_k ? p.k : p.q) +
+                          (is_k ? tok * p.k_tok + (int64_t)(h - p.hq) * p.k_head : tok * p.q_tok + (int64_t)h * p.q_head);
+    float x[8], other[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int i = d0 + j;
+      const int o = i >= 2 * half ? i : p.interleaved ? i ^ 1 : i < half ? i + half : i - half;
+      x[j] = live ? from16<BF16>(row[i]) : 0.f;
+      other[j] = live ? from16<BF16>(row[o]) : 0.f;
+    }
+    __syncthreads();  // the angles; rows read
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int i = d0 + j;
+      if (live && i < 2 * half) {
+        const bool second = p.interleaved ? i & 1 : i >= half;
+        const float2 c = s_cs[p.interleaved ? i >> 1 : second ? i - half : i];
+        const float a = __fmul_rn(x[j], c.x), b = __fmul_rn(other[j], c.y);
+        x[j] = second ? __fadd_rn(a, b) : __fsub_rn(a, b);
+      }
+    }
+    const uint4 y = pack8<BF16>(x);
+    uint16_t* dst = reinterpret_cast<uint16_t*>(is_k ? p.k_out : p.q_out);
+    if (live && dst)
+      store8<ROT_ANY>(dst + (is_k ? tok * p.ko_tok + (int64_t)(h - p.hq) * p.ko_head
+                                  : tok * p.qo_tok + (int64_t)h * p.qo_head), d0, d0 + 4, y);
+    if (STORE && slot >= 0 && __any_sync(0xffffffffu, h < heads && is_k)) {
+      uint4 vw = make_uint4(0u, 0u, 0u, 0u);
+      if (live && is_k)
+        vw = load8<ROT_ANY>(reinterpret_cast<const uint16_t*>(p.v) + tok * p.v_tok + (int64_t)(h - p.hq) * p.v_head, d0,
+                            d0 + 4);
+      quantize8<D, ROT_ANY, BF16>(y, vw, p.cache + (slot * p.kv + (is_k ? h - p.hq : 0)) * (D + 8), act, live && is_k,
+                                  li, d0, d0 + 4);
+    }
+    __syncthreads();  // before the next pass's rows are written
+  }
+}
+
+template <int D, int LAYOUT, bool STORE, bool BF16>
+int rotary_launch_tokens(const RotaryParams& p, cudaStream_t st) {
+  // four tokens per CTA from two CTAs per SM on, one below
+  if (p.num_tokens >= 8 * 148)
+    rotary_kernel<D, LAYOUT, STORE, BF16, 4><<<(p.num_tokens + 3) / 4, kRotThreads, 0, st>>>(p);
+  else
+    rotary_kernel<D, LAYOUT, STORE, BF16, 1><<<p.num_tokens, kRotThreads, 0, st>>>(p);
+  return launch_status();
+}
+
+template <int D, bool STORE, bool BF16>
+int rotary_launch_typed(const RotaryParams& p, int layout, cudaStream_t st) {
+  if (layout == ROT_HALF) return rotary_launch_tokens<D, ROT_HALF, STORE, BF16>(p, st);
+  if (layout == ROT_INTERLEAVED) return rotary_launch_tokens<D, ROT_INTERLEAVED, STORE, BF16>(p, st);
+  rotary_any_kernel<D, STORE, BF16><<<p.num_tokens, kRotThreads, 0, st>>>(p);
+  return launch_status();
 }
 
 template <int D, bool STORE>
 int rotary_launch_d(const RotaryParams& p, int layout, cudaStream_t st) {
-  const dim3 grid((unsigned)p.num_tokens);
-  if (layout == ROT_HALF)
-    rotary_kernel<D, ROT_HALF, STORE><<<grid, kRotThreads, 0, st>>>(p);
-  else if (layout == ROT_INTERLEAVED)
-    rotary_kernel<D, ROT_INTERLEAVED, STORE><<<grid, kRotThreads, 0, st>>>(p);
-  else
-    rotary_kernel<D, ROT_ANY, STORE><<<grid, kRotThreads, 0, st>>>(p);
-  return launch_status();
+  return p.bf16 ? rotary_launch_typed<D, STORE, true>(p, layout, st) : rotary_launch_typed<D, STORE, false>(p, layout, st);
 }
 
 // Whether rows at these strides can be read and written `bytes` at a time.
