@@ -210,10 +210,7 @@ struct Vec8<float> {
 // over tokens, four at a time so that their slot ids and code words are in
 // flight together; places are found once, with 32-bit arithmetic.
 constexpr int kLoadThreads = 256;
-#ifndef LOAD_U
-#define LOAD_U 4
-#endif
-constexpr int kLoadUnroll = LOAD_U;
+constexpr int kLoadUnroll = 4;
 
 template <int D, typename T>
 __global__ void __launch_bounds__(kLoadThreads)
@@ -257,13 +254,22 @@ __global__ void __launch_bounds__(kLoadThreads)
     if (t >= num_tokens) return;
     const float mn = half_bits_to_float((uint16_t)(rulers[u] & 0xFFFFu));
     const float st = half_bits_to_float((uint16_t)(rulers[u] >> 16));
+    // A nibble left where it is under the bits of 2^23 is the float 2^23 +
+    // code * 16^j: one multiply-add with 16^-j and -2^23 16^-j gives the code,
+    // exactly, without shifts or integer conversions.  Five nibbles fit below
+    // bit 23; the others are taken from the word shifted once.
+    const uint64_t st2 = f2_pack(st, st), mn2 = f2_pack(mn, mn);
+    const uint32_t w0 = codes[u], w1 = codes[u] >> 16;
     float x[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      // 2^23 + code has the code in its low mantissa bits: code as a float
-      // without the slower integer conversion
-      const float code = __uint_as_float(((codes[u] >> (4 * j)) & 15u) | 0x4B000000u) - 8388608.f;
-      x[j] = __fmaf_rn(code, st, mn);
+    for (int j = 0; j < 8; j += 2) {
+      const uint32_t w = j < 4 ? w0 : w1;
+      const int k = j & 3;  // nibbles k and k + 1 of w
+      const float s0 = 1.f / (float)(1 << (4 * k)), s1 = s0 / 16.f;
+      const uint64_t biased = f2_pack(__uint_as_float((w & (15u << (4 * k))) | 0x4B000000u),
+                                      __uint_as_float((w & (15u << (4 * k + 4))) | 0x4B000000u));
+      const uint64_t code = f2_fma(biased, f2_pack(s0, s1), f2_pack(-8388608.f * s0, -8388608.f * s1));
+      f2_unpack(f2_fma(code, st2, mn2), x[j], x[j + 1]);
     }
     Vec8<T>::store(out + t * kv * D, x);
   }

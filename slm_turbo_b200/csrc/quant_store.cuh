@@ -29,12 +29,13 @@ struct SlotRow {
 // The parts of the quantizer, for rows that lie across lanes in another way:
 // minimum and step of a row, a value's code, and the two fp16 rulers.
 // A code needs fl((x - mn) / step), correctly rounded.  Instead of a division
-// per value, slot_code multiplies by the row's rounded reciprocal and corrects
-// the quotient twice with its exact remainder: after the first correction it
-// is within an ulp, and by P. Markstein's theorem (IBM J. R&D 34-1, 1990) the
-// second then gives the correctly rounded quotient, for every divisor but one
-// whose mantissa is all ones.  Such steps, and those so large or small that a
-// remainder could leave the normal range, take the division.
+// per value, slot_codes8 multiplies by the row's rounded reciprocal and
+// corrects the quotient twice with its exact remainder: after the first
+// correction it is within an ulp, and by P. Markstein's theorem (IBM J. R&D
+// 34-1, 1990) the second then gives the correctly rounded quotient, for every
+// divisor but one whose mantissa is all ones.  Rows with such a step, or one
+// so large or small that a remainder could leave the normal range (infinite
+// ones among them), take the division.
 struct SlotScale {
   float mn, step, recip;
   bool divide;
@@ -48,18 +49,35 @@ __device__ __forceinline__ SlotScale slot_scale(float mn, float mx) {
   s.divide = !(s.step > 0x1p-60f && s.step < 0x1p60f) || (__float_as_uint(s.step) & 0x7FFFFFu) == 0x7FFFFFu;
   return s;
 }
-__device__ __forceinline__ uint32_t slot_code(float x, const SlotScale& s) {
-  const float d = __fsub_rn(x, s.mn);
-  float q;
+// The codes of 8 values, the first in the lowest nibble.
+__device__ __forceinline__ uint32_t slot_codes8(const float (&x)[8], const SlotScale& s) {
+  uint32_t codes = 0u;
   if (s.divide) {
-    q = __fdiv_rn(d, s.step);
-  } else {
-    q = __fmul_rn(d, s.recip);
-    q = __fmaf_rn(__fmaf_rn(-q, s.step, d), s.recip, q);
-    q = __fmaf_rn(__fmaf_rn(-q, s.step, d), s.recip, q);
+#pragma unroll 1
+    for (int j = 0; j < 8; ++j) {
+      float xj = x[0];
+#pragma unroll
+      for (int i = 1; i < 8; ++i) xj = j == i ? x[i] : xj;
+      const int c = (int)__fadd_rn(__fdiv_rn(__fsub_rn(xj, s.mn), s.step), 0.5f);
+      codes |= (uint32_t)(c < 0 ? 0 : (c > 15 ? 15 : c)) << (4 * j);
+    }
+    return codes;
   }
-  const int c = (int)__fadd_rn(q, 0.5f);
-  return (uint32_t)(c < 0 ? 0 : (c > 15 ? 15 : c));
+  const uint64_t neg_mn = f2_pack(-s.mn, -s.mn), neg_step = f2_pack(-s.step, -s.step),
+                 recip = f2_pack(s.recip, s.recip), half = f2_pack(0.5f, 0.5f);
+#pragma unroll
+  for (int j = 6; j >= 0; j -= 2) {
+    const uint64_t d = f2_add(f2_pack(x[j], x[j + 1]), neg_mn);
+    uint64_t q = f2_mul(d, recip);
+    q = f2_fma(f2_fma(q, neg_step, d), recip, q);
+    q = f2_fma(f2_fma(q, neg_step, d), recip, q);
+    float lo, hi;
+    f2_unpack(f2_add(q, half), lo, hi);
+    // 0 <= x - mn <= mx - mn, and step is (mx - mn) / 15 to half an ulp: the
+    // quotient is at most 15 (1 + 2^-23), so no clamp is needed; NaN gives 0
+    codes = (codes << 8) | (uint32_t)((int)hi * 16 + (int)lo);
+  }
+  return codes;
 }
 __device__ __forceinline__ uint32_t slot_rulers(const SlotScale& s) {
   return (uint32_t)__half_as_ushort(__float2half_rn(s.mn)) |

@@ -117,52 +117,78 @@ __device__ __forceinline__ uint4 pack8(const float (&y)[8]) {
 }
 
 // The turned row's 8 values.  cs: cos and sin of pairs pair0..pair0+3, of
-// which the first `on` turn.
+// which the first `on` turn.  Every product and sum is rounded by itself.
 template <int LAYOUT, bool BF16>
-__device__ __forceinline__ uint4 turn8(const uint4& w, const float2* cs, int on) {
+__device__ __forceinline__ uint4 turn8(const uint4& w, const float4 (&cs)[2], int on) {
+  if (on <= 0) return w;
   float x[8], y[8];
   unpack8<BF16>(w, x);
+  const float c[4] = {cs[0].x, cs[0].z, cs[1].x, cs[1].z}, s[4] = {cs[0].y, cs[0].w, cs[1].y, cs[1].w};
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const int i1 = LAYOUT == ROT_HALF ? j : 2 * j, i2 = LAYOUT == ROT_HALF ? 4 + j : 2 * j + 1;
-    const float a = x[i1], b = x[i2];
-    y[i1] = j < on ? __fsub_rn(__fmul_rn(a, cs[j].x), __fmul_rn(b, cs[j].y)) : a;
-    y[i2] = j < on ? __fadd_rn(__fmul_rn(b, cs[j].x), __fmul_rn(a, cs[j].y)) : b;
+    // scalar: packed multiplies and adds were seen contracted into one rounding
+    y[i1] = __fsub_rn(__fmul_rn(x[i1], c[j]), __fmul_rn(x[i2], s[j]));
+    y[i2] = __fadd_rn(__fmul_rn(x[i2], c[j]), __fmul_rn(x[i1], s[j]));
+  }
+  if (on < 4) {
+#pragma unroll
+    for (int j = 1; j < 4; ++j)
+      if (j >= on) y[2 * j] = x[2 * j], y[2 * j + 1] = x[2 * j + 1];
   }
   return pack8<BF16>(y);
 }
 
+// Smallest and largest of two packed 16-bit values each.
+template <bool BF16>
+__device__ __forceinline__ uint32_t min2(uint32_t a, uint32_t b) {
+  if constexpr (BF16) {
+    const __nv_bfloat162 r = __hmin2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
+  } else {
+    const __half2 r = __hmin2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
+  }
+}
+template <bool BF16>
+__device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+  if constexpr (BF16) {
+    const __nv_bfloat162 r = __hmax2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
+  } else {
+    const __half2 r = __hmax2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
+  }
+}
+
 // One row of k (turned) and v into its slot: the lanes of the row are
-// neighbours in the warp, and the whole warp takes part in the exchange.
+// neighbours in the warp, and the whole warp takes part in the exchange.  The
+// rows hold 16-bit values, so their extremes are found on packed ones: k's in
+// the lower half of a word, v's in the upper.
 template <int D, int LAYOUT, bool BF16>
 __device__ __forceinline__ void quantize8(const uint4& kw, const uint4& vw, uint8_t* row, bool act, bool write, int li,
                                           int d0, int d1) {
-  float mn[2] = {INFINITY, INFINITY}, mx[2] = {-INFINITY, -INFINITY}, vx[8], kx[8];
-  unpack8<BF16>(vw, vx);
-  unpack8<BF16>(kw, kx);
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    if (act) {
-      mn[0] = fminf(mn[0], kx[j]), mx[0] = fmaxf(mx[0], kx[j]);
-      mn[1] = fminf(mn[1], vx[j]), mx[1] = fmaxf(mx[1], vx[j]);
-    }
-  }
+  constexpr uint32_t INF = BF16 ? 0x7F807F80u : 0x7C007C00u, NEG_INF = INF | 0x80008000u;
+  const uint32_t k_lo = min2<BF16>(min2<BF16>(kw.x, kw.y), min2<BF16>(kw.z, kw.w));
+  const uint32_t k_hi = max2<BF16>(max2<BF16>(kw.x, kw.y), max2<BF16>(kw.z, kw.w));
+  const uint32_t v_lo = min2<BF16>(min2<BF16>(vw.x, vw.y), min2<BF16>(vw.z, vw.w));
+  const uint32_t v_hi = max2<BF16>(max2<BF16>(vw.x, vw.y), max2<BF16>(vw.z, vw.w));
+  uint32_t lo = min2<BF16>(__byte_perm(k_lo, v_lo, 0x5410), __byte_perm(k_lo, v_lo, 0x7632));
+  uint32_t hi = max2<BF16>(__byte_perm(k_hi, v_hi, 0x5410), __byte_perm(k_hi, v_hi, 0x7632));
+  if (!act) lo = INF, hi = NEG_INF;
 #pragma unroll
   for (int o = RotGeom<D>::LANES / 2; o > 0; o >>= 1) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      mn[i] = fminf(mn[i], __shfl_xor_sync(0xffffffffu, mn[i], o));
-      mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], o));
-    }
+    lo = min2<BF16>(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+    hi = max2<BF16>(hi, __shfl_xor_sync(0xffffffffu, hi, o));
   }
   if (!write) return;
-  const SlotScale ks = slot_scale(mn[0], mx[0]), vs = slot_scale(mn[1], mx[1]);
-  uint32_t kc = 0u, vc = 0u;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    kc |= slot_code(kx[j], ks) << (4 * j);
-    vc |= slot_code(vx[j], vs) << (4 * j);
-  }
+  const SlotScale ks = slot_scale(from16<BF16>(lo & 0xFFFFu), from16<BF16>(hi & 0xFFFFu));
+  const SlotScale vs = slot_scale(from16<BF16>(lo >> 16), from16<BF16>(hi >> 16));
+  float x[8];
+  unpack8<BF16>(kw, x);
+  const uint32_t kc = slot_codes8(x, ks);
+  unpack8<BF16>(vw, x);
+  const uint32_t vc = slot_codes8(x, vs);
   if (LAYOUT == ROT_HALF) {
     *reinterpret_cast<uint16_t*>(row + d0 / 2) = (uint16_t)kc;
     *reinterpret_cast<uint16_t*>(row + d1 / 2) = (uint16_t)(kc >> 16);
@@ -224,11 +250,8 @@ __global__ void __launch_bounds__(kRotThreads, 4) rotary_kernel(const RotaryPara
     }
     __syncthreads();
   };
-  auto pairs_of = [&](int t, float2 (&cs)[4]) {
-    const float4 a = act ? s_cs4[t][pair0 / 2] : make_float4(0.f, 0.f, 0.f, 0.f);
-    const float4 b = act ? s_cs4[t][pair0 / 2 + 1] : a;
-    cs[0] = make_float2(a.x, a.y), cs[1] = make_float2(a.z, a.w);
-    cs[2] = make_float2(b.x, b.y), cs[3] = make_float2(b.z, b.w);
+  auto pairs_of = [&](int t, float4 (&cs)[2]) {
+    if (act) cs[0] = s_cs4[t][pair0 / 2], cs[1] = s_cs4[t][pair0 / 2 + 1];
   };
 
   bool first = true;
@@ -261,7 +284,7 @@ __global__ void __launch_bounds__(kRotThreads, 4) rotary_kernel(const RotaryPara
 #pragma unroll
       for (int r = 0; r < ROWS; ++r) {
         const bool live = tt[r] < nt;
-        float2 cs[4];
+        float4 cs[2] = {};
         pairs_of(live ? tt[r] : 0, cs);
         const uint4 y = turn8<LAYOUT, BF16>(x[r], cs, on);
         if (live && act && k_out)
@@ -301,7 +324,7 @@ __global__ void __launch_bounds__(kRotThreads, 4) rotary_kernel(const RotaryPara
 #pragma unroll
       for (int r = 0; r < kRotRows; ++r) {
         if (!act || tt[r] >= nt) continue;
-        float2 cs[4];
+        float4 cs[2] = {};
         pairs_of(tt[r], cs);
         store8<LAYOUT>(out[r], d0, d1, turn8<LAYOUT, BF16>(x[r], cs, on));
       }

@@ -1,6 +1,6 @@
 // tcgen05.cuh -- inline-PTX wrappers of the 5th-generation tensor core
 // (sm_100a): tensor memory, tcgen05.mma with operands in shared or tensor
-// memory, shared-memory matrix descriptors, and packed fp32 arithmetic.
+// memory, and shared-memory matrix descriptors.
 #pragma once
 
 #include "ptx.cuh"
@@ -103,31 +103,6 @@ __device__ __forceinline__ void regs_raise() {
 template <int N>
 __device__ __forceinline__ void regs_lower() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
-}
-
-// ------------------------------------------------------- packed fp32 pairs --
-__device__ __forceinline__ uint64_t f2_pack(float lo, float hi) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-  return r;
-}
-__device__ __forceinline__ void f2_unpack(uint64_t x, float& lo, float& hi) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(x));
-}
-__device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
 }
 
 }  // namespace slmt
