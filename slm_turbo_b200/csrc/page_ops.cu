@@ -207,17 +207,18 @@ struct Vec8<float> {
 };
 
 // A thread keeps its place in a token's slots (head, K or V, piece) and walks
-// over tokens, four at a time so that their slot ids and code words are in
-// flight together; places are found once, with 32-bit arithmetic.
+// over tokens, four at a time; places are found once, with 32-bit arithmetic.
+// The next four tokens' slot ids are fetched two steps ahead and their code
+// words one step ahead of their conversion.
 constexpr int kLoadThreads = 256;
 constexpr int kLoadUnroll = 4;
 
 template <int D, typename T>
 __global__ void __launch_bounds__(kLoadThreads)
     load_kernel(const uint8_t* __restrict__ cache, int64_t num_slots, const int64_t* __restrict__ slot_mapping,
-                int64_t num_tokens, int kv, int places, int sub_tokens, T* __restrict__ key, T* __restrict__ value,
-                int32_t* err) {
-  constexpr int PIECES = D / 4;  // 8-value pieces of a row's K and V
+                int64_t num_tokens, int kv, int places, int sub_tokens, int steps, T* __restrict__ key,
+                T* __restrict__ value, int32_t* err) {
+  constexpr int PIECES = D / 4, U = kLoadUnroll;  // 8-value pieces of a row's K and V
   // `places` pieces of a token in this block's pass (kv * PIECES when a block
   // holds whole tokens, sub_tokens of them; else a part, by blockIdx.y)
   const int sub = threadIdx.x / places;
@@ -226,52 +227,70 @@ __global__ void __launch_bounds__(kLoadThreads)
   const int h = place / PIECES, piece = place - h * PIECES;
   const int which = piece >= PIECES / 2, c = piece - which * (PIECES / 2);
   const int64_t slot_bytes = (int64_t)kv * (D + 8);
-  const uint8_t* base = cache + (int64_t)h * (D + 8);
-  const int code_at = which * (D / 2) + 4 * c, ruler_at = D + 4 * which;
+  const uint8_t* code_base = cache + (int64_t)h * (D + 8) + which * (D / 2) + 4 * c;
+  const int to_ruler = D + 4 * which - which * (D / 2) - 4 * c;
   T* out = (which ? value : key) + (int64_t)h * D + 8 * c;
-  const int64_t t0 = (int64_t)blockIdx.x * (sub_tokens * kLoadUnroll) + sub;
-  int64_t slot[kLoadUnroll];
-  uint32_t codes[kLoadUnroll], rulers[kLoadUnroll];
+  int64_t t = (int64_t)blockIdx.x * (sub_tokens * U) * steps + sub;  // first token of this step
+  int64_t slot[U];
+  uint32_t codes[U], rulers[U];
+  auto fetch_slots = [&](int64_t from) {
 #pragma unroll
-  for (int u = 0; u < kLoadUnroll; ++u) {
-    const int64_t t = t0 + u * sub_tokens;
-    slot[u] = t < num_tokens ? slot_mapping[t] : -1;
-  }
-#pragma unroll
-  for (int u = 0; u < kLoadUnroll; ++u) {
-    codes[u] = rulers[u] = 0u;  // code 0, min 0: a row of zeros
-    if (slot[u] >= 0 && slot[u] < num_slots) {
-      const uint8_t* s = base + slot[u] * slot_bytes;
-      codes[u] = *reinterpret_cast<const uint32_t*>(s + code_at);
-      rulers[u] = *reinterpret_cast<const uint32_t*>(s + ruler_at);
-    } else if (slot[u] >= num_slots && place == 0) {
-      set_error(err, SLMT_DEVERR_SLOT);
+    for (int u = 0; u < U; ++u) {
+      const int64_t tok = from + u * sub_tokens;
+      slot[u] = tok < num_tokens ? slot_mapping[tok] : -1;
     }
-  }
+  };
+  auto fetch_codes = [&] {
 #pragma unroll
-  for (int u = 0; u < kLoadUnroll; ++u) {
-    const int64_t t = t0 + u * sub_tokens;
-    if (t >= num_tokens) return;
-    const float mn = half_bits_to_float((uint16_t)(rulers[u] & 0xFFFFu));
-    const float st = half_bits_to_float((uint16_t)(rulers[u] >> 16));
-    // A nibble left where it is under the bits of 2^23 is the float 2^23 +
-    // code * 16^j: one multiply-add with 16^-j and -2^23 16^-j gives the code,
-    // exactly, without shifts or integer conversions.  Five nibbles fit below
-    // bit 23; the others are taken from the word shifted once.
-    const uint64_t st2 = f2_pack(st, st), mn2 = f2_pack(mn, mn);
-    const uint32_t w0 = codes[u], w1 = codes[u] >> 16;
-    float x[8];
-#pragma unroll
-    for (int j = 0; j < 8; j += 2) {
-      const uint32_t w = j < 4 ? w0 : w1;
-      const int k = j & 3;  // nibbles k and k + 1 of w
-      const float s0 = 1.f / (float)(1 << (4 * k)), s1 = s0 / 16.f;
-      const uint64_t biased = f2_pack(__uint_as_float((w & (15u << (4 * k))) | 0x4B000000u),
-                                      __uint_as_float((w & (15u << (4 * k + 4))) | 0x4B000000u));
-      const uint64_t code = f2_fma(biased, f2_pack(s0, s1), f2_pack(-8388608.f * s0, -8388608.f * s1));
-      f2_unpack(f2_fma(code, st2, mn2), x[j], x[j + 1]);
+    for (int u = 0; u < U; ++u) {
+      codes[u] = rulers[u] = 0u;  // code 0, min 0: a row of zeros
+      if ((uint64_t)slot[u] < (uint64_t)num_slots) {
+        const uint8_t* s = code_base + slot[u] * slot_bytes;
+        codes[u] = *reinterpret_cast<const uint32_t*>(s);
+        rulers[u] = *reinterpret_cast<const uint32_t*>(s + to_ruler);
+      } else if (slot[u] >= 0 && place == 0) {
+        set_error(err, SLMT_DEVERR_SLOT);
+      }
     }
-    Vec8<T>::store(out + t * kv * D, x);
+  };
+  fetch_slots(t);
+  fetch_codes();
+  if (steps > 1) fetch_slots(t + U * sub_tokens);
+#pragma unroll 1
+  for (int step = 0; step < steps; ++step) {
+    uint32_t now_codes[U], now_rulers[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) now_codes[u] = codes[u], now_rulers[u] = rulers[u];
+    if (step + 1 < steps) {
+      fetch_codes();
+      if (step + 2 < steps) fetch_slots(t + 2 * U * sub_tokens);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t tok = t + u * sub_tokens;
+      if (tok >= num_tokens) return;
+      const float mn = half_bits_to_float((uint16_t)(now_rulers[u] & 0xFFFFu));
+      const float st = half_bits_to_float((uint16_t)(now_rulers[u] >> 16));
+      // A nibble left where it is under the bits of 2^23 is the float 2^23 +
+      // code * 16^j: one multiply-add with 16^-j and -2^23 16^-j gives the
+      // code, exactly, without shifts or integer conversions.  Five nibbles
+      // fit below bit 23; four are taken from the word as it is, four shifted.
+      const uint64_t st2 = f2_pack(st, st), mn2 = f2_pack(mn, mn);
+      const uint32_t w0 = now_codes[u], w1 = w0 >> 16;
+      float x[8];
+#pragma unroll
+      for (int j = 0; j < 8; j += 2) {
+        const uint32_t w = j < 4 ? w0 : w1;
+        const int k = j & 3;  // nibbles k and k + 1 of w
+        const float s0 = 1.f / (float)(1 << (4 * k)), s1 = s0 / 16.f;
+        const uint64_t biased = f2_pack(__uint_as_float((w & (15u << (4 * k))) | 0x4B000000u),
+                                        __uint_as_float((w & (15u << (4 * k + 4))) | 0x4B000000u));
+        const uint64_t code = f2_fma(biased, f2_pack(s0, s1), f2_pack(-8388608.f * s0, -8388608.f * s1));
+        f2_unpack(f2_fma(code, st2, mn2), x[j], x[j + 1]);
+      }
+      Vec8<T>::store(out + tok * kv * D, x);
+    }
+    t += U * sub_tokens;
   }
 }
 
@@ -282,10 +301,13 @@ int load_launch_typed(const uint8_t* cache, int64_t num_slots, const int64_t* sl
   const int places = (int)std::min<int64_t>(all, kLoadThreads);
   const int sub_tokens = kLoadThreads / places;
   const int64_t parts = (all + kLoadThreads - 1) / kLoadThreads;
-  const int64_t per_block = (int64_t)sub_tokens * kLoadUnroll, blocks = (tokens + per_block - 1) / per_block;
+  const int64_t per_step = (int64_t)sub_tokens * kLoadUnroll, all_steps = (tokens + per_step - 1) / per_step;
+  // several steps per block once every SM has its 6 blocks of a step each
+  const int64_t steps = std::max<int64_t>(1, std::min<int64_t>(8, all_steps * parts / (148 * 6)));
+  const int64_t blocks = (all_steps + steps - 1) / steps;
   if (blocks > INT32_MAX || parts > 65535) return SLMT_ERR_UNSUPPORTED;
   load_kernel<D, T><<<dim3((unsigned)blocks, (unsigned)parts), kLoadThreads, 0, st>>>(
-      cache, num_slots, slot_mapping, tokens, kv, places, sub_tokens, (T*)key, (T*)value, err);
+      cache, num_slots, slot_mapping, tokens, kv, places, sub_tokens, (int)steps, (T*)key, (T*)value, err);
   return launch_status();
 }
 
