@@ -55,7 +55,7 @@ struct PromptParams {
 };
 
 struct PromptCtl {
-  uint64_t q_full[2], q_empty[2], s_full[2], p_ready[2], o_full[2], drain;
+  uint64_t q_full[2], q_empty[2], s_full[2], p_half[2], p_ready[2], o_full[2], drain;
   uint64_t kv_full[kMaxStages], kv_empty[kMaxStages], v_ok[kMaxStages];
   uint32_t tmem;
   uint32_t tile_bad[2];
@@ -128,6 +128,39 @@ __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
   }
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t exp2_mufu(uint64_t x) {
+  float lo, hi;
+  f2_unpack(x, lo, hi);
+  return f2_pack(exp2_approx(lo), exp2_approx(hi));
+}
+// 2^x on the FMA pipe, for part of the weights: the exponential unit gives 16
+// results a clock and SM and would bound the kernel.  x = n + f with n the
+// nearest integer (by adding 1.5 * 2^23), 2^f on [-1/2, 1/2] by the degree-4
+// polynomial of least relative error (2^-18.5), 2^n from n's bits.  From -127
+// down 2^n is zero, -inf among them; NaN stays NaN.  x is below 2^7.
+__device__ __forceinline__ uint64_t exp2_fma(uint64_t x) {
+  float lo, hi;
+  f2_unpack(x, lo, hi);
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(lo) : "f"(-127.f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(hi) : "f"(-127.f));
+  x = f2_pack(lo, hi);
+  constexpr float MAGIC = 12582912.f + 127.f;
+  const uint64_t t = f2_add(x, f2_pack(MAGIC, MAGIC));
+  const uint64_t f = f2_add(x, f2_add(f2_pack(MAGIC, MAGIC), t ^ 0x8000000080000000ull));
+  uint64_t r = f2_fma(f, f2_pack(0x1.3997d6p-7f, 0x1.3997d6p-7f), f2_pack(0x1.ca1440p-5f, 0x1.ca1440p-5f));
+  r = f2_fma(r, f, f2_pack(0x1.ec06dap-3f, 0x1.ec06dap-3f));
+  r = f2_fma(r, f, f2_pack(0x1.62e0dcp-1f, 0x1.62e0dcp-1f));
+  r = f2_fma(r, f, f2_pack(0x1.ffffe8p-1f, 0x1.ffffe8p-1f));
+  f2_unpack(t, lo, hi);
+  const uint64_t scale = f2_pack(__uint_as_float(__float_as_uint(lo) << 23), __uint_as_float(__float_as_uint(hi) << 23));
+  return f2_mul(r, scale);
+}
+
 // Write 16 finished columns of an output row.
 __device__ __forceinline__ void store16(void* out, int out_dtype, int64_t at, const float* x) {
   if (out_dtype == SLMT_DTYPE_F32) {
@@ -167,7 +200,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (tid == 0) {
     for (int x = 0; x < 2; ++x) {
       mbar_init(&c->q_full[x], 1), mbar_init(&c->q_empty[x], 1);
-      mbar_init(&c->s_full[x], 1), mbar_init(&c->p_ready[x], 128);
+      mbar_init(&c->s_full[x], 1);
+      mbar_init(&c->p_half[x], 128), mbar_init(&c->p_ready[x], 128);
       mbar_init(&c->o_full[x], 2);  // the commit, and the thread that set tile_bad
     }
     for (int s = 0; s < STAGES; ++s) {
@@ -260,102 +294,117 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     } else if (warp == 8) {
       // ----------------------------------------------------------- products
-      if (lane == 0) {
-        constexpr uint32_t idesc_s = mma_idesc(BF16, 128, 128, false), idesc_o = mma_idesc(BF16, 128, D, true);
-        const uint32_t q_addr = smem_addr(smem), ring_addr = smem_addr(ring);
-        uint32_t fill = 0, nq[2] = {0, 0}, np[2] = {0, 0}, ok_phase = 0;
-        auto full = [&](uint32_t f) { return mbar_wait(&c->kv_full[f % STAGES], (f / STAGES) & 1u, limit); };
-        auto scores = [&](int x, uint32_t f) {
-          const uint32_t a = q_addr + x * TILE, b = ring_addr + (f % STAGES) * TILE;
+      // The whole warp walks and waits, so that what the products need is the
+      // same in every lane; one lane issues.
+      constexpr uint32_t idesc_s = mma_idesc(BF16, 128, 128, false), idesc_o = mma_idesc(BF16, 128, D, true);
+      constexpr uint32_t HI = desc_hi(1024);
+      const bool leader = elect_one();
+      const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+      const uint32_t q_lo = desc_lo(smem_addr(smem), 16), k_lo = desc_lo(smem_addr(ring), 16),
+                     v_lo = desc_lo(smem_addr(ring), 16384);
+      uint32_t fill = 0, nq[2] = {0, 0}, np[2] = {0, 0}, ok_phase = 0;
+      auto wait = [&](uint64_t* bar, uint32_t phase) {
+        return __all_sync(0xffffffffu, mbar_wait(bar, phase & 1u, limit));
+      };
+      auto full = [&](uint32_t f) { return wait(&c->kv_full[f % STAGES], f / STAGES); };
+      auto commit = [&](uint64_t* bar) {
+        if (leader) mma_commit(bar);
+      };
+      auto scores = [&](int x, uint32_t f) {
+        const uint32_t a = q_lo + x * (TILE >> 4), b = k_lo + (f % STAGES) * (TILE >> 4);
+        if (leader) {
 #pragma unroll
           for (int u = 0; u < D / 16; ++u) {
-            const uint32_t off = (u >> 2) * 16384 + (u & 3) * 32;
-            mma_ss(tmem + col_s + 128 * x, smem_desc(a + off, 16, 1024), smem_desc(b + off, 16, 1024), idesc_s, u > 0);
+            const uint32_t off = ((u >> 2) * 16384 + (u & 3) * 32) >> 4;
+            mma_ss(tm + col_s + 128 * x, a + off, HI, b + off, HI, idesc_s, u > 0);
           }
           mma_commit(&c->s_full[x]);
-        };
-        auto weigh = [&](int x, uint32_t f, bool first) {
-          const uint32_t b = ring_addr + (f % STAGES) * TILE;
+        }
+      };
+      // half the keys at a time: the first half's weights are there while the
+      // second half's are still being computed
+      auto weigh = [&](int x, uint32_t f, bool first, int half) {
+        const uint32_t b = v_lo + (f % STAGES) * (TILE >> 4);
+        if (leader) {
 #pragma unroll
-          for (int u = 0; u < 8; ++u)
-            mma_ts(tmem + col_o + D * x, tmem + col_s + 128 * x + 8 * u, smem_desc(b + u * 2048, 16384, 1024), idesc_o,
-                   !first || u > 0);
-        };
-        auto wait_q = [&](int x) { return mbar_wait(&c->q_full[x], nq[x]++ & 1u, limit); };
-        auto wait_p = [&](int x) {
-          const bool ok = mbar_wait(&c->p_ready[x], np[x]++ & 1u, limit);
-          tc_fence_after();
-          return ok;
-        };
-        Walk w;
-        Item it;
-        w.begin(c);
-        while (!failed && w.next(c, p, it)) {
-          uint32_t bad = 0;
-          bool ok = full(fill) && wait_q(0);
-          if (!ok) {
+          for (int u = 4 * half; u < 4 * half + 4; ++u)
+            mma_ts(tm + col_o + D * x, tm + col_s + 128 * x + 8 * u, b + u * (2048 >> 4), HI, idesc_o,
+                   u > 0 || !first);
+        }
+      };
+      Walk w;
+      Item it;
+      w.begin(c);
+      while (!failed && w.next(c, p, it)) {
+        const int steps[2] = {__shfl_sync(0xffffffffu, it.steps[0], 0), __shfl_sync(0xffffffffu, it.steps[1], 0)};
+        const int nk = max(steps[0], steps[1]), guard = __shfl_sync(0xffffffffu, it.guard, 0);
+        uint32_t bad = 0;
+        if (!full(fill)) failed = true;
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          if (failed || steps[x] == 0) continue;
+          if (!wait(&c->q_full[x], nq[x]++)) {
+            failed = true;
+            continue;
+          }
+          scores(x, fill);
+          if (steps[x] == 1) commit(&c->q_empty[x]);
+        }
+        commit(&c->kv_empty[fill % STAGES]);
+        for (int j = 0; j < nk && !failed; ++j) {
+          const uint32_t fv = fill + 2 * j + 1, fk = fv + 1;
+          if (!full(fv)) {
             failed = true;
             break;
           }
-          scores(0, fill);
-          if (it.steps[0] == 1) mma_commit(&c->q_empty[0]);
-          if (it.steps[1]) {
-            if (!wait_q(1)) {
+          if (j >= guard) {
+            const uint32_t s = fv % STAGES;
+            if (!wait(&c->v_ok[s], ok_phase >> s)) {
               failed = true;
               break;
             }
-            scores(1, fill);
-            if (it.steps[1] == 1) mma_commit(&c->q_empty[1]);
+            ok_phase ^= 1u << s;
+            bad |= c->slot_bad[s][0] | c->slot_bad[s][1];
           }
-          mma_commit(&c->kv_empty[fill % STAGES]);
-          for (int j = 0; j < it.nk; ++j) {
-            const uint32_t fv = fill + 2 * j + 1, fk = fv + 1;
-            if (!full(fv)) {
-              failed = true;
-              break;
-            }
-            if (j >= it.guard) {
-              const uint32_t s = fv % STAGES;
-              if (!mbar_wait(&c->v_ok[s], (ok_phase >> s) & 1u, limit)) {
-                failed = true;
-                break;
-              }
-              ok_phase ^= 1u << s;
-              bad |= c->slot_bad[s][0] | c->slot_bad[s][1];
-            }
-            bool have_k = j + 1 >= it.nk;  // nothing to wait for
+          bool have_k = j + 1 >= nk;  // nothing to wait for
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
-              if (j >= it.steps[x]) continue;
-              if (!wait_p(x)) {
+          for (int x = 0; x < 2; ++x) {
+            if (j >= steps[x]) continue;
+            if (!wait(&c->p_half[x], np[x])) {
+              failed = true;
+              break;
+            }
+            tc_fence_after();
+            weigh(x, fv, j == 0, 0);
+            if (!wait(&c->p_ready[x], np[x]++)) {
+              failed = true;
+              break;
+            }
+            tc_fence_after();
+            weigh(x, fv, j == 0, 1);
+            if (j + 1 < steps[x]) {
+              if (!have_k && !full(fk)) {
                 failed = true;
                 break;
               }
-              weigh(x, fv, j == 0);
-              if (j + 1 < it.steps[x]) {
-                if (!have_k && !full(fk)) {
-                  failed = true;
-                  break;
-                }
-                have_k = true;
-                scores(x, fk);
-                if (j + 2 == it.steps[x]) mma_commit(&c->q_empty[x]);
-              } else {
-                c->tile_bad[x] = bad;
-                mbar_arrive(&c->o_full[x]);
-                mma_commit(&c->o_full[x]);
-              }
+              have_k = true;
+              scores(x, fk);
+              if (j + 2 == steps[x]) commit(&c->q_empty[x]);
+            } else if (leader) {
+              c->tile_bad[x] = bad;
+              mbar_arrive(&c->o_full[x]);
+              mma_commit(&c->o_full[x]);
             }
-            if (failed) break;
-            mma_commit(&c->kv_empty[fv % STAGES]);
-            if (j + 1 < it.nk) mma_commit(&c->kv_empty[fk % STAGES]);
           }
-          fill += 2 * it.nk;
+          if (failed) break;
+          commit(&c->kv_empty[fv % STAGES]);
+          if (j + 1 < nk) commit(&c->kv_empty[fk % STAGES]);
         }
-        if (failed) {  // products in flight read shared and tensor memory
-          mma_commit(&c->drain);
-          mbar_wait(&c->drain, 0, limit);
-        }
+        fill += 2 * nk;
+      }
+      if (failed) {  // products in flight read shared and tensor memory
+        commit(&c->drain);
+        wait(&c->drain, 0);
       }
     } else {
       // ------------------------------------------- non-finite values in V
@@ -406,6 +455,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     regs_raise<208>();
     constexpr float SHIFT = BF16 ? 0.f : 6.f;  // fp16 weights lie in [2^-24, 2^14]: a row's largest is 2^6 or more
     constexpr float MOVE = 8.f;
+    constexpr int FMA_EXP = 4;  // of 16 pairs
     const int x = warp >> 2, row = tid & 127;
     const int row_tok = row / p.group, row_head = row - row_tok * p.group;
     const uint32_t lane_base = (uint32_t)(warp & 3) << 21;
@@ -438,11 +488,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-        for (int i = 4; i < 128; i += 4) {
+        for (int i = 4; i < 124; i += 8) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k) mx[k] = fmaxf(mx[k], s[i + k]);
+          for (int k = 0; k < 4; ++k) mx[k] = max3(mx[k], s[i + k], s[i + 4 + k]);
         }
-        const float top = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
+#pragma unroll
+        for (int k = 0; k < 4; ++k) mx[k] = fmaxf(mx[k], s[124 + k]);
+        const float top = max3(m, max3(mx[0], mx[1], mx[2]), mx[3]);
         if (j == 0) {
           m = top;
         } else {
@@ -464,29 +516,40 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         ref = m == -INFINITY ? 0.f : m;
-        const uint64_t neg = f2_pack(-ref, -ref), scale2 = f2_pack(sc, sc), shift2 = f2_pack(SHIFT, SHIFT);
-        uint64_t acc = f2_pack(0.f, 0.f);
+        // exponents s * sc - ref * sc in one rounding: that of ref * sc is the
+        // same for the whole row and cancels, as long as it stays below one
+        float offset = fmaf(-ref, sc, SHIFT);
+        if (__any_sync(0xffffffffu, !(fabsf(ref * sc) < 0x1p20f))) {
+          // the difference first: exact near the maximum, whatever its size
+#pragma unroll
+          for (int i = 0; i < 128; ++i) s[i] -= ref;
+          offset = SHIFT;
+        }
+        const uint64_t scale2 = f2_pack(sc, sc), offset2 = f2_pack(offset, offset);
+        uint64_t acc0 = f2_pack(0.f, 0.f), acc1 = acc0;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           uint32_t w16[16];
 #pragma unroll
           for (int k = 0; k < 16; ++k) {
-            // the difference first: exact near the maximum, whatever its size
-            const uint64_t e = f2_fma(f2_add(f2_pack(s[32 * i + 2 * k], s[32 * i + 2 * k + 1]), neg), scale2, shift2);
+            uint64_t e = f2_fma(f2_pack(s[32 * i + 2 * k], s[32 * i + 2 * k + 1]), scale2, offset2);
+            e = k % 16 < FMA_EXP ? exp2_fma(e) : exp2_mufu(e);
+            if (k & 1) acc1 = f2_add(acc1, e);
+            else acc0 = f2_add(acc0, e);
             float lo, hi;
             f2_unpack(e, lo, hi);
-            lo = exp2_approx(lo), hi = exp2_approx(hi);
-            acc = f2_add(acc, f2_pack(lo, hi));
             w16[k] = pack16<BF16>(lo, hi);
           }
           tmem_st16(ts + 16 * i, w16);
+          if (i & 1) {
+            tmem_wait_st();
+            tc_fence_before();
+            mbar_arrive(i == 1 ? &c->p_half[x] : &c->p_ready[x]);
+          }
         }
         float a0, a1;
-        f2_unpack(acc, a0, a1);
+        f2_unpack(f2_add(acc0, acc1), a0, a1);
         sum += a0 + a1;
-        tmem_wait_st();
-        tc_fence_before();
-        mbar_arrive(&c->p_ready[x]);
       }
       if (failed) break;
       if (!__all_sync(0xffffffffu, mbar_wait(&c->o_full[x], no++ & 1u, limit))) {
@@ -499,26 +562,27 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int h = it.head * p.group + row_head;
       const int64_t at = (int64_t)(it.start + tok) * p.o_tok + (int64_t)h * p.o_head;
       const bool bad = c->tile_bad[x] != 0;
-#pragma unroll 1
-      for (int i = 0; i < D / 16; ++i) {
-        float o[16];
-        tmem_ld16(o, to + 16 * i);
-        tmem_wait_ld();
+      float o[D];
 #pragma unroll
-        for (int k = 0; k < 16; ++k) o[k] *= inv;
-        if (bad && valid) {
-          // the values taken out of the V tiles, for the rows that attend to them
-          for (int j = 128 * it.guard; j <= tok; ++j) {
-            const uint16_t* v = reinterpret_cast<const uint16_t*>(p.v) + (int64_t)(it.start + j) * p.v_tok +
-                                (int64_t)it.head * p.v_head + 16 * i;
+      for (int i = 0; i < D / 16; ++i) tmem_ld16(o + 16 * i, to + 16 * i);
+      tmem_wait_ld();
+      if (bad && valid) {
+        // the values taken out of the V tiles, for the rows that attend to them
+        for (int j = 128 * it.guard; j <= tok; ++j) {
+          const uint16_t* v = reinterpret_cast<const uint16_t*>(p.v) + (int64_t)(it.start + j) * p.v_tok +
+                              (int64_t)it.head * p.v_head;
 #pragma unroll
-            for (int k = 0; k < 16; ++k) {
-              const float y = BF16 ? __bfloat162float(__ushort_as_bfloat16(v[k])) : __half2float(__ushort_as_half(v[k]));
-              if (!(y - y == 0.f)) o[k] += y;
-            }
+          for (int k = 0; k < D; ++k) {
+            const float y = BF16 ? __bfloat162float(__ushort_as_bfloat16(v[k])) : __half2float(__ushort_as_half(v[k]));
+            if (!(y - y == 0.f)) o[k] += y;
           }
         }
-        if (valid) store16(p.out, p.out_dtype, at + 16 * i, o);
+      }
+#pragma unroll
+      for (int k = 0; k < D; ++k) o[k] *= inv;
+      if (valid) {
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) store16(p.out, p.out_dtype, at + 16 * i, o + 16 * i);
       }
       tc_fence_before();  // O is read before the next item's first product overwrites it
     }
