@@ -12,11 +12,19 @@
 //   P = exp2((S - m) scale log2 e)   rounded to the inputs' type, over S in TMEM
 //   O += P V    tcgen05.mma, P from TMEM, V in shared memory as it was copied
 //
-// Warps 0-3 and 4-7 are the softmax of tile A and of tile B, a row per thread;
-// while one of them works on its scores, the tensor core computes the other
-// tile's products.  Warp 8 issues the products, warp 9 the tiled copies into
-// a ring of K and V tiles, warps 10 and 11 look at the V tiles on the
-// diagonal (below).  Every role walks the same list of items by itself.
+// Warps 0-3 and 4-7 are the softmax of tile A and of tile B, a row per thread.
+// A tile's scores are made 64 keys at a time into two halves of its 128
+// columns: while the softmax works on one half, the tensor core weighs V with
+// the other half's P and replaces that half by the next key tile's scores, so
+// neither waits for the other.  (With scores of 128 keys at once a tile's
+// softmax and its products took turns; 64 keys cost S 256 + 2 * 64 cycles
+// instead of half of 512, as both operands come from shared memory.)  Warps 8
+// and 9 issue the products, one for each tile: the tensor core's queue is
+// short, and one warp's waits between two tiles would leave it empty.  Warp 10
+// issues the tiled copies into a ring of K and V tiles, warp 11 looks at the V
+// tiles on the diagonal (below).  Every role walks the same list of items
+// by itself; the next item's first scores go out as soon as its tile's last
+// weights are used.
 //
 // Running maximum: the reference m of a row moves only when a score passes it
 // by more than 2^8 in weight; until then old weights stay on their scale, and
@@ -55,11 +63,12 @@ struct PromptParams {
 };
 
 struct PromptCtl {
-  uint64_t q_full[2], q_empty[2], s_full[2], p_half[2], p_ready[2], o_full[2], drain;
+  uint64_t q_full[2], q_empty[2], o_full[2], pv_done[2], drain[2];
+  uint64_t s_full[2][2], p_ready[2][2];  // [tile][half of its columns]
   uint64_t kv_full[kMaxStages], kv_empty[kMaxStages], v_ok[kMaxStages];
   uint32_t tmem;
   uint32_t tile_bad[2];
-  uint32_t slot_bad[kMaxStages][2];
+  uint32_t slot_bad[kMaxStages];
   uint32_t sort_key[kMaxReqs];  // (pairs of tiles << kReqBits) | request, descending
   int start[kMaxReqs], rows[kMaxReqs];
 };
@@ -78,9 +87,9 @@ struct Item {
   int req, head;     // request of this launch, kv head
   int start, rows;   // the request's first row and its number of rows
   int tok[2];        // first token of tile A and B
-  int steps[2];      // key tiles of each (0: no rows in tile B)
-  int nk;            // key tiles loaded
-  int guard;         // first key tile that some row of A or B does not see whole
+  int steps[2];      // 64-key steps of each (0: no rows in tile B)
+  int nk;            // 128-key tiles loaded
+  int guard;         // first of these that some row of A or B does not see whole
 };
 
 // The items in the order of falling cost -- requests' last tiles first -- dealt
@@ -110,9 +119,9 @@ struct Walk {
     it.rows = c->rows[it.req];
     it.tok[0] = level * 2 * p.tile_tokens;
     it.tok[1] = it.tok[0] + p.tile_tokens;
-    it.steps[0] = (min(it.tok[1], it.rows) + 127) >> 7;
-    it.steps[1] = it.tok[1] < it.rows ? (min(it.tok[1] + p.tile_tokens, it.rows) + 127) >> 7 : 0;
-    it.nk = max(it.steps[0], it.steps[1]);
+    it.steps[0] = (min(it.tok[1], it.rows) + 63) >> 6;
+    it.steps[1] = it.tok[1] < it.rows ? (min(it.tok[1] + p.tile_tokens, it.rows) + 63) >> 6 : 0;
+    it.nk = (max(it.steps[0], it.steps[1]) + 1) >> 1;
     it.guard = (it.tok[0] + 1) >> 7;
     return true;
   }
@@ -133,34 +142,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
-__device__ __forceinline__ uint64_t exp2_mufu(uint64_t x) {
-  float lo, hi;
-  f2_unpack(x, lo, hi);
-  return f2_pack(exp2_approx(lo), exp2_approx(hi));
-}
-// 2^x on the FMA pipe, for part of the weights: the exponential unit gives 16
-// results a clock and SM and would bound the kernel.  x = n + f with n the
-// nearest integer (by adding 1.5 * 2^23), 2^f on [-1/2, 1/2] by the degree-4
-// polynomial of least relative error (2^-18.5), 2^n from n's bits.  From -127
-// down 2^n is zero, -inf among them; NaN stays NaN.  x is below 2^7.
-__device__ __forceinline__ uint64_t exp2_fma(uint64_t x) {
-  float lo, hi;
-  f2_unpack(x, lo, hi);
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(lo) : "f"(-127.f));
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(hi) : "f"(-127.f));
-  x = f2_pack(lo, hi);
-  constexpr float MAGIC = 12582912.f + 127.f;
-  const uint64_t t = f2_add(x, f2_pack(MAGIC, MAGIC));
-  const uint64_t f = f2_add(x, f2_add(f2_pack(MAGIC, MAGIC), t ^ 0x8000000080000000ull));
-  uint64_t r = f2_fma(f, f2_pack(0x1.3997d6p-7f, 0x1.3997d6p-7f), f2_pack(0x1.ca1440p-5f, 0x1.ca1440p-5f));
-  r = f2_fma(r, f, f2_pack(0x1.ec06dap-3f, 0x1.ec06dap-3f));
-  r = f2_fma(r, f, f2_pack(0x1.62e0dcp-1f, 0x1.62e0dcp-1f));
-  r = f2_fma(r, f, f2_pack(0x1.ffffe8p-1f, 0x1.ffffe8p-1f));
-  f2_unpack(t, lo, hi);
-  const uint64_t scale = f2_pack(__uint_as_float(__float_as_uint(lo) << 23), __uint_as_float(__float_as_uint(hi) << 23));
-  return f2_mul(r, scale);
-}
-
 // Write 16 finished columns of an output row.
 __device__ __forceinline__ void store16(void* out, int out_dtype, int64_t at, const float* x) {
   if (out_dtype == SLMT_DTYPE_F32) {
@@ -200,16 +181,16 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (tid == 0) {
     for (int x = 0; x < 2; ++x) {
       mbar_init(&c->q_full[x], 1), mbar_init(&c->q_empty[x], 1);
-      mbar_init(&c->s_full[x], 1);
-      mbar_init(&c->p_half[x], 128), mbar_init(&c->p_ready[x], 128);
+      for (int h = 0; h < 2; ++h) mbar_init(&c->s_full[x][h], 1), mbar_init(&c->p_ready[x][h], 128);
+      mbar_init(&c->pv_done[x], 1);
       mbar_init(&c->o_full[x], 2);  // the commit, and the thread that set tile_bad
     }
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(&c->kv_full[s], 1);
-      mbar_init(&c->kv_empty[s], s & 1 ? 3 : 1);  // V tiles: the commit and both guard warps
-      mbar_init(&c->v_ok[s], 2);
+      mbar_init(&c->kv_empty[s], s & 1 ? 3 : 2);  // both tiles' products; V tiles: and the guard warp
+      mbar_init(&c->v_ok[s], 1);
     }
-    mbar_init(&c->drain, 1);
+    mbar_init(&c->drain[0], 1), mbar_init(&c->drain[1], 1);
     fence_mbar_init();
   }
   if (warp == 8) tmem_alloc(&c->tmem, kTmemCols);
@@ -254,8 +235,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   bool failed = false;
   if (warp >= 8) {
-    regs_lower<88>();
-    if (warp == 9) {
+    if (warp == 10) {
       // ------------------------------------------------------------ copies
       if (lane == 0) {
         uint32_t fill = 0, nq[2] = {0, 0};
@@ -292,124 +272,131 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int x = 0; x < 2; ++x)
           if (nq[x] && !mbar_wait(&c->q_full[x], (nq[x] - 1) & 1u, limit)) failed = true;
       }
-    } else if (warp == 8) {
+    } else if (warp < 10) {
       // ----------------------------------------------------------- products
       // The whole warp walks and waits, so that what the products need is the
-      // same in every lane; one lane issues.
-      constexpr uint32_t idesc_s = mma_idesc(BF16, 128, 128, false), idesc_o = mma_idesc(BF16, 128, D, true);
+      // same in every lane and stays in uniform registers; one lane issues.
+      constexpr uint32_t idesc_s = mma_idesc(BF16, 128, 64, false), idesc_o = mma_idesc(BF16, 128, D, true);
       constexpr uint32_t HI = desc_hi(1024);
+      const int x = __shfl_sync(0xffffffffu, warp - 8, 0);
       const bool leader = elect_one();
       const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
-      const uint32_t q_lo = desc_lo(smem_addr(smem), 16), k_lo = desc_lo(smem_addr(ring), 16),
+      const uint32_t t_s = tm + col_s + 128 * x, t_o = tm + col_o + D * x;
+      const uint32_t q_lo = desc_lo(smem_addr(smem), 16) + x * (TILE >> 4), k_lo = desc_lo(smem_addr(ring), 16),
                      v_lo = desc_lo(smem_addr(ring), 16384);
-      uint32_t fill = 0, nq[2] = {0, 0}, np[2] = {0, 0}, ok_phase = 0;
+      uint32_t fill = 0, nq = 0, p_phase = 0, ok_phase = 0;
       auto wait = [&](uint64_t* bar, uint32_t phase) {
-        return __all_sync(0xffffffffu, mbar_wait(bar, phase & 1u, limit));
+        const bool ok = __all_sync(0xffffffffu, mbar_wait(bar, phase & 1u, limit));
+        failed |= !ok;
+        return ok;
       };
       auto full = [&](uint32_t f) { return wait(&c->kv_full[f % STAGES], f / STAGES); };
-      auto commit = [&](uint64_t* bar) {
-        if (leader) mma_commit(bar);
-      };
-      auto scores = [&](int x, uint32_t f) {
-        const uint32_t a = q_lo + x * (TILE >> 4), b = k_lo + (f % STAGES) * (TILE >> 4);
+      // scores with half h of the keys of fill f
+      auto scores = [&](int h, uint32_t f, bool last) {
+        const uint32_t b = k_lo + (f % STAGES) * (TILE >> 4) + h * (8192 >> 4);
         if (leader) {
 #pragma unroll
           for (int u = 0; u < D / 16; ++u) {
             const uint32_t off = ((u >> 2) * 16384 + (u & 3) * 32) >> 4;
-            mma_ss(tm + col_s + 128 * x, a + off, HI, b + off, HI, idesc_s, u > 0);
+            mma_ss(t_s + 64 * h, q_lo + off, HI, b + off, HI, idesc_s, u > 0);
           }
-          mma_commit(&c->s_full[x]);
+          mma_commit(&c->s_full[x][h]);
+          if (last) mma_commit(&c->q_empty[x]);
         }
       };
-      // half the keys at a time: the first half's weights are there while the
-      // second half's are still being computed
-      auto weigh = [&](int x, uint32_t f, bool first, int half) {
-        const uint32_t b = v_lo + (f % STAGES) * (TILE >> 4);
+      auto weigh = [&](int h, uint32_t f, bool first) {
+        const uint32_t b = v_lo + (f % STAGES) * (TILE >> 4) + h * (8192 >> 4);
         if (leader) {
 #pragma unroll
-          for (int u = 4 * half; u < 4 * half + 4; ++u)
-            mma_ts(tm + col_o + D * x, tm + col_s + 128 * x + 8 * u, b + u * (2048 >> 4), HI, idesc_o,
-                   u > 0 || !first);
+          for (int u = 0; u < 4; ++u)
+            mma_ts(t_o, t_s + 64 * h + 8 * u, b + u * (2048 >> 4), HI, idesc_o, u > 0 || !first);
+          mma_commit(&c->pv_done[x]);
         }
       };
+      auto release = [&](uint32_t f) {  // once the products issued so far are done
+        if (leader) mma_commit(&c->kv_empty[f % STAGES]);
+      };
+      auto skip = [&](uint32_t f) {  // a tile of keys that this tile of rows does not reach
+        if (full(f) && leader) mbar_arrive(&c->kv_empty[f % STAGES]);
+      };
+      struct Next {
+        int steps, nk, guard;
+      };
       Walk w;
-      Item it;
       w.begin(c);
-      while (!failed && w.next(c, p, it)) {
-        const int steps[2] = {__shfl_sync(0xffffffffu, it.steps[0], 0), __shfl_sync(0xffffffffu, it.steps[1], 0)};
-        const int nk = max(steps[0], steps[1]), guard = __shfl_sync(0xffffffffu, it.guard, 0);
+      auto fetch = [&](Next& n) {
+        Item it;
+        const bool more = w.next(c, p, it);
+        n.steps = __shfl_sync(0xffffffffu, more ? it.steps[x] : 0, 0);
+        n.nk = __shfl_sync(0xffffffffu, more ? it.nk : 0, 0);
+        n.guard = __shfl_sync(0xffffffffu, more ? it.guard : 0, 0);
+      };
+      // the first scores of an item whose first keys are fill f
+      auto begin_tile = [&](const Next& n, uint32_t f) {
+        if (n.nk == 0) return;
+        if (n.steps == 0) return skip(f);
+        if (!full(f) || !wait(&c->q_full[x], nq++)) return;
+        tc_fence_after();
+        scores(0, f, n.steps == 1);
+        if (n.steps > 1) scores(1, f, n.steps == 2);
+        release(f);
+      };
+      Next cur, nxt;
+      fetch(cur);
+      begin_tile(cur, fill);
+      while (!failed && cur.nk) {
+        fetch(nxt);
         uint32_t bad = 0;
-        if (!full(fill)) failed = true;
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          if (failed || steps[x] == 0) continue;
-          if (!wait(&c->q_full[x], nq[x]++)) {
-            failed = true;
+        for (int j = 0; j < cur.nk && !failed; ++j) {
+          const uint32_t fv = fill + 2 * j + 1, fk = fv + 1;
+          const bool guarded = j >= cur.guard, more_keys = j + 1 < cur.nk;
+          if (2 * j >= cur.steps) {
+            if (guarded) ok_phase ^= 1u << (fv % STAGES);
+            skip(fv);
+            if (more_keys) skip(fk);
             continue;
           }
-          scores(x, fill);
-          if (steps[x] == 1) commit(&c->q_empty[x]);
-        }
-        commit(&c->kv_empty[fill % STAGES]);
-        for (int j = 0; j < nk && !failed; ++j) {
-          const uint32_t fv = fill + 2 * j + 1, fk = fv + 1;
-          if (!full(fv)) {
-            failed = true;
-            break;
-          }
-          if (j >= guard) {
+          if (!full(fv)) break;
+          if (guarded) {
             const uint32_t s = fv % STAGES;
-            if (!wait(&c->v_ok[s], ok_phase >> s)) {
-              failed = true;
-              break;
-            }
+            if (!wait(&c->v_ok[s], ok_phase >> s)) break;
             ok_phase ^= 1u << s;
-            bad |= c->slot_bad[s][0] | c->slot_bad[s][1];
+            bad |= c->slot_bad[s];
           }
-          bool have_k = j + 1 >= nk;  // nothing to wait for
+          const bool keys = 2 * j + 2 < cur.steps;  // of the next key tile, for this tile
+          if (keys && !full(fk)) break;
 #pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            if (j >= steps[x]) continue;
-            if (!wait(&c->p_half[x], np[x])) {
-              failed = true;
-              break;
-            }
+          for (int h = 0; h < 2; ++h) {
+            const int i = 2 * j + h;
+            if (i >= cur.steps || failed) continue;
+            if (!wait(&c->p_ready[x][h], p_phase >> h)) continue;
+            p_phase ^= 1u << h;
             tc_fence_after();
-            weigh(x, fv, j == 0, 0);
-            if (!wait(&c->p_ready[x], np[x]++)) {
-              failed = true;
-              break;
-            }
-            tc_fence_after();
-            weigh(x, fv, j == 0, 1);
-            if (j + 1 < steps[x]) {
-              if (!have_k && !full(fk)) {
-                failed = true;
-                break;
-              }
-              have_k = true;
-              scores(x, fk);
-              if (j + 2 == steps[x]) commit(&c->q_empty[x]);
-            } else if (leader) {
+            weigh(h, fv, i == 0);
+            if (i + 2 < cur.steps) {
+              scores(h, fk, i + 3 == cur.steps);
+            } else if (i + 1 == cur.steps && leader) {
               c->tile_bad[x] = bad;
               mbar_arrive(&c->o_full[x]);
               mma_commit(&c->o_full[x]);
             }
           }
           if (failed) break;
-          commit(&c->kv_empty[fv % STAGES]);
-          if (j + 1 < nk) commit(&c->kv_empty[fk % STAGES]);
+          release(fv);
+          if (keys) release(fk);
+          else if (more_keys) skip(fk);
         }
-        fill += 2 * nk;
+        fill += 2 * cur.nk;
+        if (!failed) begin_tile(nxt, fill);
+        cur = nxt;
       }
       if (failed) {  // products in flight read shared and tensor memory
-        commit(&c->drain);
-        wait(&c->drain, 0);
+        if (leader) mma_commit(&c->drain[x]);
+        wait(&c->drain[x], 0);
       }
     } else {
       // ------------------------------------------- non-finite values in V
       constexpr uint32_t EXP = BF16 ? 0x7F80u : 0x7C00u;
-      const int half = warp - 10;
       uint32_t fill = 0;
       Walk w;
       Item it;
@@ -422,10 +409,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             break;
           }
           if (j >= it.guard) {
-            uint4* tile = reinterpret_cast<uint4*>(ring + s * TILE + half * (TILE / 2));
+            uint4* tile = reinterpret_cast<uint4*>(ring + s * TILE);
             uint32_t top = 0;
 #pragma unroll 8
-            for (int i = lane; i < TILE / 32; i += 32) {
+            for (int i = lane; i < TILE / 16; i += 32) {
               const uint4 x = tile[i];
               top = __vmaxu2(top, x.x & 0x7FFF7FFFu);
               top = __vmaxu2(top, x.y & 0x7FFF7FFFu);
@@ -435,13 +422,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             const bool found = __any_sync(0xffffffffu, (top & 0xFFFFu) >= EXP || (top >> 16) >= EXP);
             if (found) {
               uint16_t* v = reinterpret_cast<uint16_t*>(tile);
-              for (int i = lane; i < TILE / 4; i += 32)
+              for (int i = lane; i < TILE / 2; i += 32)
                 if ((v[i] & EXP) == EXP) v[i] = 0;
               fence_proxy_async_shared();  // before the tensor core reads them
             }
             __syncwarp();
             if (lane == 0) {
-              c->slot_bad[s][half] = found;
+              c->slot_bad[s] = found;
               mbar_arrive(&c->v_ok[s]);
             }
           }
@@ -452,16 +439,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else {
     // ---------------------------------------------------------------- softmax
-    regs_raise<208>();
     constexpr float SHIFT = BF16 ? 0.f : 6.f;  // fp16 weights lie in [2^-24, 2^14]: a row's largest is 2^6 or more
     constexpr float MOVE = 8.f;
-    constexpr int FMA_EXP = 4;  // of 16 pairs
     const int x = warp >> 2, row = tid & 127;
     const int row_tok = row / p.group, row_head = row - row_tok * p.group;
     const uint32_t lane_base = (uint32_t)(warp & 3) << 21;
     const uint32_t ts = tmem + lane_base + col_s + 128 * x, to = tmem + lane_base + col_o + D * x;
     const float sc = p.scale_log2;
-    uint32_t ns = 0, no = 0;
+    uint32_t s_phase = 0, np = 0, no = 0;
     Walk w;
     Item it;
     w.begin(c);
@@ -469,84 +454,91 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int steps = it.steps[x];
       if (steps == 0) continue;
       const int tok = min(it.tok[x] + row_tok, it.rows - 1);
-      const int first_hidden = (it.tok[x] + 1) >> 7;  // first key tile that a row of this tile does not see whole
-      float m = -INFINITY, ref = 0.f, sum = 0.f;
-      for (int j = 0; j < steps; ++j) {
-        if (!__all_sync(0xffffffffu, mbar_wait(&c->s_full[x], ns++ & 1u, limit))) {
+      const int first_hidden = (it.tok[x] + 1) >> 6;  // first step with a key that a row of this tile does not see
+      float m = -INFINITY, sum = 0.f;
+      for (int i = 0; i < steps; ++i) {
+        const int h = i & 1;
+        const uint32_t th = ts + 64 * h;
+        if (!__all_sync(0xffffffffu, mbar_wait(&c->s_full[x][h], (s_phase >> h) & 1u, limit))) {
           failed = true;
           break;
         }
+        s_phase ^= 1u << h;
         tc_fence_after();
-        float s[128];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) tmem_ld32(s + 32 * i, ts + 32 * i);
+        float s[64];
+        tmem_ld32(s, th);
+        tmem_ld32(s + 32, th + 32);
         tmem_wait_ld();
-        if (j >= first_hidden) {
-          const int seen = tok - 128 * j;  // columns 0..seen are attended to
+        if (i >= first_hidden) {
+          const int seen = tok - 64 * i;  // columns 0..seen are attended to
 #pragma unroll
-          for (int i = 0; i < 128; ++i) s[i] = i <= seen ? s[i] : -INFINITY;
+          for (int k = 0; k < 64; ++k) s[k] = k <= seen ? s[k] : -INFINITY;
         }
         float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-        for (int i = 4; i < 124; i += 8) {
+        for (int k = 4; k < 60; k += 8) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k) mx[k] = max3(mx[k], s[i + k], s[i + 4 + k]);
+          for (int l = 0; l < 4; ++l) mx[l] = max3(mx[l], s[k + l], s[k + 4 + l]);
         }
 #pragma unroll
-        for (int k = 0; k < 4; ++k) mx[k] = fmaxf(mx[k], s[124 + k]);
+        for (int l = 0; l < 4; ++l) mx[l] = fmaxf(mx[l], s[60 + l]);
         const float top = max3(m, max3(mx[0], mx[1], mx[2]), mx[3]);
-        if (j == 0) {
+        if (i == 0) {
           m = top;
         } else {
           const bool move = (top - m) * sc > MOVE;
           if (__any_sync(0xffffffffu, move)) {
-            // products up to the last step's are done: this step's scores, issued after them, are
+            // O is idle once the last step's product is done (the one before it
+            // is: this step's scores were issued after it)
+            if (!__all_sync(0xffffffffu, mbar_wait(&c->pv_done[x], (np - 1) & 1u, limit))) {
+              failed = true;
+              break;
+            }
+            tc_fence_after();
             const float f = move ? exp2_approx((m - top) * sc) : 1.f;
             if (move) m = top;
             sum *= f;
-#pragma unroll
-            for (int i = 0; i < D / 16; ++i) {
+#pragma unroll 1
+            for (int k = 0; k < D; k += 16) {
               float o[16];
-              tmem_ld16(o, to + 16 * i);
+              tmem_ld16(o, to + k);
               tmem_wait_ld();
 #pragma unroll
-              for (int k = 0; k < 16; ++k) o[k] *= f;
-              tmem_st16(to + 16 * i, reinterpret_cast<uint32_t*>(o));
+              for (int l = 0; l < 16; ++l) o[l] *= f;
+              tmem_st16(to + k, reinterpret_cast<uint32_t*>(o));
             }
           }
         }
-        ref = m == -INFINITY ? 0.f : m;
+        const float ref = m == -INFINITY ? 0.f : m;
         // exponents s * sc - ref * sc in one rounding: that of ref * sc is the
         // same for the whole row and cancels, as long as it stays below one
         float offset = fmaf(-ref, sc, SHIFT);
         if (__any_sync(0xffffffffu, !(fabsf(ref * sc) < 0x1p20f))) {
           // the difference first: exact near the maximum, whatever its size
 #pragma unroll
-          for (int i = 0; i < 128; ++i) s[i] -= ref;
+          for (int k = 0; k < 64; ++k) s[k] -= ref;
           offset = SHIFT;
         }
         const uint64_t scale2 = f2_pack(sc, sc), offset2 = f2_pack(offset, offset);
         uint64_t acc0 = f2_pack(0.f, 0.f), acc1 = acc0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int k0 = 0; k0 < 32; k0 += 16) {
           uint32_t w16[16];
 #pragma unroll
           for (int k = 0; k < 16; ++k) {
-            uint64_t e = f2_fma(f2_pack(s[32 * i + 2 * k], s[32 * i + 2 * k + 1]), scale2, offset2);
-            e = k % 16 < FMA_EXP ? exp2_fma(e) : exp2_mufu(e);
-            if (k & 1) acc1 = f2_add(acc1, e);
-            else acc0 = f2_add(acc0, e);
             float lo, hi;
-            f2_unpack(e, lo, hi);
+            f2_unpack(f2_fma(f2_pack(s[2 * (k0 + k)], s[2 * (k0 + k) + 1]), scale2, offset2), lo, hi);
+            lo = exp2_approx(lo), hi = exp2_approx(hi);
+            if (k & 1) acc1 = f2_add(acc1, f2_pack(lo, hi));
+            else acc0 = f2_add(acc0, f2_pack(lo, hi));
             w16[k] = pack16<BF16>(lo, hi);
           }
-          tmem_st16(ts + 16 * i, w16);
-          if (i & 1) {
-            tmem_wait_st();
-            tc_fence_before();
-            mbar_arrive(i == 1 ? &c->p_half[x] : &c->p_ready[x]);
-          }
+          tmem_st16(th + k0, w16);
         }
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(&c->p_ready[x][h]);
+        ++np;
         float a0, a1;
         f2_unpack(f2_add(acc0, acc1), a0, a1);
         sum += a0 + a1;
