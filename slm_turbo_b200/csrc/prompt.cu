@@ -60,6 +60,7 @@ struct PromptParams {
   uint64_t wait_limit_ns;
   float scale_log2;
   int num_tokens, num_reqs, max_query, kv, group, tile_tokens, out_dtype;
+  uint32_t kv_recip;  // 2^32 / kv, rounded up
 };
 
 struct PromptCtl {
@@ -69,7 +70,7 @@ struct PromptCtl {
   uint32_t tmem;
   uint32_t tile_bad[2];
   uint32_t slot_bad[kMaxStages];
-  uint32_t sort_key[kMaxReqs];  // (pairs of tiles << kReqBits) | request, descending
+  alignas(16) uint32_t sort_key[kMaxReqs];  // (pairs of tiles << kReqBits) | request, descending
   int start[kMaxReqs], rows[kMaxReqs];
 };
 
@@ -97,24 +98,28 @@ struct Item {
 // item of each other.  Level t holds the items of tile pair t of every request
 // that has one: those are the first `count` of the requests sorted by length.
 struct Walk {
-  int k, level, count;
-  int64_t base;
+  int row, level, count, base;  // deal, tile pair, requests of the level, items before it
   __device__ __forceinline__ void begin(const PromptCtl* c) {
-    k = 0, count = 0, base = 0;
+    row = 0, count = 0, base = 0;
     level = (int)(c->sort_key[0] >> kReqBits);
   }
   __device__ __forceinline__ bool next(const PromptCtl* c, const PromptParams& p, Item& it) {
-    const int nc = gridDim.x;
-    const int64_t at = (int64_t)k * nc + ((k & 1) ? nc - 1 - (int)blockIdx.x : (int)blockIdx.x);
-    ++k;
-    while (at >= base + (int64_t)count * p.kv) {
-      base += (int64_t)count * p.kv;
+    const int nc = gridDim.x, me = blockIdx.x;
+    const int at = row * nc + ((row & 1) ? nc - 1 - me : me);
+    ++row;
+    int in_level = count * p.kv;
+    while (at - base >= in_level) {
+      base += in_level;
       if (--level < 0) return false;
       while (count < p.num_reqs && (int)(c->sort_key[count] >> kReqBits) > level) ++count;
+      in_level = count * p.kv;
     }
-    const int rem = (int)(at - base);
-    it.head = rem % p.kv;
-    it.req = (int)(c->sort_key[rem / p.kv] & ((1u << kReqBits) - 1));
+    // rem / kv by 2^32 / kv rounded up (which kv 1 has no room for): at most one too large
+    const int rem = at - base;
+    int rank = p.kv == 1 ? rem : (int)__umulhi((uint32_t)rem, p.kv_recip);
+    it.head = rem - rank * p.kv;
+    if (it.head < 0) --rank, it.head += p.kv;
+    it.req = (int)(c->sort_key[rank] & ((1u << kReqBits) - 1));
     it.start = c->start[it.req];
     it.rows = c->rows[it.req];
     it.tok[0] = level * 2 * p.tile_tokens;
@@ -194,9 +199,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     fence_mbar_init();
   }
   if (warp == 8) tmem_alloc(&c->tmem, kTmemCols);
-  int n2 = 1;
+  if (tid == 32 * 10) prefetch_map(&map_q), prefetch_map(&map_k), prefetch_map(&map_v);
+  int n2 = 4;
   while (n2 < p.num_reqs) n2 <<= 1;
   unsigned bad_len = 0u;
+  uint32_t mine = 0u;
   for (int r = tid; r < n2; r += kThreads) {
     int n = 0, a = 0;
     if (r < p.num_reqs) {
@@ -211,21 +218,37 @@ __global__ void __launch_bounds__(kThreads, 1)
       c->rows[r] = n;
     }
     const int pairs = (n + 2 * p.tile_tokens - 1) / (2 * p.tile_tokens);
-    c->sort_key[r] = ((uint32_t)pairs << kReqBits) | (uint32_t)r;
+    mine = ((uint32_t)pairs << kReqBits) | (uint32_t)r;
+    c->sort_key[r] = mine;
   }
   if (bad_len && blockIdx.x == 0 && p.err) atomicOr(reinterpret_cast<unsigned int*>(p.err), bad_len);
   __syncthreads();
-  for (int k = 2; k <= n2; k <<= 1)
-    for (int j = k >> 1; j > 0; j >>= 1) {
-      for (int i = tid; i < n2; i += kThreads) {
-        const int o = i ^ j;
-        if (o > i) {
-          const uint32_t x = c->sort_key[i], y = c->sort_key[o];
-          if ((x < y) == ((i & k) == 0)) c->sort_key[i] = y, c->sort_key[o] = x;
-        }
+  if (n2 <= 256) {
+    // a thread counts the keys above its own (all differ): 48 requests 2 us
+    // sooner than by the sort below, whose every pass is a barrier
+    int rank = 0;
+    if (tid < n2) {
+#pragma unroll 4
+      for (int i = 0; i < n2; i += 4) {
+        const uint4 k = *reinterpret_cast<const uint4*>(c->sort_key + i);
+        rank += (k.x > mine) + (k.y > mine) + (k.z > mine) + (k.w > mine);
       }
-      __syncthreads();
     }
+    __syncthreads();
+    if (tid < n2) c->sort_key[rank] = mine;
+  } else {
+    for (int k = 2; k <= n2; k <<= 1)
+      for (int j = k >> 1; j > 0; j >>= 1) {
+        for (int i = tid; i < n2; i += kThreads) {
+          const int o = i ^ j;
+          if (o > i) {
+            const uint32_t x = c->sort_key[i], y = c->sort_key[o];
+            if ((x < y) == ((i & k) == 0)) c->sort_key[i] = y, c->sort_key[o] = x;
+          }
+        }
+        __syncthreads();
+      }
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -447,6 +470,48 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t ts = tmem + lane_base + col_s + 128 * x, to = tmem + lane_base + col_o + D * x;
     const float sc = p.scale_log2;
     uint32_t s_phase = 0, np = 0, no = 0;
+    // A finished item's output is written after the next item's first weights
+    // are computed and before they are announced (that product overwrites O):
+    // the wait for the item's last product is then over.
+    struct Pending {
+      int64_t at;
+      float sum;
+      int start, head, tok, guard;
+      bool any, valid;
+    } last;
+    last.any = false;
+    auto finish = [&] {
+      last.any = false;
+      if (!__all_sync(0xffffffffu, mbar_wait(&c->o_full[x], no++ & 1u, limit))) {
+        failed = true;
+        return;
+      }
+      tc_fence_after();
+      const float inv = 1.f / last.sum;
+      const bool bad = c->tile_bad[x] != 0;
+      float o[D];
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) tmem_ld16(o + 16 * i, to + 16 * i);
+      tmem_wait_ld();
+      if (bad && last.valid) {
+        // the values taken out of the V tiles, for the rows that attend to them
+        for (int j = 128 * last.guard; j <= last.tok; ++j) {
+          const uint16_t* v = reinterpret_cast<const uint16_t*>(p.v) + (int64_t)(last.start + j) * p.v_tok +
+                              (int64_t)last.head * p.v_head;
+#pragma unroll
+          for (int k = 0; k < D; ++k) {
+            const float y = BF16 ? __bfloat162float(__ushort_as_bfloat16(v[k])) : __half2float(__ushort_as_half(v[k]));
+            if (!(y - y == 0.f)) o[k] += y;
+          }
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < D; ++k) o[k] *= inv;
+      if (last.valid) {
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) store16(p.out, p.out_dtype, last.at + 16 * i, o + 16 * i);
+      }
+    };
     Walk w;
     Item it;
     w.begin(c);
@@ -471,8 +536,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_wait_ld();
         if (i >= first_hidden) {
           const int seen = tok - 64 * i;  // columns 0..seen are attended to
+          const uint32_t lo = seen >= 31 ? 0xFFFFFFFFu : seen < 0 ? 0u : (2u << seen) - 1u;
+          const uint32_t hi = seen >= 63 ? 0xFFFFFFFFu : seen < 32 ? 0u : (2u << (seen - 32)) - 1u;
 #pragma unroll
-          for (int k = 0; k < 64; ++k) s[k] = k <= seen ? s[k] : -INFINITY;
+          for (int k = 0; k < 32; ++k) {
+            s[k] = lo & (1u << k) ? s[k] : -INFINITY;
+            s[32 + k] = hi & (1u << k) ? s[32 + k] : -INFINITY;
+          }
         }
         float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
@@ -535,6 +605,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           tmem_st16(th + k0, w16);
         }
+        if (i == 0 && last.any) {
+          finish();
+          if (failed) break;
+        }
         tmem_wait_st();
         tc_fence_before();
         mbar_arrive(&c->p_ready[x][h]);
@@ -543,41 +617,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         f2_unpack(f2_add(acc0, acc1), a0, a1);
         sum += a0 + a1;
       }
-      if (failed) break;
-      if (!__all_sync(0xffffffffu, mbar_wait(&c->o_full[x], no++ & 1u, limit))) {
-        failed = true;
-        break;
-      }
-      tc_fence_after();
-      const bool valid = row_tok < p.tile_tokens && it.tok[x] + row_tok < it.rows;
-      const float inv = 1.f / sum;
       const int h = it.head * p.group + row_head;
-      const int64_t at = (int64_t)(it.start + tok) * p.o_tok + (int64_t)h * p.o_head;
-      const bool bad = c->tile_bad[x] != 0;
-      float o[D];
-#pragma unroll
-      for (int i = 0; i < D / 16; ++i) tmem_ld16(o + 16 * i, to + 16 * i);
-      tmem_wait_ld();
-      if (bad && valid) {
-        // the values taken out of the V tiles, for the rows that attend to them
-        for (int j = 128 * it.guard; j <= tok; ++j) {
-          const uint16_t* v = reinterpret_cast<const uint16_t*>(p.v) + (int64_t)(it.start + j) * p.v_tok +
-                              (int64_t)it.head * p.v_head;
-#pragma unroll
-          for (int k = 0; k < D; ++k) {
-            const float y = BF16 ? __bfloat162float(__ushort_as_bfloat16(v[k])) : __half2float(__ushort_as_half(v[k]));
-            if (!(y - y == 0.f)) o[k] += y;
-          }
-        }
-      }
-#pragma unroll
-      for (int k = 0; k < D; ++k) o[k] *= inv;
-      if (valid) {
-#pragma unroll
-        for (int i = 0; i < D / 16; ++i) store16(p.out, p.out_dtype, at + 16 * i, o + 16 * i);
-      }
-      tc_fence_before();  // O is read before the next item's first product overwrites it
+      last.at = (int64_t)(it.start + tok) * p.o_tok + (int64_t)h * p.o_head;
+      last.sum = sum;
+      last.start = it.start, last.head = it.head, last.tok = tok, last.guard = it.guard;
+      last.any = true, last.valid = row_tok < p.tile_tokens && it.tok[x] + row_tok < it.rows;
     }
+    if (!failed && last.any) finish();
   }
   if (failed && p.err) atomicOr(reinterpret_cast<unsigned int*>(p.err), SLMT_DEVERR_TIMEOUT);
   __syncthreads();
@@ -680,6 +726,7 @@ extern "C" int slmt_prompt_attention(const void* q, int64_t q_token_stride, int6
   p.num_tokens = (int)num_tokens;
   p.max_query = (int)max_query;
   p.kv = (int)num_kv_heads;
+  p.kv_recip = (uint32_t)(((1ull << 32) + num_kv_heads - 1) / num_kv_heads);
   p.group = group;
   p.tile_tokens = tile_tokens;
   p.out_dtype = out_dtype;
@@ -695,6 +742,7 @@ extern "C" int slmt_prompt_attention(const void* q, int64_t q_token_stride, int6
     // no more CTAs than there can be items
     const int64_t pairs = std::min(nr * ((max_query + 2 * tile_tokens - 1) / (2 * tile_tokens)),
                                    num_tokens / (2 * tile_tokens) + nr);
+    if (pairs * num_kv_heads >= INT32_MAX / 2) return SLMT_ERR_UNSUPPORTED;  // items are numbered in 32 bits
     const int grid = (int)std::min<int64_t>(sms, pairs * num_kv_heads);
     int rc;
     if (head_dim == 64)

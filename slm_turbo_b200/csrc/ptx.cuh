@@ -142,6 +142,11 @@ __device__ __forceinline__ void prefetch_l2(const void* p) {
   asm volatile("prefetch.global.L2 [%0];" ::"l"(p));
 }
 
+// Bring a tensor map (a __grid_constant__ kernel parameter) close to the copy unit.
+__device__ __forceinline__ void prefetch_map(const void* tmap) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(tmap) : "memory");
+}
+
 // Tiled 2-D TMA copy global -> shared of the box at (c0, c1) of `tmap`, with
 // the same rules as tma_load_3d.  No multicast.
 __device__ __forceinline__ void tma_load_2d(void* dst, const void* tmap, int c0, int c1, uint64_t* bar) {
