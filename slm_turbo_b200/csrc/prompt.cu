@@ -36,6 +36,7 @@
 // such values; where there are some they are taken out of the tile, and added
 // to the rows that do attend to them at the end, read from global memory.
 #include <atomic>
+#include <type_traits>
 
 #include "internal.h"
 #include "tcgen05.cuh"
@@ -64,12 +65,12 @@ struct PromptParams {
 };
 
 struct PromptCtl {
-  uint64_t q_full[2], q_empty[2], o_full[2], pv_done[2], drain[2];
-  uint64_t s_full[2][2], p_ready[2][2];  // [tile][half of its columns]
+  uint64_t q_full[2], q_empty[2], o_full[2], drain;
+  uint64_t s_full[2], p_ready[2][2];  // [tile], [tile][first or second 64 keys]
   uint64_t kv_full[kMaxStages], kv_empty[kMaxStages], v_ok[kMaxStages];
   uint32_t tmem;
   uint32_t tile_bad[2];
-  uint32_t slot_bad[kMaxStages];
+  uint32_t slot_bad[kMaxStages][2];
   alignas(16) uint32_t sort_key[kMaxReqs];  // (pairs of tiles << kReqBits) | request, descending
   int start[kMaxReqs], rows[kMaxReqs];
 };
@@ -186,20 +187,20 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (tid == 0) {
     for (int x = 0; x < 2; ++x) {
       mbar_init(&c->q_full[x], 1), mbar_init(&c->q_empty[x], 1);
-      for (int h = 0; h < 2; ++h) mbar_init(&c->s_full[x][h], 1), mbar_init(&c->p_ready[x][h], 128);
-      mbar_init(&c->pv_done[x], 1);
+      mbar_init(&c->s_full[x], 1);
+      for (int h = 0; h < 2; ++h) mbar_init(&c->p_ready[x][h], 128);
       mbar_init(&c->o_full[x], 2);  // the commit, and the thread that set tile_bad
     }
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(&c->kv_full[s], 1);
-      mbar_init(&c->kv_empty[s], s & 1 ? 3 : 2);  // both tiles' products; V tiles: and the guard warp
-      mbar_init(&c->v_ok[s], 1);
+      mbar_init(&c->kv_empty[s], s & 1 ? 3 : 1);  // the products; V tiles: and both guard warps
+      mbar_init(&c->v_ok[s], 2);
     }
-    mbar_init(&c->drain[0], 1), mbar_init(&c->drain[1], 1);
+    mbar_init(&c->drain, 1);
     fence_mbar_init();
   }
   if (warp == 8) tmem_alloc(&c->tmem, kTmemCols);
-  if (tid == 32 * 10) prefetch_map(&map_q), prefetch_map(&map_k), prefetch_map(&map_v);
+  if (tid == 32 * 9) prefetch_map(&map_q), prefetch_map(&map_k), prefetch_map(&map_v);
   int n2 = 4;
   while (n2 < p.num_reqs) n2 <<= 1;
   unsigned bad_len = 0u;
@@ -258,7 +259,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   bool failed = false;
   if (warp >= 8) {
-    if (warp == 10) {
+    regs_lower<88>();
+    if (warp == 9) {
       // ------------------------------------------------------------ copies
       if (lane == 0) {
         uint32_t fill = 0, nq[2] = {0, 0};
@@ -295,131 +297,133 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int x = 0; x < 2; ++x)
           if (nq[x] && !mbar_wait(&c->q_full[x], (nq[x] - 1) & 1u, limit)) failed = true;
       }
-    } else if (warp < 10) {
+    } else if (warp == 8) {
       // ----------------------------------------------------------- products
       // The whole warp walks and waits, so that what the products need is the
       // same in every lane and stays in uniform registers; one lane issues.
-      constexpr uint32_t idesc_s = mma_idesc(BF16, 128, 64, false), idesc_o = mma_idesc(BF16, 128, D, true);
+      constexpr uint32_t idesc_s = mma_idesc(BF16, 128, 128, false), idesc_s64 = mma_idesc(BF16, 128, 64, false),
+                         idesc_o = mma_idesc(BF16, 128, D, true);
       constexpr uint32_t HI = desc_hi(1024);
-      const int x = __shfl_sync(0xffffffffu, warp - 8, 0);
       const bool leader = elect_one();
       const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
-      const uint32_t t_s = tm + col_s + 128 * x, t_o = tm + col_o + D * x;
-      const uint32_t q_lo = desc_lo(smem_addr(smem), 16) + x * (TILE >> 4), k_lo = desc_lo(smem_addr(ring), 16),
+      const uint32_t q_lo = desc_lo(smem_addr(smem), 16), k_lo = desc_lo(smem_addr(ring), 16),
                      v_lo = desc_lo(smem_addr(ring), 16384);
-      uint32_t fill = 0, nq = 0, p_phase = 0, ok_phase = 0;
+      uint32_t fill = 0, nq[2] = {0, 0}, p_phase[2] = {0, 0}, ok_phase = 0;
       auto wait = [&](uint64_t* bar, uint32_t phase) {
         const bool ok = __all_sync(0xffffffffu, mbar_wait(bar, phase & 1u, limit));
         failed |= !ok;
         return ok;
       };
       auto full = [&](uint32_t f) { return wait(&c->kv_full[f % STAGES], f / STAGES); };
-      // scores with half h of the keys of fill f
-      auto scores = [&](int h, uint32_t f, bool last) {
-        const uint32_t b = k_lo + (f % STAGES) * (TILE >> 4) + h * (8192 >> 4);
+      auto release = [&](uint32_t f) {  // once the products issued so far are done
+        if (leader) mma_commit(&c->kv_empty[f % STAGES]);
+      };
+      // scores of tile x with the keys of fill f, or the first 64 of them
+      auto scores = [&](int x, uint32_t f, bool two, bool last) {
+        const uint32_t a = q_lo + x * (TILE >> 4), b = k_lo + (f % STAGES) * (TILE >> 4);
+        const uint32_t idesc = two ? idesc_s : idesc_s64;
         if (leader) {
 #pragma unroll
           for (int u = 0; u < D / 16; ++u) {
             const uint32_t off = ((u >> 2) * 16384 + (u & 3) * 32) >> 4;
-            mma_ss(t_s + 64 * h, q_lo + off, HI, b + off, HI, idesc_s, u > 0);
+            mma_ss(tm + col_s + 128 * x, a + off, HI, b + off, HI, idesc, u > 0);
           }
-          mma_commit(&c->s_full[x][h]);
+          mma_commit(&c->s_full[x]);
           if (last) mma_commit(&c->q_empty[x]);
         }
       };
-      auto weigh = [&](int h, uint32_t f, bool first) {
+      // half the keys at a time: the first half's weights are there while the
+      // second half's are still being computed
+      auto weigh = [&](int x, int h, uint32_t f, bool first) {
         const uint32_t b = v_lo + (f % STAGES) * (TILE >> 4) + h * (8192 >> 4);
         if (leader) {
 #pragma unroll
           for (int u = 0; u < 4; ++u)
-            mma_ts(t_o, t_s + 64 * h + 8 * u, b + u * (2048 >> 4), HI, idesc_o, u > 0 || !first);
-          mma_commit(&c->pv_done[x]);
+            mma_ts(tm + col_o + D * x, tm + col_s + 128 * x + 32 * h + 8 * u, b + u * (2048 >> 4), HI, idesc_o,
+                   u > 0 || !first);
         }
       };
-      auto release = [&](uint32_t f) {  // once the products issued so far are done
-        if (leader) mma_commit(&c->kv_empty[f % STAGES]);
-      };
-      auto skip = [&](uint32_t f) {  // a tile of keys that this tile of rows does not reach
-        if (full(f) && leader) mbar_arrive(&c->kv_empty[f % STAGES]);
-      };
       struct Next {
-        int steps, nk, guard;
+        int steps[2], nk, guard;
       };
       Walk w;
       w.begin(c);
       auto fetch = [&](Next& n) {
         Item it;
         const bool more = w.next(c, p, it);
-        n.steps = __shfl_sync(0xffffffffu, more ? it.steps[x] : 0, 0);
+        n.steps[0] = __shfl_sync(0xffffffffu, more ? it.steps[0] : 0, 0);
+        n.steps[1] = __shfl_sync(0xffffffffu, more ? it.steps[1] : 0, 0);
         n.nk = __shfl_sync(0xffffffffu, more ? it.nk : 0, 0);
         n.guard = __shfl_sync(0xffffffffu, more ? it.guard : 0, 0);
       };
-      // the first scores of an item whose first keys are fill f
-      auto begin_tile = [&](const Next& n, uint32_t f) {
-        if (n.nk == 0) return;
-        if (n.steps == 0) return skip(f);
-        if (!full(f) || !wait(&c->q_full[x], nq++)) return;
+      // tile x's first scores of an item whose first keys are fill f
+      auto begin_tile = [&](const Next& n, int x, uint32_t f) {
+        if (n.steps[x] == 0 || !full(f) || !wait(&c->q_full[x], nq[x]++)) return;
         tc_fence_after();
-        scores(0, f, n.steps == 1);
-        if (n.steps > 1) scores(1, f, n.steps == 2);
-        release(f);
+        scores(x, f, n.steps[x] > 1, n.steps[x] <= 2);
       };
       Next cur, nxt;
       fetch(cur);
-      begin_tile(cur, fill);
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+        if (!failed) begin_tile(cur, x, fill);
+      if (cur.nk) release(fill);
       while (!failed && cur.nk) {
         fetch(nxt);
+        const uint32_t next_fill = fill + 2 * cur.nk;
         uint32_t bad = 0;
-        for (int j = 0; j < cur.nk && !failed; ++j) {
+        for (int j = 0; j < cur.nk; ++j) {
           const uint32_t fv = fill + 2 * j + 1, fk = fv + 1;
-          const bool guarded = j >= cur.guard, more_keys = j + 1 < cur.nk;
-          if (2 * j >= cur.steps) {
-            if (guarded) ok_phase ^= 1u << (fv % STAGES);
-            skip(fv);
-            if (more_keys) skip(fk);
-            continue;
-          }
+          const bool more_keys = j + 1 < cur.nk;
           if (!full(fv)) break;
-          if (guarded) {
+          if (j >= cur.guard) {
             const uint32_t s = fv % STAGES;
             if (!wait(&c->v_ok[s], ok_phase >> s)) break;
             ok_phase ^= 1u << s;
-            bad |= c->slot_bad[s];
+            bad |= c->slot_bad[s][0] | c->slot_bad[s][1];
           }
-          const bool keys = 2 * j + 2 < cur.steps;  // of the next key tile, for this tile
-          if (keys && !full(fk)) break;
+          if (more_keys && !full(fk)) break;
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int i = 2 * j + h;
-            if (i >= cur.steps || failed) continue;
-            if (!wait(&c->p_ready[x][h], p_phase >> h)) continue;
-            p_phase ^= 1u << h;
+          for (int x = 0; x < 2; ++x) {
+            if (2 * j >= cur.steps[x] || failed) continue;
+            if (!wait(&c->p_ready[x][0], p_phase[x])) continue;
             tc_fence_after();
-            weigh(h, fv, i == 0);
-            if (i + 2 < cur.steps) {
-              scores(h, fk, i + 3 == cur.steps);
-            } else if (i + 1 == cur.steps && leader) {
-              c->tile_bad[x] = bad;
-              mbar_arrive(&c->o_full[x]);
-              mma_commit(&c->o_full[x]);
+            weigh(x, 0, fv, j == 0);
+            if (!wait(&c->p_ready[x][1], p_phase[x])) continue;
+            p_phase[x] ^= 1u;
+            if (2 * j + 1 < cur.steps[x]) {
+              tc_fence_after();
+              weigh(x, 1, fv, false);
+            }
+            if (2 * j + 2 < cur.steps[x]) {
+              scores(x, fk, 2 * j + 3 < cur.steps[x], 2 * j + 4 >= cur.steps[x]);
+            } else {
+              if (leader) {
+                c->tile_bad[x] = bad;
+                mbar_arrive(&c->o_full[x]);
+                mma_commit(&c->o_full[x]);
+              }
             }
           }
           if (failed) break;
           release(fv);
-          if (keys) release(fk);
-          else if (more_keys) skip(fk);
+          if (more_keys) release(fk);
         }
-        fill += 2 * cur.nk;
-        if (!failed) begin_tile(nxt, fill);
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+          if (!failed) begin_tile(nxt, x, next_fill);
+        if (nxt.nk && !failed) release(next_fill);
+        fill = next_fill;
         cur = nxt;
       }
       if (failed) {  // products in flight read shared and tensor memory
-        if (leader) mma_commit(&c->drain[x]);
-        wait(&c->drain[x], 0);
+        if (leader) mma_commit(&c->drain);
+        wait(&c->drain, 0);
       }
     } else {
       // ------------------------------------------- non-finite values in V
       constexpr uint32_t EXP = BF16 ? 0x7F80u : 0x7C00u;
+      const int half = warp - 10;
       uint32_t fill = 0;
       Walk w;
       Item it;
@@ -432,10 +436,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             break;
           }
           if (j >= it.guard) {
-            uint4* tile = reinterpret_cast<uint4*>(ring + s * TILE);
+            uint4* tile = reinterpret_cast<uint4*>(ring + s * TILE + half * (TILE / 2));
             uint32_t top = 0;
 #pragma unroll 8
-            for (int i = lane; i < TILE / 16; i += 32) {
+            for (int i = lane; i < TILE / 32; i += 32) {
               const uint4 x = tile[i];
               top = __vmaxu2(top, x.x & 0x7FFF7FFFu);
               top = __vmaxu2(top, x.y & 0x7FFF7FFFu);
@@ -445,13 +449,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             const bool found = __any_sync(0xffffffffu, (top & 0xFFFFu) >= EXP || (top >> 16) >= EXP);
             if (found) {
               uint16_t* v = reinterpret_cast<uint16_t*>(tile);
-              for (int i = lane; i < TILE / 2; i += 32)
+              for (int i = lane; i < TILE / 4; i += 32)
                 if ((v[i] & EXP) == EXP) v[i] = 0;
               fence_proxy_async_shared();  // before the tensor core reads them
             }
             __syncwarp();
             if (lane == 0) {
-              c->slot_bad[s] = found;
+              c->slot_bad[s][half] = found;
               mbar_arrive(&c->v_ok[s]);
             }
           }
@@ -462,14 +466,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else {
     // ---------------------------------------------------------------- softmax
+    regs_raise<208>();
     constexpr float SHIFT = BF16 ? 0.f : 6.f;  // fp16 weights lie in [2^-24, 2^14]: a row's largest is 2^6 or more
     constexpr float MOVE = 8.f;
+    constexpr int OUT = D == 80 ? 80 : 64;  // output columns at a time
     const int x = warp >> 2, row = tid & 127;
     const int row_tok = row / p.group, row_head = row - row_tok * p.group;
     const uint32_t lane_base = (uint32_t)(warp & 3) << 21;
     const uint32_t ts = tmem + lane_base + col_s + 128 * x, to = tmem + lane_base + col_o + D * x;
     const float sc = p.scale_log2;
-    uint32_t s_phase = 0, np = 0, no = 0;
+    uint32_t ns = 0, no = 0;
     // A finished item's output is written after the next item's first weights
     // are computed and before they are announced (that product overwrites O):
     // the wait for the item's last product is then over.
@@ -489,28 +495,128 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_after();
       const float inv = 1.f / last.sum;
       const bool bad = c->tile_bad[x] != 0;
-      float o[D];
+#pragma unroll 1
+      for (int i = 0; i < D; i += OUT) {
+        float o[OUT];
 #pragma unroll
-      for (int i = 0; i < D / 16; ++i) tmem_ld16(o + 16 * i, to + 16 * i);
+        for (int k = 0; k < OUT; k += 16) tmem_ld16(o + k, to + i + k);
+        tmem_wait_ld();
+        if (bad && last.valid) {
+          // the values taken out of the V tiles, for the rows that attend to them
+          for (int j = 128 * last.guard; j <= last.tok; ++j) {
+            const uint16_t* v = reinterpret_cast<const uint16_t*>(p.v) + (int64_t)(last.start + j) * p.v_tok +
+                                (int64_t)last.head * p.v_head + i;
+#pragma unroll
+            for (int k = 0; k < OUT; ++k) {
+              const float y = BF16 ? __bfloat162float(__ushort_as_bfloat16(v[k])) : __half2float(__ushort_as_half(v[k]));
+              if (!(y - y == 0.f)) o[k] += y;
+            }
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < OUT; ++k) o[k] *= inv;
+        if (last.valid) {
+#pragma unroll
+          for (int k = 0; k < OUT; k += 16) store16(p.out, p.out_dtype, last.at + i + k, o + k);
+        }
+      }
+    };
+    int tok = 0, first_hidden = 0;
+    float m = 0.f, sum = 0.f;
+    // The softmax of one step over KEYS keys: 128, or 64 where the others are
+    // hidden from all of the tile.  False if a wait ran out.
+    auto step = [&](auto keys, int j) {
+      constexpr int KEYS = decltype(keys)::value;
+      if (!__all_sync(0xffffffffu, mbar_wait(&c->s_full[x], ns++ & 1u, limit))) return false;
+      tc_fence_after();
+      float s[KEYS];
+#pragma unroll
+      for (int k = 0; k < KEYS; k += 32) tmem_ld32(s + k, ts + k);
       tmem_wait_ld();
-      if (bad && last.valid) {
-        // the values taken out of the V tiles, for the rows that attend to them
-        for (int j = 128 * last.guard; j <= last.tok; ++j) {
-          const uint16_t* v = reinterpret_cast<const uint16_t*>(p.v) + (int64_t)(last.start + j) * p.v_tok +
-                              (int64_t)last.head * p.v_head;
+      if (j >= first_hidden) {
+        const int seen = tok - 128 * j;  // columns 0..seen are attended to
 #pragma unroll
-          for (int k = 0; k < D; ++k) {
-            const float y = BF16 ? __bfloat162float(__ushort_as_bfloat16(v[k])) : __half2float(__ushort_as_half(v[k]));
-            if (!(y - y == 0.f)) o[k] += y;
+        for (int k = 0; k < KEYS; k += 32) {
+          const uint32_t word = seen >= k + 31 ? 0xFFFFFFFFu : seen < k ? 0u : (2u << (seen - k)) - 1u;
+#pragma unroll
+          for (int l = 0; l < 32; ++l) s[k + l] = word & (1u << l) ? s[k + l] : -INFINITY;
+        }
+      }
+      float mx[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+      for (int k = 4; k < KEYS - 4; k += 8) {
+#pragma unroll
+        for (int l = 0; l < 4; ++l) mx[l] = max3(mx[l], s[k + l], s[k + 4 + l]);
+      }
+#pragma unroll
+      for (int l = 0; l < 4; ++l) mx[l] = fmaxf(mx[l], s[KEYS - 4 + l]);
+      const float top = max3(m, max3(mx[0], mx[1], mx[2]), mx[3]);
+      if (j == 0) {
+        m = top;
+      } else {
+        const bool move = (top - m) * sc > MOVE;
+        if (__any_sync(0xffffffffu, move)) {
+          // products up to the last step's are done: this step's scores, issued after them, are
+          const float f = move ? exp2_approx((m - top) * sc) : 1.f;
+          if (move) m = top;
+          sum *= f;
+#pragma unroll 1
+          for (int k = 0; k < D; k += 16) {
+            float o[16];
+            tmem_ld16(o, to + k);
+            tmem_wait_ld();
+#pragma unroll
+            for (int l = 0; l < 16; ++l) o[l] *= f;
+            tmem_st16(to + k, reinterpret_cast<uint32_t*>(o));
           }
         }
       }
+      const float ref = m == -INFINITY ? 0.f : m;
+      // exponents s * sc - ref * sc in one rounding: that of ref * sc is the
+      // same for the whole row and cancels, as long as it stays below one
+      float offset = fmaf(-ref, sc, SHIFT);
+      if (__any_sync(0xffffffffu, !(fabsf(ref * sc) < 0x1p20f))) {
+        // the difference first: exact near the maximum, whatever its size
 #pragma unroll
-      for (int k = 0; k < D; ++k) o[k] *= inv;
-      if (last.valid) {
-#pragma unroll
-        for (int i = 0; i < D / 16; ++i) store16(p.out, p.out_dtype, last.at + 16 * i, o + 16 * i);
+        for (int k = 0; k < KEYS; ++k) s[k] -= ref;
+        offset = SHIFT;
       }
+      const bool hold = j == 0 && last.any;  // the last item's output comes first
+      const uint64_t scale2 = f2_pack(sc, sc), offset2 = f2_pack(offset, offset);
+      uint64_t acc0 = f2_pack(0.f, 0.f), acc1 = acc0;
+#pragma unroll
+      for (int k0 = 0; k0 < KEYS / 2; k0 += 16) {
+        uint32_t w16[16];
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+          float lo, hi;
+          f2_unpack(f2_fma(f2_pack(s[2 * (k0 + k)], s[2 * (k0 + k) + 1]), scale2, offset2), lo, hi);
+          lo = exp2_approx(lo), hi = exp2_approx(hi);
+          if (k & 1) acc1 = f2_add(acc1, f2_pack(lo, hi));
+          else acc0 = f2_add(acc0, f2_pack(lo, hi));
+          w16[k] = pack16<BF16>(lo, hi);
+        }
+        tmem_st16(ts + k0, w16);
+        if (k0 == 16 && KEYS == 128) {
+          tmem_wait_st();
+          tc_fence_before();
+          if (!hold) mbar_arrive(&c->p_ready[x][0]);
+        }
+      }
+      float a0, a1;
+      f2_unpack(f2_add(acc0, acc1), a0, a1);
+      sum += a0 + a1;
+      tmem_wait_st();
+      if (hold) {
+        const float keep = sum;
+        finish();
+        sum = keep;
+        if (failed) return false;
+      }
+      tc_fence_before();
+      if (hold || KEYS == 64) mbar_arrive(&c->p_ready[x][0]);
+      mbar_arrive(&c->p_ready[x][1]);
+      return true;
     };
     Walk w;
     Item it;
@@ -518,105 +624,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     while (!failed && w.next(c, p, it)) {
       const int steps = it.steps[x];
       if (steps == 0) continue;
-      const int tok = min(it.tok[x] + row_tok, it.rows - 1);
-      const int first_hidden = (it.tok[x] + 1) >> 6;  // first step with a key that a row of this tile does not see
-      float m = -INFINITY, sum = 0.f;
-      for (int i = 0; i < steps; ++i) {
-        const int h = i & 1;
-        const uint32_t th = ts + 64 * h;
-        if (!__all_sync(0xffffffffu, mbar_wait(&c->s_full[x][h], (s_phase >> h) & 1u, limit))) {
-          failed = true;
-          break;
-        }
-        s_phase ^= 1u << h;
-        tc_fence_after();
-        float s[64];
-        tmem_ld32(s, th);
-        tmem_ld32(s + 32, th + 32);
-        tmem_wait_ld();
-        if (i >= first_hidden) {
-          const int seen = tok - 64 * i;  // columns 0..seen are attended to
-          const uint32_t lo = seen >= 31 ? 0xFFFFFFFFu : seen < 0 ? 0u : (2u << seen) - 1u;
-          const uint32_t hi = seen >= 63 ? 0xFFFFFFFFu : seen < 32 ? 0u : (2u << (seen - 32)) - 1u;
-#pragma unroll
-          for (int k = 0; k < 32; ++k) {
-            s[k] = lo & (1u << k) ? s[k] : -INFINITY;
-            s[32 + k] = hi & (1u << k) ? s[32 + k] : -INFINITY;
-          }
-        }
-        float mx[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-        for (int k = 4; k < 60; k += 8) {
-#pragma unroll
-          for (int l = 0; l < 4; ++l) mx[l] = max3(mx[l], s[k + l], s[k + 4 + l]);
-        }
-#pragma unroll
-        for (int l = 0; l < 4; ++l) mx[l] = fmaxf(mx[l], s[60 + l]);
-        const float top = max3(m, max3(mx[0], mx[1], mx[2]), mx[3]);
-        if (i == 0) {
-          m = top;
-        } else {
-          const bool move = (top - m) * sc > MOVE;
-          if (__any_sync(0xffffffffu, move)) {
-            // O is idle once the last step's product is done (the one before it
-            // is: this step's scores were issued after it)
-            if (!__all_sync(0xffffffffu, mbar_wait(&c->pv_done[x], (np - 1) & 1u, limit))) {
-              failed = true;
-              break;
-            }
-            tc_fence_after();
-            const float f = move ? exp2_approx((m - top) * sc) : 1.f;
-            if (move) m = top;
-            sum *= f;
-#pragma unroll 1
-            for (int k = 0; k < D; k += 16) {
-              float o[16];
-              tmem_ld16(o, to + k);
-              tmem_wait_ld();
-#pragma unroll
-              for (int l = 0; l < 16; ++l) o[l] *= f;
-              tmem_st16(to + k, reinterpret_cast<uint32_t*>(o));
-            }
-          }
-        }
-        const float ref = m == -INFINITY ? 0.f : m;
-        // exponents s * sc - ref * sc in one rounding: that of ref * sc is the
-        // same for the whole row and cancels, as long as it stays below one
-        float offset = fmaf(-ref, sc, SHIFT);
-        if (__any_sync(0xffffffffu, !(fabsf(ref * sc) < 0x1p20f))) {
-          // the difference first: exact near the maximum, whatever its size
-#pragma unroll
-          for (int k = 0; k < 64; ++k) s[k] -= ref;
-          offset = SHIFT;
-        }
-        const uint64_t scale2 = f2_pack(sc, sc), offset2 = f2_pack(offset, offset);
-        uint64_t acc0 = f2_pack(0.f, 0.f), acc1 = acc0;
-#pragma unroll
-        for (int k0 = 0; k0 < 32; k0 += 16) {
-          uint32_t w16[16];
-#pragma unroll
-          for (int k = 0; k < 16; ++k) {
-            float lo, hi;
-            f2_unpack(f2_fma(f2_pack(s[2 * (k0 + k)], s[2 * (k0 + k) + 1]), scale2, offset2), lo, hi);
-            lo = exp2_approx(lo), hi = exp2_approx(hi);
-            if (k & 1) acc1 = f2_add(acc1, f2_pack(lo, hi));
-            else acc0 = f2_add(acc0, f2_pack(lo, hi));
-            w16[k] = pack16<BF16>(lo, hi);
-          }
-          tmem_st16(th + k0, w16);
-        }
-        if (i == 0 && last.any) {
-          finish();
-          if (failed) break;
-        }
-        tmem_wait_st();
-        tc_fence_before();
-        mbar_arrive(&c->p_ready[x][h]);
-        ++np;
-        float a0, a1;
-        f2_unpack(f2_add(acc0, acc1), a0, a1);
-        sum += a0 + a1;
+      tok = min(it.tok[x] + row_tok, it.rows - 1);
+      first_hidden = (it.tok[x] + 1) >> 7;  // first key tile that a row of this tile does not see whole
+      m = -INFINITY, sum = 0.f;
+      for (int j = 0; 2 * j < steps && !failed; ++j) {
+        const bool ok = 2 * j + 1 < steps ? step(std::integral_constant<int, 128>(), j)
+                                          : step(std::integral_constant<int, 64>(), j);
+        failed |= !ok;
       }
+      if (failed) break;
       const int h = it.head * p.group + row_head;
       last.at = (int64_t)(it.start + tok) * p.o_tok + (int64_t)h * p.o_head;
       last.sum = sum;
