@@ -75,8 +75,8 @@ const char* slmt_status_string(int status);
 int slmt_device_sm_count(int device);
 
 /*
- * Bound of every wait inside the decode kernels (pipeline barriers, the
- * split-K merge's wait for the other CTAs of a segment), in nanoseconds, for
+ * Bound of every wait inside the decode and prompt-attention kernels (pipeline
+ * barriers, the split-K merge's wait for the other CTAs of a segment), in nanoseconds, for
  * launches issued after the call; ns <= 0 restores the default of 4 s.  A
  * wait that runs out sets SLMT_DEVERR_TIMEOUT in *err_flag and the kernel
  * returns (after its in-flight copies landed) instead of hanging; its
@@ -88,8 +88,8 @@ int64_t slmt_set_wait_limit_ns(int64_t ns);
 
 /*
  * Test hook for failure detection, off by default: while on, the consumer
- * warps of CTA 0 of every decode launch wait on a barrier that nothing
- * completes, so that wait runs out after the wait limit above and the launch
+ * warps of CTA 0 of every decode and prompt-attention launch wait on a barrier
+ * that nothing completes, so that wait runs out after the wait limit above and the launch
  * reports SLMT_DEVERR_TIMEOUT without faulting or hanging.  Process-wide;
  * returns the previous setting.  No counterpart in the reference.
  */

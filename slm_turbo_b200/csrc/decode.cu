@@ -106,6 +106,7 @@ PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
 }
 
 uint64_t wait_limit_ns() { return g_wait_limit_ns.load(std::memory_order_relaxed); }
+int debug_stall() { return g_debug_stall.load(std::memory_order_relaxed); }
 
 namespace {
 

@@ -28,10 +28,11 @@ inline int launch_status() {
 // SM count of the current device, cached per device id.
 int current_device_sms(int* device_out);
 
-// cuTensorMapEncodeTiled of the driver (null if it has none), and the bound of
-// in-kernel waits set by slmt_set_wait_limit_ns (decode.cu).
+// cuTensorMapEncodeTiled of the driver (null if it has none), and the settings
+// of slmt_set_wait_limit_ns and slmt_set_debug_stall (decode.cu).
 PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder();
 uint64_t wait_limit_ns();
+int debug_stall();
 
 // Bytes at the start of a split-K workspace of `workspace_bytes` that hold
 // the per-segment arrival counters (zero between calls).  Every entry point

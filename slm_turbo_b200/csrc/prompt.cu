@@ -12,19 +12,30 @@
 //   P = exp2((S - m) scale log2 e)   rounded to the inputs' type, over S in TMEM
 //   O += P V    tcgen05.mma, P from TMEM, V in shared memory as it was copied
 //
-// Warps 0-3 and 4-7 are the softmax of tile A and of tile B, a row per thread.
-// A tile's scores are made 64 keys at a time into two halves of its 128
-// columns: while the softmax works on one half, the tensor core weighs V with
-// the other half's P and replaces that half by the next key tile's scores, so
-// neither waits for the other.  (With scores of 128 keys at once a tile's
-// softmax and its products took turns; 64 keys cost S 256 + 2 * 64 cycles
-// instead of half of 512, as both operands come from shared memory.)  Warps 8
-// and 9 issue the products, one for each tile: the tensor core's queue is
-// short, and one warp's waits between two tiles would leave it empty.  Warp 10
-// issues the tiled copies into a ring of K and V tiles, warp 11 looks at the V
-// tiles on the diagonal (below).  Every role walks the same list of items
-// by itself; the next item's first scores go out as soon as its tile's last
-// weights are used.
+// Warps 0-3 and 4-7 are the softmax of tile A and of tile B, a row per thread;
+// while one of them works on its scores, the tensor core computes the other
+// tile's products.  Warp 8 issues the products, warp 9 the tiled copies into
+// a ring of K and V tiles, warps 10 and 11 look at the V tiles on the
+// diagonal (below).  Every role walks the same list of items by itself.
+//
+// What bounds it, per step of 256 rows by 128 keys at D 128 (cycles of an SM):
+// the products need 4 * 512, the exponentials 2 * 1024 of the 16-a-clock unit;
+// a tile's softmax (1950) and its products (950 with their signals) take turns,
+// so a step takes about 2900.  Long prompts run into the power cap before that
+// counts: one of 16384 tokens (32/8 heads, bf16) takes 1.72 ms, 1280 TFLOP/s,
+// in a short run and about 1.95 ms, 1130 TFLOP/s, with the clock held at 1.7
+// GHz.  Short ones are bound by their chain: products, softmax, products,
+// output (a prompt of 130 tokens beside three shorter ones: 9.6 us).
+// Measured and dropped, in turn on one box: scores of 64 keys at a time into
+// alternating halves (the softmax then never waits, but S costs 768 cycles in
+// place of 512 and its products change accumulators twice as often), one
+// product warp per tile (products into different accumulators interleave), two
+// warps to a row, and a part of the exponentials by a polynomial on the FMA
+// pipe (12 instructions in place of 2): 2.0-2.4 ms, 2.2-2.4 ms, 2.2 ms and
+// 1.93 against 1.95 ms.
+//
+// The next item's first scores go out as soon as this one's products are
+// issued, and an item's output is written behind the next one's first weights.
 //
 // Running maximum: the reference m of a row moves only when a score passes it
 // by more than 2^8 in weight; until then old weights stay on their scale, and
@@ -46,8 +57,8 @@ namespace slmt {
 namespace {
 
 constexpr int kThreads = 384;
-constexpr int kMaxReqs = 2048;    // requests of one launch (sorted in shared memory)
-constexpr int kReqBits = 11;
+constexpr int kMaxReqs = 1024;    // requests of one launch (sorted in shared memory)
+constexpr int kReqBits = 10;
 constexpr uint32_t kTmemCols = 512;
 constexpr int kMaxStages = 6;
 
@@ -60,12 +71,12 @@ struct PromptParams {
   int64_t v_tok, v_head, o_tok, o_head;
   uint64_t wait_limit_ns;
   float scale_log2;
-  int num_tokens, num_reqs, max_query, kv, group, tile_tokens, out_dtype;
+  int num_tokens, num_reqs, max_query, kv, group, tile_tokens, out_dtype, stall;
   uint32_t kv_recip;  // 2^32 / kv, rounded up
 };
 
 struct PromptCtl {
-  uint64_t q_full[2], q_empty[2], o_full[2], drain;
+  uint64_t q_full[2], q_empty[2], o_full[2], drain, never;
   uint64_t s_full[2], p_ready[2][2];  // [tile], [tile][first or second 64 keys]
   uint64_t kv_full[kMaxStages], kv_empty[kMaxStages], v_ok[kMaxStages];
   uint32_t tmem;
@@ -73,6 +84,7 @@ struct PromptCtl {
   uint32_t slot_bad[kMaxStages][2];
   alignas(16) uint32_t sort_key[kMaxReqs];  // (pairs of tiles << kReqBits) | request, descending
   int start[kMaxReqs], rows[kMaxReqs];
+  uint4 stage[8][32 * 4];  // up to 64 bytes of each of a softmax warp's output rows
 };
 
 template <int D>
@@ -148,28 +160,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
-// Write 16 finished columns of an output row.
-__device__ __forceinline__ void store16(void* out, int out_dtype, int64_t at, const float* x) {
-  if (out_dtype == SLMT_DTYPE_F32) {
-    float4* o = reinterpret_cast<float4*>(reinterpret_cast<float*>(out) + at);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
-    return;
-  }
-  uint4* o = reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(out) + at);
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    uint4 w;
-    if (out_dtype == SLMT_DTYPE_F16)
-      w = make_uint4(pack_half2(x[8 * i], x[8 * i + 1]), pack_half2(x[8 * i + 2], x[8 * i + 3]),
-                     pack_half2(x[8 * i + 4], x[8 * i + 5]), pack_half2(x[8 * i + 6], x[8 * i + 7]));
-    else
-      w = make_uint4(pack16<true>(x[8 * i], x[8 * i + 1]), pack16<true>(x[8 * i + 2], x[8 * i + 3]),
-                     pack16<true>(x[8 * i + 4], x[8 * i + 5]), pack16<true>(x[8 * i + 6], x[8 * i + 7]));
-    o[i] = w;
-  }
-}
-
 template <int D, bool BF16>
 __global__ void __launch_bounds__(kThreads, 1)
     prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
@@ -182,6 +172,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t* ring = smem + 2 * TILE;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint64_t limit = p.wait_limit_ns;
+  const uint64_t drain_limit = max(limit, (uint64_t)1000000000);  // of the last waits, for what is in flight
 
   // ---- set-up: barriers, tensor memory, the requests sorted by length
   if (tid == 0) {
@@ -196,7 +187,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&c->kv_empty[s], s & 1 ? 3 : 1);  // the products; V tiles: and both guard warps
       mbar_init(&c->v_ok[s], 2);
     }
-    mbar_init(&c->drain, 1);
+    mbar_init(&c->drain, 1), mbar_init(&c->never, 1);
     fence_mbar_init();
   }
   if (warp == 8) tmem_alloc(&c->tmem, kTmemCols);
@@ -293,9 +284,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         // no copy is in flight when this thread is done, whatever happened
         for (uint32_t f = fill > (uint32_t)STAGES ? fill - STAGES : 0; f < fill; ++f)
-          if (!mbar_wait(&c->kv_full[f % STAGES], (f / STAGES) & 1u, limit)) failed = true;
+          if (!mbar_wait(&c->kv_full[f % STAGES], (f / STAGES) & 1u, drain_limit)) failed = true;
         for (int x = 0; x < 2; ++x)
-          if (nq[x] && !mbar_wait(&c->q_full[x], (nq[x] - 1) & 1u, limit)) failed = true;
+          if (nq[x] && !mbar_wait(&c->q_full[x], (nq[x] - 1) & 1u, drain_limit)) failed = true;
       }
     } else if (warp == 8) {
       // ----------------------------------------------------------- products
@@ -416,10 +407,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         fill = next_fill;
         cur = nxt;
       }
-      if (failed) {  // products in flight read shared and tensor memory
-        if (leader) mma_commit(&c->drain);
-        wait(&c->drain, 0);
-      }
+      // products in flight read shared and tensor memory
+      if (leader) mma_commit(&c->drain);
+      if (!mbar_wait(&c->drain, 0, drain_limit)) failed = true;
     } else {
       // ------------------------------------------- non-finite values in V
       constexpr uint32_t EXP = BF16 ? 0x7F80u : 0x7C00u;
@@ -469,7 +459,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     regs_raise<208>();
     constexpr float SHIFT = BF16 ? 0.f : 6.f;  // fp16 weights lie in [2^-24, 2^14]: a row's largest is 2^6 or more
     constexpr float MOVE = 8.f;
-    constexpr int OUT = D == 80 ? 80 : 64;  // output columns at a time
+    constexpr int OUT = D == 80 ? 16 : 32, PIECES = OUT / 8;  // output columns at a time, 16-byte pieces of them
     const int x = warp >> 2, row = tid & 127;
     const int row_tok = row / p.group, row_head = row - row_tok * p.group;
     const uint32_t lane_base = (uint32_t)(warp & 3) << 21;
@@ -495,6 +485,17 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_after();
       const float inv = 1.f / last.sum;
       const bool bad = c->tile_bad[x] != 0;
+      // A thread has a row, but a warp's store of 32 rows' pieces would touch 32
+      // lines: OUT columns of each row go through shared memory, and PIECES
+      // lanes write a row's.  (Pieces lie swapped by bits of the row, which
+      // keeps both sides free of bank conflicts.)
+      const uint32_t rows_valid = __ballot_sync(0xffffffffu, last.valid);
+      int64_t row_at[PIECES];
+#pragma unroll
+      for (int r = 0; r < PIECES; ++r)
+        row_at[r] = __shfl_sync(0xffffffffu, last.at, 32 / PIECES * r + lane / PIECES);
+      auto place = [](int row, int piece) { return PIECES * row + (piece ^ ((row / (8 / PIECES)) & (PIECES - 1))); };
+      uint4* stage = c->stage[warp];
 #pragma unroll 1
       for (int i = 0; i < D; i += OUT) {
         float o[OUT];
@@ -515,12 +516,36 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
 #pragma unroll
         for (int k = 0; k < OUT; ++k) o[k] *= inv;
-        if (last.valid) {
+        if (p.out_dtype == SLMT_DTYPE_F32) {
+          if (last.valid) {
+            float4* to_row = reinterpret_cast<float4*>(reinterpret_cast<float*>(p.out) + last.at + i);
 #pragma unroll
-          for (int k = 0; k < OUT; k += 16) store16(p.out, p.out_dtype, last.at + i + k, o + k);
+            for (int k = 0; k < OUT / 4; ++k) to_row[k] = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+          }
+          continue;
         }
+#pragma unroll
+        for (int k = 0; k < PIECES; ++k) {
+          uint32_t w4[4];
+#pragma unroll
+          for (int l = 0; l < 4; ++l)
+            w4[l] = p.out_dtype == SLMT_DTYPE_BF16 ? pack16<true>(o[8 * k + 2 * l], o[8 * k + 2 * l + 1])
+                                                   : pack16<false>(o[8 * k + 2 * l], o[8 * k + 2 * l + 1]);
+          stage[place(lane, k)] = make_uint4(w4[0], w4[1], w4[2], w4[3]);
+        }
+        __syncwarp();
+#pragma unroll
+        for (int r = 0; r < PIECES; ++r) {
+          const int src = 32 / PIECES * r + lane / PIECES, piece = lane % PIECES;
+          const uint4 w = stage[place(src, piece)];
+          if (rows_valid >> src & 1u)
+            *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p.out) + row_at[r] + i + 8 * piece) = w;
+        }
+        __syncwarp();
       }
     };
+    // test hook: a wait that runs out
+    if (p.stall && blockIdx.x == 0 && x == 0 && !__all_sync(0xffffffffu, mbar_wait(&c->never, 0, limit))) failed = true;
     int tok = 0, first_hidden = 0;
     float m = 0.f, sum = 0.f;
     // The softmax of one step over KEYS keys: 128, or 64 where the others are
@@ -738,6 +763,7 @@ extern "C" int slmt_prompt_attention(const void* q, int64_t q_token_stride, int6
   p.v_tok = v_token_stride, p.v_head = v_head_stride;
   p.o_tok = out_token_stride, p.o_head = out_head_stride;
   p.wait_limit_ns = wait_limit_ns();
+  p.stall = debug_stall();
   p.scale_log2 = sm_scale * 1.4426950408889634f;
   p.num_tokens = (int)num_tokens;
   p.max_query = (int)max_query;

@@ -266,9 +266,6 @@ __device__ __forceinline__ float half_bits_to_float(uint16_t b) {
   return __half2float(__ushort_as_half(b));
 }
 
-// Named barrier of two warps.
-__device__ __forceinline__ void pair_sync(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
-
 // ------------------------------------------------------- packed fp32 pairs --
 __device__ __forceinline__ uint64_t f2_pack(float lo, float hi) {
   uint64_t r;

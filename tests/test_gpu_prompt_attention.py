@@ -308,3 +308,27 @@ def test_prompt_step_then_decode_step(dev):
         s = torch.einsum("hd,nhd->hn", qr1[r].double(), kk.double().repeat_interleave(hq // kv, 1)) * 0.125
         o = torch.einsum("hn,nhd->hd", torch.softmax(s, -1), vv.double().repeat_interleave(hq // kv, 1))
         assert_close(out1[r].cpu().numpy(), o.cpu().numpy(), what=f"request {r}")
+
+
+def test_a_wait_that_runs_out_is_reported(dev):
+    """The test hook makes one softmax wait run out after 2 ms: every role
+    gives up in its own time, nothing hangs, and the next call is right."""
+    import time
+    from slm_turbo_b200 import _lib
+    lib = _lib.load()
+    for d, heads in ((128, (8, 2)), (64, (8, 2)), (80, (4, 4))):
+        lens = [900, 40, 1, 300]
+        q, k, v, start = _inputs(lens, *heads, d, torch.bfloat16, dev)
+        torch.cuda.synchronize()
+        prev = lib.slmt_set_wait_limit_ns(2_000_000)
+        lib.slmt_set_debug_stall(1)
+        try:
+            t0 = time.perf_counter()
+            kd.kv_prompt_attention(q, k, v, start, 900)
+            torch.cuda.synchronize()
+            took = time.perf_counter() - t0
+        finally:
+            lib.slmt_set_debug_stall(0)
+            lib.slmt_set_wait_limit_ns(prev)
+        assert kd.read_device_errors(dev) == 4 and took < 1.0
+        _check(kd.kv_prompt_attention(q, k, v, start, 900), *_ref(q, k, v, lens, d ** -0.5, torch.float32))
