@@ -110,11 +110,13 @@ struct Item {
 // to the CTAs back and forth, so that their sums stay within about one small
 // item of each other.  Level t holds the items of tile pair t of every request
 // that has one: those are the first `count` of the requests sorted by length.
+// A whole warp walks together.
 struct Walk {
   int row, level, count, base;  // deal, tile pair, requests of the level, items before it
+  int longest;                  // pairs of the longest request that is not among them
   __device__ __forceinline__ void begin(const PromptCtl* c) {
     row = 0, count = 0, base = 0;
-    level = (int)(c->sort_key[0] >> kReqBits);
+    level = longest = (int)(c->sort_key[0] >> kReqBits);
   }
   __device__ __forceinline__ bool next(const PromptCtl* c, const PromptParams& p, Item& it) {
     const int nc = gridDim.x, me = blockIdx.x;
@@ -124,7 +126,14 @@ struct Walk {
     while (at - base >= in_level) {
       base += in_level;
       if (--level < 0) return false;
-      while (count < p.num_reqs && (int)(c->sort_key[count] >> kReqBits) > level) ++count;
+      while (longest > level) {  // requests join: 32 looked at together
+        const int i = count + (int)(threadIdx.x & 31);
+        const int pairs = i < p.num_reqs ? (int)(c->sort_key[i] >> kReqBits) : 0;
+        const uint32_t in = __ballot_sync(0xffffffffu, pairs > level);
+        count += __popc(in);
+        longest = in == 0xffffffffu ? (count < p.num_reqs ? (int)(c->sort_key[count] >> kReqBits) : 0)
+                                    : __shfl_sync(0xffffffffu, pairs, __ffs(~in) - 1);
+      }
       in_level = count * p.kv;
     }
     // rem / kv by 2^32 / kv rounded up (which kv 1 has no room for): at most one too large
@@ -253,24 +262,29 @@ __global__ void __launch_bounds__(kThreads, 1)
     regs_lower<88>();
     if (warp == 9) {
       // ------------------------------------------------------------ copies
-      if (lane == 0) {
+      {
+        const bool leader = elect_one();
         uint32_t fill = 0, nq[2] = {0, 0};
         auto load_q = [&](const Item& it, int x) {
-          if (!mbar_wait(&c->q_empty[x], (nq[x] & 1u) ^ 1u, limit)) return false;
+          if (!__all_sync(0xffffffffu, mbar_wait(&c->q_empty[x], (nq[x] & 1u) ^ 1u, limit))) return false;
           ++nq[x];
-          mbar_arrive_expect_tx(&c->q_full[x], (uint32_t)(PANELS * 128 * p.tile_tokens * p.group));
-          for (int d = 0; d < PANELS; ++d)
-            tma_load_3d(smem + x * TILE + d * 16384, &map_q, d * 64, it.head * p.group, it.start + it.tok[x],
-                        &c->q_full[x]);
+          if (leader) {
+            mbar_arrive_expect_tx(&c->q_full[x], (uint32_t)(PANELS * 128 * p.tile_tokens * p.group));
+            for (int d = 0; d < PANELS; ++d)
+              tma_load_3d(smem + x * TILE + d * 16384, &map_q, d * 64, it.head * p.group, it.start + it.tok[x],
+                          &c->q_full[x]);
+          }
           return true;
         };
         auto load_kv = [&](const Item& it, int j, const CUtensorMap* map) {
           const uint32_t s = fill % STAGES;
-          if (!mbar_wait(&c->kv_empty[s], ((fill / STAGES) & 1u) ^ 1u, limit)) return false;
+          if (!__all_sync(0xffffffffu, mbar_wait(&c->kv_empty[s], ((fill / STAGES) & 1u) ^ 1u, limit))) return false;
           ++fill;
-          mbar_arrive_expect_tx(&c->kv_full[s], TILE);
-          for (int d = 0; d < PANELS; ++d)
-            tma_load_3d(ring + s * TILE + d * 16384, map, d * 64, it.head, it.start + 128 * j, &c->kv_full[s]);
+          if (leader) {
+            mbar_arrive_expect_tx(&c->kv_full[s], TILE);
+            for (int d = 0; d < PANELS; ++d)
+              tma_load_3d(ring + s * TILE + d * 16384, map, d * 64, it.head, it.start + 128 * j, &c->kv_full[s]);
+          }
           return true;
         };
         Walk w;
@@ -282,7 +296,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int j = 1; ok && j < it.nk; ++j) ok = load_kv(it, j, &map_k) && load_kv(it, j, &map_v);
           failed = !ok;
         }
-        // no copy is in flight when this thread is done, whatever happened
+        // no copy is in flight when this warp is done, whatever happened
         for (uint32_t f = fill > (uint32_t)STAGES ? fill - STAGES : 0; f < fill; ++f)
           if (!mbar_wait(&c->kv_full[f % STAGES], (f / STAGES) & 1u, drain_limit)) failed = true;
         for (int x = 0; x < 2; ++x)
