@@ -138,8 +138,6 @@ def device_state(device: torch.device) -> _DeviceState:
     return st
 
 
-_err_ptrs: dict = {}  # device index -> address of its error word (lives as long as the process)
-
 _ws_need: dict = {}
 
 
@@ -169,22 +167,24 @@ def workspace(device: torch.device, num_seqs: int, hq: int, kv: int, d: int) -> 
     return ws
 
 
-def call_on(index: int, fn, *args) -> int:
-    """Status of the C entry ``fn(*args, stream)`` on device `index` and its
-    current stream.  The entries launch on the current CUDA device, which need
-    not be `index`."""
-    if torch._C._cuda_getDevice() == index:
-        return fn(*args, torch._C._cuda_getCurrentRawStream(index))
-    with torch.cuda.device(index):
-        return fn(*args, torch._C._cuda_getCurrentRawStream(index))
+_host = None
 
 
-def error_ptr(index: int) -> int:
-    """Address of device `index`'s error word (allocated once, never freed)."""
-    p = _err_ptrs.get(index)
-    if p is None:
-        p = _err_ptrs[index] = device_state(torch.device("cuda", index)).err.data_ptr()
-    return p
+def host():
+    """The Python module of the serving-step entry points (csrc/host.cpp);
+    ImportError if it is not built, like the library."""
+    global _host
+    if _host is None:
+        load()
+        try:
+            from . import _host as module
+        except ImportError as e:
+            raise ImportError(f"_host.so is not built or does not load ({e}); run `python -m slm_turbo_b200.build` "
+                              "(there is no CPU fallback)") from e
+        # a device's error word is allocated once and never freed
+        module.set_error_words(lambda index: device_state(torch.device("cuda", index)).err.data_ptr())
+        _host = module
+    return _host
 
 
 def error_word(device: torch.device) -> torch.Tensor:

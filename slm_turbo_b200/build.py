@@ -1,9 +1,11 @@
-"""Build the sm_100a C-ABI library ``libslm_turbo_b200.so`` in-tree with nvcc.
+"""Build the sm_100a C-ABI library ``libslm_turbo_b200.so`` in-tree with nvcc,
+and the Python module ``_host.so`` (host side of the serving-step entry points,
+a C++ file on top of the library and torch's headers) with g++.
 
     python -m slm_turbo_b200.build          # or build_library() from Python
 
-The library is written next to this file so that it travels with the source
-tree; there is no JIT cache and no Python extension module.  Flags: sm_100a
+Both are written next to this file so that they travel with the source tree;
+there is no JIT cache.  Flags of the library: sm_100a
 only, -O3, -lineinfo, IEEE division/rounding (no --use_fast_math: the
 quantizers must match the reference bit for bit).
 """
@@ -12,6 +14,7 @@ from __future__ import annotations
 import os
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -21,6 +24,8 @@ CSRC = HERE / "csrc"
 INCLUDE = ROOT / "include"
 LIB_NAME = "libslm_turbo_b200.so"
 LIB_PATH = HERE / LIB_NAME
+HOST_PATH = HERE / "_host.so"
+HOST_SOURCE = CSRC / "host.cpp"
 SOURCES = ["decode.cu", "store.cu", "decode_noalloc.cu",
            "decode_d64_paged.cu", "decode_d64_contig.cu", "decode_d80_paged.cu", "decode_d80_contig.cu",
            "decode_d128_paged.cu", "decode_d128_contig.cu", "prefill.cu",
@@ -50,9 +55,31 @@ def _stale() -> bool:
     return any(d.stat().st_mtime > t for d in deps)
 
 
+def build_host(force: bool = False, verbose: bool = False) -> Path:
+    """Compile the Python module on top of the library (skips if up to date)."""
+    deps = [HOST_SOURCE, INCLUDE / "slm_turbo_b200.h"]
+    if not force and HOST_PATH.exists() and all(d.stat().st_mtime <= HOST_PATH.stat().st_mtime for d in deps):
+        return HOST_PATH
+    import torch
+    root = Path(torch.__file__).resolve().parent
+    tmp = HOST_PATH.with_suffix(".so.tmp")
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-I", str(INCLUDE),
+           "-I", "/usr/local/cuda/include", "-isystem", str(root / "include"),
+           "-isystem", str(root / "include/torch/csrc/api/include"), "-I", sysconfig.get_paths()["include"],
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", str(HOST_SOURCE), "-o", str(tmp),
+           "-L", str(HERE), f"-l:{LIB_NAME}", "-Wl,-rpath,$ORIGIN",
+           "-L", str(root / "lib"), "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_python"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    subprocess.run(cmd, check=True)
+    os.replace(tmp, HOST_PATH)
+    return HOST_PATH
+
+
 def build_library(force: bool = False, verbose: bool = False, extra_flags=None) -> Path:
     """Compile every .cu source into one shared library (skips if up to date)."""
     if not force and not _stale():
+        build_host(verbose=verbose)
         return LIB_PATH
     build_dir = HERE / "_build"
     build_dir.mkdir(exist_ok=True)
@@ -85,6 +112,7 @@ def build_library(force: bool = False, verbose: bool = False, extra_flags=None) 
         print(" ".join(cmd), flush=True)
     subprocess.run(cmd, check=True)
     os.replace(tmp, LIB_PATH)
+    build_host(force=force, verbose=verbose)
     return LIB_PATH
 
 

@@ -498,28 +498,6 @@ def kv_append_per_channel(x_new, scale, zero, packed, pos):
 # =============================================================================
 #  The serving step around the cache
 # =============================================================================
-def _same_device(what, index, *tensors):
-    for t in tensors:
-        if t is not None and t.get_device() != index:
-            raise RuntimeError(f"{what}: tensors on {t.device} and cuda:{index}")
-
-
-def _no_autograd(what, *tensors):
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t is not None and t.requires_grad:
-                raise RuntimeError(f"{what}: has no backward pass; call it under torch.no_grad() or on detached "
-                                   "tensors")
-
-
-def _int32(t):
-    return t if t.dtype == torch.int32 and t.is_contiguous() else t.to(torch.int32).contiguous()
-
-
-def _ptr(t):
-    return None if t is None else t.data_ptr()
-
-
 def kv_page_plan(query_start_loc, seq_lens, block_tables, block_size, num_tokens, free_blocks=None,
                  free_cursor=None, slot_mapping=None, positions=None):
     """Where the tokens of one serving step go, from the requests' lengths.
@@ -537,45 +515,8 @@ def kv_page_plan(query_start_loc, seq_lens, block_tables, block_size, num_tokens
     written in place.  A free list that is too short, entries below 0 and
     lengths beyond the table give slot -1 and set a device error bit.
     """
-    L = _lib.load()
-    _require_cuda(block_tables, "page plan: block_tables", (torch.int32,))
-    index = block_tables.get_device()
-    num_tokens = int(num_tokens)
-    R = seq_lens.numel()
-    if block_tables.dim() != 2:
-        raise RuntimeError(f"page plan: block_tables must be [{R}, max_blocks], got {tuple(block_tables.shape)}")
-    rows, width = block_tables.shape
-    row_stride, col_stride = block_tables.stride()
-    if rows < R or (width > 1 and col_stride != 1):
-        raise RuntimeError(f"page plan: block_tables must be [{R}, max_blocks] with unit column stride")
-    if query_start_loc.numel() < R + 1:
-        raise RuntimeError(f"page plan: query_start_loc needs {R + 1} entries, has {query_start_loc.numel()}")
-    if num_tokens < 0:
-        raise RuntimeError(f"page plan: num_tokens must not be negative, got {num_tokens}")
-    num_free = 0
-    if free_blocks is not None:
-        if free_blocks.dtype != torch.int32 or not free_blocks.is_contiguous():
-            raise RuntimeError("page plan: free_blocks must be contiguous int32")
-        num_free = free_blocks.numel()
-    if free_cursor is not None and (free_cursor.dtype != torch.int32 or free_cursor.numel() != 1):
-        raise RuntimeError("page plan: free_cursor must be one int32")
-    if slot_mapping is None:
-        slot_mapping = block_tables.new_empty(num_tokens, dtype=torch.int64)
-    elif slot_mapping.dtype != torch.int64 or not slot_mapping.is_contiguous() or slot_mapping.numel() != num_tokens:
-        raise RuntimeError(f"page plan: slot_mapping must be contiguous int64 of length {num_tokens}")
-    if positions is None:
-        positions = block_tables.new_empty(num_tokens, dtype=torch.int64)
-    elif positions.dtype != torch.int64 or not positions.is_contiguous() or positions.numel() != num_tokens:
-        raise RuntimeError(f"page plan: positions must be contiguous int64 of length {num_tokens}")
-    _same_device("page plan", index, query_start_loc, seq_lens, free_blocks, free_cursor, slot_mapping, positions)
-    qsl, sl = _int32(query_start_loc), _int32(seq_lens)
-    cursor = block_tables.new_empty(1)
-    rc = _lib.call_on(
-        index, L.slmt_page_plan, qsl.data_ptr(), sl.data_ptr(), R, block_tables.data_ptr(), row_stride, width,
-        int(block_size), _ptr(free_blocks), num_free, _ptr(free_cursor), num_tokens, slot_mapping.data_ptr(),
-        positions.data_ptr(), cursor.data_ptr(), _lib.error_ptr(index))
-    _lib.check(rc, "page plan")
-    return slot_mapping, positions, cursor
+    return _lib.host().page_plan(query_start_loc, seq_lens, block_tables, block_size, num_tokens, free_blocks,
+                                 free_cursor, slot_mapping, positions)
 
 
 def kv_rotary_inv_freq(rotary_dim, base=10000.0, scaling=None, device=None):
@@ -649,34 +590,6 @@ def kv_rotary_inv_freq(rotary_dim, base=10000.0, scaling=None, device=None):
     return freq.to(torch.float32).to(device or "cpu"), factor_out
 
 
-def _rotary_args(what, query, key, positions, inv_freq, query_out, key_out):
-    """Checks of kv_rotary / kv_rotary_store; returns the tensors to pass."""
-    _require_cuda(query, f"{what}: query", _QDT)
-    _require_cuda(key, f"{what}: key", _QDT)
-    dtype = query.dtype
-    if dtype != key.dtype:
-        raise RuntimeError(f"{what}: query/key dtypes differ")
-    qs, ks = query.shape, key.shape
-    if len(qs) != 3 or len(ks) != 3 or qs[0] != ks[0] or qs[2] != ks[2]:
-        raise RuntimeError(f"{what}: query/key must be [N, H, D] and [N, KV, D], got {tuple(qs)} and {tuple(ks)}")
-    if positions.dtype not in (torch.int32, torch.int64) or positions.shape != qs[:1]:
-        raise RuntimeError(f"{what}: positions must be int32/int64 of length {qs[0]}")
-    if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 or 2 * inv_freq.numel() > qs[2]:
-        raise RuntimeError(f"{what}: inv_freq must be float32 with at most head_dim/2 entries")
-    if query_out is not None and (query_out.shape != qs or query_out.dtype != dtype or query_out.stride(2) != 1):
-        raise RuntimeError(f"{what}: query_out must be {tuple(qs)} {dtype} with unit head-dim stride")
-    if key_out is not None and (key_out.shape != ks or key_out.dtype != dtype or key_out.stride(2) != 1):
-        raise RuntimeError(f"{what}: key_out must be {tuple(ks)} {dtype} with unit head-dim stride")
-    _same_device(what, query.get_device(), key, positions, inv_freq, query_out, key_out)
-    _no_autograd(what, query, key, inv_freq, query_out, key_out)
-    # an in-place call reads the caller's own rows, whatever their strides
-    if query.stride(2) != 1:
-        query = query.contiguous()
-    if key.stride(2) != 1:
-        key = key.contiguous()
-    return query, key, positions.contiguous(), inv_freq.contiguous(), qs, ks
-
-
 def kv_rotary(query, key, positions, inv_freq, interleaved=False, attention_scaling=1.0, query_out=None,
               key_out=None):
     """Rotary positions of query [N, Hq, D] and key [N, KV, D] (fp16/bf16).
@@ -688,20 +601,7 @@ def kv_rotary(query, key, positions, inv_freq, interleaved=False, attention_scal
     copied.  Negative positions turn back.  Returns (query, key) rotated: new
     tensors, or ``query_out`` / ``key_out``, which may be the inputs themselves.
     """
-    L = _lib.load()
-    q, k, pos, freq, qs, ks = _rotary_args("rotary", query, key, positions, inv_freq, query_out, key_out)
-    qo = q.new_empty(qs) if query_out is None else query_out
-    ko = k.new_empty(ks) if key_out is None else key_out
-    qt, qh, _ = q.stride()
-    kt, kh, _ = k.stride()
-    qot, qoh, _ = qo.stride()
-    kot, koh, _ = ko.stride()
-    rc = _lib.call_on(
-        q.get_device(), L.slmt_rotary, q.data_ptr(), qt, qh, k.data_ptr(), kt, kh, _lib.dtype_tag(q.dtype),
-        pos.data_ptr(), _lib.dtype_tag(pos.dtype), freq.data_ptr(), 2 * freq.numel(), 1 if interleaved else 0,
-        attention_scaling, qs[0], qs[1], ks[1], qs[2], qo.data_ptr(), qot, qoh, ko.data_ptr(), kot, koh)
-    _lib.check(rc, "rotary")
-    return qo, ko
+    return _lib.host().rotary(query, key, positions, inv_freq, interleaved, attention_scaling, query_out, key_out)
 
 
 def kv_rotary_store(query, key, value, positions, inv_freq, kv_cache, slot_mapping, interleaved=False,
@@ -715,40 +615,8 @@ def kv_rotary_store(query, key, value, positions, inv_freq, kv_cache, slot_mappi
     with ``return_key=False`` (a decode step, whose key is read from the cache)
     the rotated key goes to the cache only and None is returned for it.
     """
-    L = _lib.load()
-    q, k, pos, freq, qs, ks = _rotary_args("rotary store", query, key, positions, inv_freq, query_out, key_out)
-    N, KV, D = ks
-    _require_cuda(value, "rotary store: value", _QDT)
-    if value.dtype != k.dtype or value.shape != ks:
-        raise RuntimeError(f"rotary store: value must be {tuple(ks)} {k.dtype}")
-    if kv_cache.dtype != torch.uint8 or not kv_cache.is_contiguous() or kv_cache.dim() != 4:
-        raise RuntimeError("rotary store: kv_cache must be contiguous uint8 [num_blocks, block_size, KV, D+8]")
-    NB, bs, cache_kv, row = kv_cache.shape
-    if cache_kv != KV or row != D + 8:
-        raise RuntimeError(f"rotary store: cache rows are {(cache_kv, row)}, expected {(KV, D + 8)}")
-    if slot_mapping.dtype != torch.int64 or slot_mapping.numel() != N:
-        raise RuntimeError(f"rotary store: slot_mapping must be int64 of length {N}")
-    if key_out is not None and not return_key:
-        raise RuntimeError("rotary store: key_out is given but return_key is False")
-    index = q.get_device()
-    _same_device("rotary store", index, value, kv_cache, slot_mapping)
-    _no_autograd("rotary store", value)
-    v = value if value.stride(2) == 1 else value.contiguous()
-    sm = slot_mapping.contiguous()
-    qo = q.new_empty(qs) if query_out is None else query_out
-    ko = k.new_empty(ks) if key_out is None and return_key else key_out
-    qt, qh, _ = q.stride()
-    kt, kh, _ = k.stride()
-    vt, vh, _ = v.stride()
-    qot, qoh, _ = qo.stride()
-    kot, koh, _ = (0, 0, 0) if ko is None else ko.stride()
-    rc = _lib.call_on(
-        index, L.slmt_rotary_store, q.data_ptr(), qt, qh, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh,
-        _lib.dtype_tag(q.dtype), pos.data_ptr(), _lib.dtype_tag(pos.dtype), freq.data_ptr(), 2 * freq.numel(),
-        1 if interleaved else 0, attention_scaling, N, qs[1], KV, D, qo.data_ptr(), qot, qoh, _ptr(ko), kot, koh,
-        kv_cache.data_ptr(), NB, bs, sm.data_ptr(), _lib.error_ptr(index))
-    _lib.check(rc, "rotary store")
-    return qo, ko
+    return _lib.host().rotary_store(query, key, value, positions, inv_freq, kv_cache, slot_mapping, interleaved,
+                                    attention_scaling, query_out, key_out, return_key)
 
 
 def kv_dequantize_load(kv_cache, slot_mapping, dtype=torch.float16, key_out=None, value_out=None):
@@ -758,38 +626,7 @@ def kv_dequantize_load(kv_cache, slot_mapping, dtype=torch.float16, key_out=None
     set a device error bit.  ``key_out`` / ``value_out``: contiguous tensors to
     write instead of new ones.
     """
-    L = _lib.load()
-    _require_cuda(kv_cache, "load: kv_cache", (torch.uint8,))
-    if kv_cache.dim() != 4 or not kv_cache.is_contiguous():
-        raise RuntimeError("load: kv_cache must be contiguous [num_blocks, block_size, KV, D+8]")
-    if slot_mapping.dtype != torch.int64 or slot_mapping.dim() != 1:
-        raise RuntimeError("load: slot_mapping must be int64 [N]")
-    NB, bs, KV, row = kv_cache.shape
-    N, D, index = slot_mapping.numel(), row - 8, kv_cache.get_device()
-    shape = (N, KV, D)
-    for t in (key_out, value_out):
-        if t is not None and (t.shape != shape or t.dtype != dtype or not t.is_contiguous()):
-            raise RuntimeError(f"load: key_out and value_out must be contiguous {shape} {dtype}")
-    _same_device("load", index, slot_mapping, key_out, value_out)
-    _no_autograd("load", key_out, value_out)
-    sm = slot_mapping.contiguous()
-    k = kv_cache.new_empty(shape, dtype=dtype) if key_out is None else key_out
-    v = kv_cache.new_empty(shape, dtype=dtype) if value_out is None else value_out
-    rc = _lib.call_on(index, L.slmt_kv_dequantize_load, kv_cache.data_ptr(), NB, bs, KV, D, sm.data_ptr(), N,
-                      k.data_ptr(), v.data_ptr(), _lib.dtype_tag(dtype), _lib.error_ptr(index))
-    _lib.check(rc, "load")
-    return k, v
-
-
-def _tile_ready(t):
-    """`t` itself where 16-byte rows can be copied from it, else a dense copy;
-    its address and strides."""
-    token, head, dim = t.stride()
-    at = t.data_ptr()
-    if dim == 1 and token > 0 and head > 0 and (token | head) % 8 == 0 and at % 16 == 0:
-        return t, at, token, head
-    t = t.clone(memory_format=torch.contiguous_format)
-    return t, t.data_ptr(), t.stride(0), t.stride(1)
+    return _lib.host().dequantize_load(kv_cache, slot_mapping, dtype, key_out, value_out)
 
 
 def kv_prompt_attention(query, key, value, query_start_loc, max_query_len, seq_lens=None, out=None, sm_scale=None):
@@ -806,40 +643,4 @@ def kv_prompt_attention(query, key, value, query_start_loc, max_query_len, seq_l
     ones are not written.  A row sees nothing of what it does not attend to,
     NaN and infinities included.
     """
-    L = _lib.load()
-    _require_cuda(query, "prompt attention: query", _QDT)
-    qs, ks, dtype = query.shape, key.shape, query.dtype
-    if len(qs) != 3 or len(ks) != 3 or ks != value.shape or ks[0] != qs[0] or ks[2] != qs[2]:
-        raise RuntimeError(f"prompt attention: query [N, Hq, D] and key/value [N, KV, D] expected, got "
-                           f"{tuple(qs)}, {tuple(ks)}, {tuple(value.shape)}")
-    if key.dtype != dtype or value.dtype != dtype:
-        raise RuntimeError("prompt attention: query/key/value dtypes differ")
-    N, H, D = qs
-    KV = ks[1]
-    if KV == 0 or H % KV:
-        raise RuntimeError(f"prompt attention: {H} query heads do not divide over {KV} kv heads")
-    R = query_start_loc.numel() - 1
-    if R < 0 or (seq_lens is not None and seq_lens.numel() != R):
-        raise RuntimeError("prompt attention: query_start_loc must have one entry more than there are requests"
-                           + ("" if seq_lens is None else f" (seq_lens has {seq_lens.numel()})"))
-    if out is not None and (out.shape != qs or (N > 0 and out.stride(2) != 1)):
-        raise RuntimeError(f"prompt attention: out must be {tuple(qs)} with unit head-dim stride")
-    index = query.get_device()
-    _same_device("prompt attention", index, key, value, query_start_loc, seq_lens, out)
-    _no_autograd("prompt attention", query, key, value, out)
-    if out is None:
-        out = query.new_empty(qs, dtype=torch.float32)
-    if N == 0:
-        return out
-    q, qp, qt, qh = _tile_ready(query)
-    k, kp, kt, kh = _tile_ready(key)
-    v, vp, vt, vh = _tile_ready(value)
-    ot, oh, _ = out.stride()
-    qsl = _int32(query_start_loc)
-    sl = None if seq_lens is None else _int32(seq_lens)
-    rc = _lib.call_on(
-        index, L.slmt_prompt_attention, qp, qt, qh, kp, kt, kh, vp, vt, vh, _lib.dtype_tag(dtype), qsl.data_ptr(),
-        _ptr(sl), R, int(max_query_len), N, H, KV, D, D ** -0.5 if sm_scale is None else float(sm_scale),
-        out.data_ptr(), _lib.dtype_tag(out.dtype), ot, oh, _lib.error_ptr(index))
-    _lib.check(rc, "prompt attention")
-    return out
+    return _lib.host().prompt_attention(query, key, value, query_start_loc, max_query_len, seq_lens, out, sm_scale)
