@@ -374,7 +374,8 @@ int slmt_paged_decode_noalloc(const void* q, int q_dtype, int64_t q_seq_stride,
  * Block tables, slot ids and positions of one step, from request lengths.
  * Request r brings rows [query_start_loc[r], query_start_loc[r+1]) of the
  * step: the last n_r of its seq_lens[r] tokens (lengths AFTER the step; int32,
- * device).  With free_blocks (int32 [num_free], device) the pages that the
+ * device).  With free_blocks (int32 [num_free], device; not NULL even where
+ * num_free is 0) the pages that the
  * new tokens enter are taken from it in request order, from index
  * *free_cursor on (NULL: 0), and written to block_tables (int32 [num_reqs,
  * max_blocks_per_seq], row stride bt_seq_stride); without, the tables are
@@ -425,7 +426,7 @@ int slmt_rotary(const void* q, int64_t q_token_stride, int64_t q_head_stride,
  * the v rows [num_tokens, num_kv_heads, head_dim], as one launch: the same
  * rows and the same cache bytes.  k_out may be NULL (the rotated k goes to
  * the cache only).  slot_mapping as slmt_kv_quantize_store (negative: the
- * row is rotated but not stored).
+ * row is rotated but not stored; the others distinct).
  */
 int slmt_rotary_store(const void* q, int64_t q_token_stride,
                       int64_t q_head_stride, const void* k,
@@ -467,7 +468,8 @@ int slmt_kv_dequantize_load(const uint8_t* kv_cache, int64_t num_blocks,
  * bounds the requests' rows; a request with more sets SLMT_DEVERR_SEQ_LEN and
  * its rows beyond are not written.  Rows outside [0, num_tokens) set it too.
  * A row sees nothing of the keys and values it does not attend to, NaN and
- * infinities included.  sm_scale positive and finite.  Pointers 16-byte
+ * infinities included, and a request's rows do not depend on the rest of the
+ * batch.  out must not overlap k or v.  sm_scale positive and finite.  Pointers 16-byte
  * aligned, strides multiples of 16 bytes.  At most 128 query heads per kv
  * head.  No workspace, no host sync.
  */

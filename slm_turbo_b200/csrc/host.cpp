@@ -128,9 +128,11 @@ std::tuple<Tensor, Tensor, Tensor> page_plan(const Tensor& query_start_loc, cons
   Tensor slots = slot_mapping ? *slot_mapping : at::empty({num_tokens}, longs);
   Tensor pos = positions ? *positions : at::empty({num_tokens}, longs);
   Tensor cursor = at::empty({1}, block_tables.options());
+  // an empty free list is a list all the same (its tensor has no address)
+  const int32_t* list = nullptr;
+  if (free_blocks) list = free_blocks->numel() ? data<int32_t>(*free_blocks) : data<int32_t>(cursor);
   check(slmt_page_plan(data<int32_t>(qsl), data<int32_t>(sl), R, data<int32_t>(block_tables), block_tables.stride(0),
-                       block_tables.size(1), block_size, free_blocks ? data<int32_t>(*free_blocks) : nullptr,
-                       free_blocks ? free_blocks->numel() : 0, free_cursor ? data<int32_t>(*free_cursor) : nullptr,
+                       block_tables.size(1), block_size, list, free_blocks ? free_blocks->numel() : 0, free_cursor ? data<int32_t>(*free_cursor) : nullptr,
                        num_tokens, data<int64_t>(slots), data<int64_t>(pos), data<int32_t>(cursor), error_word(index),
                        c10::cuda::getCurrentCUDAStream(index).stream()),
         W);

@@ -614,11 +614,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       // exponents s * sc - ref * sc in one rounding: that of ref * sc is the
       // same for the whole row and cancels, as long as it stays below one
       float offset = fmaf(-ref, sc, SHIFT);
-      if (__any_sync(0xffffffffu, !(fabsf(ref * sc) < 0x1p20f))) {
-        // the difference first: exact near the maximum, whatever its size
+      const bool far = !(fabsf(ref * sc) < 0x1p20f);
+      if (__any_sync(0xffffffffu, far)) {
+        // for such a row the difference first: exact near the maximum, whatever
+        // its size (the other rows keep their bits)
+        const float base = far ? ref : 0.f;
 #pragma unroll
-        for (int k = 0; k < KEYS; ++k) s[k] -= ref;
-        offset = SHIFT;
+        for (int k = 0; k < KEYS; ++k) s[k] -= base;
+        if (far) offset = SHIFT;
       }
       const bool hold = j == 0 && last.any;  // the last item's output comes first
       const uint64_t scale2 = f2_pack(sc, sc), offset2 = f2_pack(offset, offset);

@@ -566,9 +566,13 @@ def kv_rotary_inv_freq(rotary_dim, base=10000.0, scaling=None, device=None):
         factor, orig = need("factor"), need("original_max_position_embeddings")
         if kind == "llama3":
             low, high = need("low_freq_factor"), need("high_freq_factor")
+            if not high > low:
+                raise RuntimeError(f"rotary scaling 'llama3': high_freq_factor {high} must exceed low_freq_factor {low}")
             turns = orig * freq / (2.0 * math.pi)  # over the original length
             keep = ((turns - low) / (high - low)).clamp(0.0, 1.0)
         else:
+            if not base > 1:
+                raise RuntimeError(f"rotary scaling 'yarn' needs a base above 1, got {base}")
             fast, slow = float(scaling.get("beta_fast") or 32.0), float(scaling.get("beta_slow") or 1.0)
 
             def index_of(turns):  # the pair that makes this many turns over the original length
@@ -611,7 +615,8 @@ def kv_rotary_store(query, key, value, positions, inv_freq, kv_cache, slot_mappi
     bytes.
 
     kv_cache [num_blocks, block_size, KV, D+8] uint8 (in place); slot_mapping
-    [N] int64 (negative: rotated, not stored).  Returns (query, key) rotated;
+    [N] int64 (negative: rotated, not stored; distinct otherwise, as for
+    ``kv_quantize_store``: two rows of one slot would race).  Returns (query, key) rotated;
     with ``return_key=False`` (a decode step, whose key is read from the cache)
     the rotated key goes to the cache only and None is returned for it.
     """
@@ -641,6 +646,7 @@ def kv_prompt_attention(query, key, value, query_start_loc, max_query_len, seq_l
     batch is ``kv_prefill_paged``'s.  Returns out [N, Hq, D] (fp32 by default,
     or the given ``out`` in fp32/fp16/bf16); rows of no request and of skipped
     ones are not written.  A row sees nothing of what it does not attend to,
-    NaN and infinities included.
+    NaN and infinities included, and a request's rows have the same bits
+    whatever else is in the batch.  ``out`` must not overlap key or value.
     """
     return _lib.host().prompt_attention(query, key, value, query_start_loc, max_query_len, seq_lens, out, sm_scale)

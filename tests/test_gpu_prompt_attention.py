@@ -332,3 +332,22 @@ def test_a_wait_that_runs_out_is_reported(dev):
             lib.slmt_set_wait_limit_ns(prev)
         assert kd.read_device_errors(dev) == 4 and took < 1.0
         _check(kd.kv_prompt_attention(q, k, v, start, 900), *_ref(q, k, v, lens, d ** -0.5, torch.float32))
+
+
+@pytest.mark.parametrize("d, dtype", [(64, torch.bfloat16), (80, torch.float16), (128, torch.bfloat16)])
+def test_a_request_does_not_depend_on_the_batch(dev, d, dtype):
+    """The same bits alone, among others, and next to rows of NaN or enormous
+    queries (which share its last tile of rows)."""
+    lens, (hq, kv) = [77, 300, 5, 513], (8, 2)
+    q, k, v, start = _inputs(lens, hq, kv, d, dtype, dev)
+    whole = kd.kv_prompt_attention(q, k, v, start, 513)
+    for r, n in enumerate(lens):
+        a, b = int(start[r]), int(start[r + 1])
+        alone = kd.kv_prompt_attention(q[a:b], k[a:b], v[a:b], torch.tensor([0, n], dtype=torch.int32, device=dev), n)
+        assert torch.equal(alone, whole[a:b])
+        dirty = q.clone()
+        dirty[:a], dirty[b:] = math.nan, math.nan
+        if r == 1:
+            dirty[b:] = 3e4
+        got = kd.kv_prompt_attention(dirty, k, v, start, 513)
+        assert torch.equal(got[a:b], whole[a:b])

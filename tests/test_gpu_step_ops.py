@@ -106,6 +106,9 @@ def test_page_plan_reports_what_does_not_fit(dev):
     slots, _, cur = kd.kv_page_plan(i32(0, 1, 2), i32(1, 1), bt, 16, 2, free_blocks=i32(5))
     assert slots.tolist() == [80, -1] and bt[:, 0].tolist() == [5, -1] and cur.item() == 1
     assert kd.read_device_errors(dev) == FREE_BLOCKS
+    # an empty list
+    slots, _, cur = kd.kv_page_plan(i32(0, 1), i32(1), bt[:1], 16, 1, free_blocks=i32())
+    assert slots.tolist() == [-1] and cur.item() == 0 and kd.read_device_errors(dev) == FREE_BLOCKS
     # a cursor behind the list
     slots, _, cur = kd.kv_page_plan(i32(0, 1), i32(1), bt[:1], 16, 1, free_blocks=i32(5), free_cursor=i32(3))
     assert slots.tolist() == [-1] and kd.read_device_errors(dev) == FREE_BLOCKS

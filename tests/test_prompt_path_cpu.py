@@ -171,6 +171,9 @@ def test_frequencies_equal_transformers():
 
 def test_bad_frequency_requests():
     for args in ((7,), (0,), (64, 0.0), (64, 10000.0, {"rope_type": "linear"}), (64, 10000.0, {"rope_type": "spiral"}),
-                 (64, 10000.0, {"rope_type": "llama3", "factor": 8.0})):
+                 (64, 10000.0, {"rope_type": "llama3", "factor": 8.0}),
+                 (64, 10000.0, {"rope_type": "llama3", "factor": 8.0, "low_freq_factor": 4.0, "high_freq_factor": 4.0,
+                                "original_max_position_embeddings": 8192}),
+                 (64, 1.0, {"rope_type": "yarn", "factor": 8.0, "original_max_position_embeddings": 8192})):
         with pytest.raises(RuntimeError):
             kd.kv_rotary_inv_freq(*args)
