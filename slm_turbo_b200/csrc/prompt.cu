@@ -380,26 +380,28 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int j = 0; j < cur.nk; ++j) {
           const uint32_t fv = fill + 2 * j + 1, fk = fv + 1;
           const bool more_keys = j + 1 < cur.nk;
-          if (!full(fv)) break;
-          if (j >= cur.guard) {
+          if (j >= cur.guard) {  // looked at: there, too
             const uint32_t s = fv % STAGES;
             if (!wait(&c->v_ok[s], ok_phase >> s)) break;
             ok_phase ^= 1u << s;
             bad |= c->slot_bad[s][0] | c->slot_bad[s][1];
+          } else if (!full(fv)) {
+            break;
           }
           if (more_keys && !full(fk)) break;
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
             if (2 * j >= cur.steps[x] || failed) continue;
+            const bool two = 2 * j + 1 < cur.steps[x];
             if (!wait(&c->p_ready[x][0], p_phase[x])) continue;
             tc_fence_after();
             weigh(x, 0, fv, j == 0);
-            if (!wait(&c->p_ready[x][1], p_phase[x])) continue;
-            p_phase[x] ^= 1u;
-            if (2 * j + 1 < cur.steps[x]) {
+            if (two) {
+              if (!wait(&c->p_ready[x][1], p_phase[x])) continue;
               tc_fence_after();
               weigh(x, 1, fv, false);
             }
+            p_phase[x] ^= 1u;
             if (2 * j + 2 < cur.steps[x]) {
               scores(x, fk, 2 * j + 3 < cur.steps[x], 2 * j + 4 >= cur.steps[x]);
             } else {
