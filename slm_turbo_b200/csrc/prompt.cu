@@ -23,7 +23,7 @@
 // a tile's softmax (1950) and its products (950 with their signals) take turns,
 // so a step takes about 2900.  Long prompts run into the power cap before that
 // counts: one of 16384 tokens (32/8 heads, bf16) takes 1.72 ms, 1280 TFLOP/s,
-// in a short run and about 1.95 ms, 1130 TFLOP/s, with the clock held at 1.7
+// in a short run and about 2.0 ms, 1100 TFLOP/s, with the clock held at 1.7
 // GHz.  Short ones are bound by their chain: products, softmax, products,
 // output (a prompt of 130 tokens beside three shorter ones: 9.6 us).
 // Measured and dropped, in turn on one box: scores of 64 keys at a time into
@@ -169,6 +169,12 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
+template <bool BF16>
+__device__ __forceinline__ uint4 pack8(const float* x) {
+  return make_uint4(pack16<BF16>(x[0], x[1]), pack16<BF16>(x[2], x[3]), pack16<BF16>(x[4], x[5]),
+                    pack16<BF16>(x[6], x[7]));
+}
+
 template <int D, bool BF16>
 __global__ void __launch_bounds__(kThreads, 1)
     prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
@@ -201,11 +207,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   if (warp == 8) tmem_alloc(&c->tmem, kTmemCols);
   if (tid == 32 * 9) prefetch_map(&map_q), prefetch_map(&map_k), prefetch_map(&map_v);
-  int n2 = 4;
-  while (n2 < p.num_reqs) n2 <<= 1;
+  constexpr int COUNTED = 512;  // requests ranked by counting, more are sorted
+  int padded = (p.num_reqs + 3) & ~3;
+  if (padded > COUNTED) padded = kMaxReqs;
   unsigned bad_len = 0u;
-  uint32_t mine = 0u;
-  for (int r = tid; r < n2; r += kThreads) {
+  for (int r = tid; r < padded; r += kThreads) {
     int n = 0, a = 0;
     if (r < p.num_reqs) {
       const int qa = p.qsl[r], qb = p.qsl[r + 1];
@@ -219,28 +225,34 @@ __global__ void __launch_bounds__(kThreads, 1)
       c->rows[r] = n;
     }
     const int pairs = (n + 2 * p.tile_tokens - 1) / (2 * p.tile_tokens);
-    mine = ((uint32_t)pairs << kReqBits) | (uint32_t)r;
-    c->sort_key[r] = mine;
+    c->sort_key[r] = ((uint32_t)pairs << kReqBits) | (uint32_t)r;
   }
   if (bad_len && blockIdx.x == 0 && p.err) atomicOr(reinterpret_cast<unsigned int*>(p.err), bad_len);
   __syncthreads();
-  if (n2 <= 256) {
-    // a thread counts the keys above its own (all differ): 48 requests 2 us
-    // sooner than by the sort below, whose every pass is a barrier
-    int rank = 0;
-    if (tid < n2) {
+  if (padded <= COUNTED) {
+    // A thread counts the keys above its own (all differ), n^2 comparisons;
+    // the sort below has a barrier in each of its log^2 n passes.  48 requests
+    // are 2 us sooner this way, 300 are 5, 1000 would be 6 later.
+    constexpr int OWN = (COUNTED + kThreads - 1) / kThreads;
+    uint32_t mine[OWN];
+    int rank[OWN] = {};
+#pragma unroll
+    for (int i = 0; i < OWN; ++i) mine[i] = tid + i * kThreads < padded ? c->sort_key[tid + i * kThreads] : 0u;
 #pragma unroll 4
-      for (int i = 0; i < n2; i += 4) {
-        const uint4 k = *reinterpret_cast<const uint4*>(c->sort_key + i);
-        rank += (k.x > mine) + (k.y > mine) + (k.z > mine) + (k.w > mine);
-      }
+    for (int r = 0; r < padded; r += 4) {
+      const uint4 k = *reinterpret_cast<const uint4*>(c->sort_key + r);
+#pragma unroll
+      for (int i = 0; i < OWN; ++i)
+        rank[i] += (k.x > mine[i]) + (k.y > mine[i]) + (k.z > mine[i]) + (k.w > mine[i]);
     }
     __syncthreads();
-    if (tid < n2) c->sort_key[rank] = mine;
+#pragma unroll
+    for (int i = 0; i < OWN; ++i)
+      if (tid + i * kThreads < padded) c->sort_key[rank[i]] = mine[i];
   } else {
-    for (int k = 2; k <= n2; k <<= 1)
+    for (int k = 2; k <= padded; k <<= 1)
       for (int j = k >> 1; j > 0; j >>= 1) {
-        for (int i = tid; i < n2; i += kThreads) {
+        for (int i = tid; i < padded; i += kThreads) {
           const int o = i ^ j;
           if (o > i) {
             const uint32_t x = c->sort_key[i], y = c->sort_key[o];
@@ -540,14 +552,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           continue;
         }
+        if (p.out_dtype == SLMT_DTYPE_BF16) {
 #pragma unroll
-        for (int k = 0; k < PIECES; ++k) {
-          uint32_t w4[4];
+          for (int k = 0; k < PIECES; ++k) stage[place(lane, k)] = pack8<true>(o + 8 * k);
+        } else {
 #pragma unroll
-          for (int l = 0; l < 4; ++l)
-            w4[l] = p.out_dtype == SLMT_DTYPE_BF16 ? pack16<true>(o[8 * k + 2 * l], o[8 * k + 2 * l + 1])
-                                                   : pack16<false>(o[8 * k + 2 * l], o[8 * k + 2 * l + 1]);
-          stage[place(lane, k)] = make_uint4(w4[0], w4[1], w4[2], w4[3]);
+          for (int k = 0; k < PIECES; ++k) stage[place(lane, k)] = pack8<false>(o + 8 * k);
         }
         __syncwarp();
 #pragma unroll
