@@ -756,7 +756,8 @@ extern "C" int slmt_prompt_attention(const void* q, int64_t q_token_stride, int6
   if (dtype != SLMT_DTYPE_F16 && dtype != SLMT_DTYPE_BF16) return SLMT_ERR_DTYPE;
   if (out_dtype != SLMT_DTYPE_F32 && out_dtype != SLMT_DTYPE_F16 && out_dtype != SLMT_DTYPE_BF16)
     return SLMT_ERR_DTYPE;
-  if (!(sm_scale > 0.f) || !(sm_scale - sm_scale == 0.f)) return SLMT_ERR_SHAPE;
+  const float scale_log2 = sm_scale * 1.4426950408889634f;
+  if (!(sm_scale > 0.f) || !(scale_log2 - scale_log2 == 0.f)) return SLMT_ERR_SHAPE;
   if (num_reqs == 0 || max_query_len == 0 || num_tokens == 0) return SLMT_OK;
   if (!q || !k || !v || !out || !query_start_loc) return SLMT_ERR_NULL;
   if (rows_overlap(num_tokens, num_q_heads, out_token_stride, out_head_stride)) return SLMT_ERR_SHAPE;
@@ -793,7 +794,7 @@ extern "C" int slmt_prompt_attention(const void* q, int64_t q_token_stride, int6
   p.o_tok = out_token_stride, p.o_head = out_head_stride;
   p.wait_limit_ns = wait_limit_ns();
   p.stall = debug_stall();
-  p.scale_log2 = sm_scale * 1.4426950408889634f;
+  p.scale_log2 = scale_log2;
   p.num_tokens = (int)num_tokens;
   p.max_query = (int)max_query;
   p.kv = (int)num_kv_heads;

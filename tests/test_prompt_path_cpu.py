@@ -87,6 +87,7 @@ PROMPT_BASE = dict(q=P, qt=1024, qh=128, k=P, kt=256, kh=128, v=P, vt=256, vh=12
     (dict(d=96), HEAD_DIM), (dict(hq=9), SHAPE), (dict(kv=0), SHAPE), (dict(r=-1), SHAPE), (dict(mq=-1), SHAPE),
     (dict(n=-1), SHAPE), (dict(hq=258, kv=2), UNSUPPORTED), (dict(dt=2), DTYPE), (dict(odt=3), DTYPE),
     (dict(sc=0.0), SHAPE), (dict(sc=-1.0), SHAPE), (dict(sc=math.inf), SHAPE), (dict(sc=math.nan), SHAPE),
+    (dict(sc=3e38), SHAPE),  # its log2 e is not finite
     (dict(q=None), NULL), (dict(k=None), NULL), (dict(v=None), NULL), (dict(out=None), NULL), (dict(qsl=None), NULL),
     (dict(q=P + 2), ALIGN), (dict(k=P + 8), ALIGN), (dict(v=P + 8), ALIGN), (dict(out=P + 4), ALIGN),
     (dict(qt=1028), ALIGN), (dict(kh=130), ALIGN), (dict(vt=257), ALIGN), (dict(ot=1022), ALIGN), (dict(ot=0), SHAPE),
