@@ -75,6 +75,13 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity,
   }
 }
 
+// One 32-byte store; `to` is 32-byte aligned.
+__device__ __forceinline__ void st_global_256(void* to, const uint4& a, const uint4& b) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(a.x), "r"(a.y), "r"(a.z),
+               "r"(a.w), "r"(b.x), "r"(b.y), "r"(b.z), "r"(b.w)
+               : "memory");
+}
+
 // ------------------------------------------------------------ async copies --
 // 1-D bulk copy global -> shared (TMA unit), completes `bytes` of tx on `bar`.
 // src and dst 16-byte aligned, bytes a multiple of 16; the source is always

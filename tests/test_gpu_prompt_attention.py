@@ -153,6 +153,22 @@ def test_strided_inputs_and_outputs(dev):
     _check(kd.kv_prompt_attention(q, k1, v1, start, 200), *_ref(q, k1, v1, lens, 1 / math.sqrt(d), torch.float32))
 
 
+@pytest.mark.parametrize("d", [64, 80, 128])
+@pytest.mark.parametrize("out_dtype", [torch.float32, torch.float16, torch.bfloat16], ids=str)
+def test_output_rows_on_16_bytes(dev, d, out_dtype):
+    """Rows that start on 16 bytes but not on 32: the same bits as elsewhere."""
+    lens, hq, kv = [70, 1, 200], 4, 2
+    q, k, v, start = _inputs(lens, hq, kv, d, torch.bfloat16, dev)
+    want = kd.kv_prompt_attention(q, k, v, start, 200, out=torch.empty(q.shape, dtype=out_dtype, device=dev))
+    pad = 16 // want.element_size()
+    rows = torch.full((sum(lens), hq * d + 2 * pad), 7.5, dtype=out_dtype, device=dev)
+    got = rows[:, pad:pad + hq * d].view(-1, hq, d)
+    assert got.data_ptr() % 32 == 16
+    kd.kv_prompt_attention(q, k, v, start, 200, out=got)
+    assert torch.equal(got, want)
+    assert (rows[:, :pad] == 7.5).all() and (rows[:, pad + hq * d:] == 7.5).all()
+
+
 def test_skipped_requests_and_rows_outside(dev):
     """Requests with a cached context, and the padding, are left as they were."""
     lens, hq, kv, d = [30, 5, 129, 1], 4, 2, 64
