@@ -34,8 +34,13 @@
 // pipe (12 instructions in place of 2): 2.0-2.4 ms, 2.2-2.4 ms, 2.2 ms and
 // 1.93 against 1.95 ms.
 //
-// The next item's first scores go out as soon as this one's products are
-// issued, and an item's output is written behind the next one's first weights.
+// A tile's first scores of the next item go out behind its own last products,
+// before the other tile's: what it does then falls beside the other's end, and
+// the two do not run into the next item in step.  An item's output is written
+// behind the next one's first weights; at D 64 tensor memory has room for two
+// accumulators per tile, so those weights need not wait for it (48 prompts of
+// 5 to 393 tokens, 32/4 heads: 44.6 us; with one accumulator and the tiles
+// starting together 48.0).
 //
 // Running maximum: the reference m of a row moves only when a score passes it
 // by more than 2^8 in weight; until then old weights stay on their scale, and
@@ -77,11 +82,11 @@ struct PromptParams {
 };
 
 struct PromptCtl {
-  uint64_t q_full[2], q_empty[2], o_full[2], drain, never;
+  uint64_t q_full[2], q_empty[2], o_full[2][2], drain, never;  // o_full: [tile][accumulator]
   uint64_t s_full[2], p_ready[2][2];  // [tile], [tile][first or second 64 keys]
   uint64_t kv_full[kMaxStages], kv_empty[kMaxStages], v_ok[kMaxStages];
   uint32_t tmem;
-  uint32_t tile_bad[2];
+  uint32_t tile_bad[2][2];
   uint32_t slot_bad[kMaxStages][2];
   alignas(16) uint32_t sort_key[kMaxReqs];  // (pairs of tiles << kReqBits) | request, descending
   int start[kMaxReqs], rows[kMaxReqs];
@@ -92,6 +97,7 @@ struct PromptGeom {
   static constexpr int PANELS = (D + 63) / 64;        // 128-byte wide panels of a tile
   static constexpr int TILE = PANELS * 128 * 128;     // bytes
   static constexpr int STAGES = D == 64 ? 6 : 4;      // K and V take turns: an even number
+  static constexpr int OUTS = D == 64 ? 2 : 1;        // accumulators of a tile: what tensor memory has room for
   static constexpr int SMEM = 1024 + (2 + STAGES) * TILE + (int)sizeof(PromptCtl);
   static_assert(SMEM <= 227 * 1024 && STAGES % 2 == 0 && STAGES <= kMaxStages, "");
 };
@@ -100,8 +106,8 @@ struct PromptGeom {
 struct Item {
   int req, head;     // request of this launch, kv head
   int start, rows;   // the request's first row and its number of rows
-  int tok[2];        // first token of tile A and B
-  int steps[2];      // 64-key steps of each (0: no rows in tile B)
+  int tok[2];        // first token of tile A and of tile B
+  int steps[2];      // 64-key steps of each (0: no rows in the tile)
   int nk;            // 128-key tiles loaded
   int guard;         // first of these that some row of A or B does not see whole
 };
@@ -144,12 +150,14 @@ struct Walk {
     it.req = (int)(c->sort_key[rank] & ((1u << kReqBits) - 1));
     it.start = c->start[it.req];
     it.rows = c->rows[it.req];
-    it.tok[0] = level * 2 * p.tile_tokens;
-    it.tok[1] = it.tok[0] + p.tile_tokens;
-    it.steps[0] = (min(it.tok[1], it.rows) + 63) >> 6;
-    it.steps[1] = it.tok[1] < it.rows ? (min(it.tok[1] + p.tile_tokens, it.rows) + 63) >> 6 : 0;
-    it.nk = (max(it.steps[0], it.steps[1]) + 1) >> 1;
-    it.guard = (it.tok[0] + 1) >> 7;
+    const int lo = level * 2 * p.tile_tokens, hi = lo + p.tile_tokens;
+    const int steps_lo = (min(hi, it.rows) + 63) >> 6;
+    const int steps_hi = hi < it.rows ? (min(hi + p.tile_tokens, it.rows) + 63) >> 6 : 0;
+    const bool turn = (row & 1) == 0;  // A and B take the longer tile in turn, and the only one
+    it.tok[0] = turn ? hi : lo, it.tok[1] = turn ? lo : hi;
+    it.steps[0] = turn ? steps_hi : steps_lo, it.steps[1] = turn ? steps_lo : steps_hi;
+    it.nk = (max(steps_lo, steps_hi) + 1) >> 1;
+    it.guard = (lo + 1) >> 7;
     return true;
   }
 };
@@ -195,7 +203,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&c->q_full[x], 1), mbar_init(&c->q_empty[x], 1);
       mbar_init(&c->s_full[x], 1);
       for (int h = 0; h < 2; ++h) mbar_init(&c->p_ready[x][h], 128);
-      mbar_init(&c->o_full[x], 2);  // the commit, and the thread that set tile_bad
+      for (int o = 0; o < 2; ++o) mbar_init(&c->o_full[x][o], 2);  // the commit, and the thread that set tile_bad
     }
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(&c->kv_full[s], 1);
@@ -303,7 +311,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         Item it;
         w.begin(c);
         while (!failed && w.next(c, p, it)) {
-          bool ok = load_kv(it, 0, &map_k) && load_q(it, 0) && (it.steps[1] == 0 || load_q(it, 1));
+          bool ok = load_kv(it, 0, &map_k) && (it.steps[0] == 0 || load_q(it, 0)) && (it.steps[1] == 0 || load_q(it, 1));
           ok = ok && load_kv(it, 0, &map_v);
           for (int j = 1; ok && j < it.nk; ++j) ok = load_kv(it, j, &map_k) && load_kv(it, j, &map_v);
           failed = !ok;
@@ -325,7 +333,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
       const uint32_t q_lo = desc_lo(smem_addr(smem), 16), k_lo = desc_lo(smem_addr(ring), 16),
                      v_lo = desc_lo(smem_addr(ring), 16384);
-      uint32_t fill = 0, nq[2] = {0, 0}, p_phase[2] = {0, 0}, ok_phase = 0;
+      uint32_t fill = 0, nq[2] = {0, 0}, p_phase[2] = {0, 0}, ok_phase = 0, out[2] = {0, 0};
       auto wait = [&](uint64_t* bar, uint32_t phase) {
         const bool ok = __all_sync(0xffffffffu, mbar_wait(bar, phase & 1u, limit));
         failed |= !ok;
@@ -356,7 +364,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (leader) {
 #pragma unroll
           for (int u = 0; u < 4; ++u)
-            mma_ts(tm + col_o + D * x, tm + col_s + 128 * x + 32 * h + 8 * u, b + u * (2048 >> 4), HI, idesc_o,
+            mma_ts(tm + col_o + D * (G::OUTS * x + out[x]), tm + col_s + 128 * x + 32 * h + 8 * u, b + u * (2048 >> 4), HI, idesc_o,
                    u > 0 || !first);
         }
       };
@@ -381,6 +389,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       };
       Next cur, nxt;
       fetch(cur);
+      // Whether tile x's first scores of item n can go out without a wait.  The
+      // queries are asked for behind the keys: once they are there, the keys'
+      // barrier is in the phase that is looked at.
+      auto at_hand = [&](const Next& n, int x, uint32_t f) {
+        return n.steps[x] != 0 && __all_sync(0xffffffffu, mbar_test(&c->q_full[x], nq[x] & 1u)) &&
+               __all_sync(0xffffffffu, mbar_test(&c->kv_full[f % STAGES], (f / STAGES) & 1u));
+      };
 #pragma unroll
       for (int x = 0; x < 2; ++x)
         if (!failed) begin_tile(cur, x, fill);
@@ -389,6 +404,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         fetch(nxt);
         const uint32_t next_fill = fill + 2 * cur.nk;
         uint32_t bad = 0;
+        bool begun[2] = {false, false};  // with the next item
         for (int j = 0; j < cur.nk; ++j) {
           const uint32_t fv = fill + 2 * j + 1, fk = fv + 1;
           const bool more_keys = j + 1 < cur.nk;
@@ -414,15 +430,25 @@ __global__ void __launch_bounds__(kThreads, 1)
               weigh(x, 1, fv, false);
             }
             p_phase[x] ^= 1u;
-            if (2 * j + 2 < cur.steps[x]) {
-              scores(x, fk, 2 * j + 3 < cur.steps[x], 2 * j + 4 >= cur.steps[x]);
-            } else {
+            bool go = 2 * j + 2 < cur.steps[x];
+            uint32_t next_k = fk;
+            int left = cur.steps[x] - 2 * j - 2;
+            if (!go) {
               if (leader) {
-                c->tile_bad[x] = bad;
-                mbar_arrive(&c->o_full[x]);
-                mma_commit(&c->o_full[x]);
+                c->tile_bad[x][out[x]] = bad;
+                mbar_arrive(&c->o_full[x][out[x]]);
+                mma_commit(&c->o_full[x][out[x]]);
+              }
+              if (G::OUTS == 2) out[x] ^= 1u;
+              // the next item's first scores, where the other tile has products to come
+              if ((2 * j + 2 < cur.steps[x ^ 1] || (x == 0 && 2 * j < cur.steps[1])) && at_hand(nxt, x, next_fill)) {
+                ++nq[x];
+                tc_fence_after();
+                go = begun[x] = true;
+                next_k = next_fill, left = nxt.steps[x];
               }
             }
+            if (go) scores(x, next_k, left > 1, left <= 2);
           }
           if (failed) break;
           release(fv);
@@ -430,7 +456,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
 #pragma unroll
         for (int x = 0; x < 2; ++x)
-          if (!failed) begin_tile(nxt, x, next_fill);
+          if (!failed && !begun[x]) begin_tile(nxt, x, next_fill);
         if (nxt.nk && !failed) release(next_fill);
         fill = next_fill;
         cur = nxt;
@@ -491,12 +517,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int x = warp >> 2, row = tid & 127;
     const int row_tok = row / p.group, row_head = row - row_tok * p.group;
     const uint32_t lane_base = (uint32_t)(warp & 3) << 21;
-    const uint32_t ts = tmem + lane_base + col_s + 128 * x, to = tmem + lane_base + col_o + D * x;
+    const uint32_t ts = tmem + lane_base + col_s + 128 * x, outs = tmem + lane_base + col_o + D * G::OUTS * x;
+    uint32_t to = outs;  // the accumulator of the item at hand
     const float sc = p.scale_log2;
     uint32_t ns = 0, no = 0;
     // A finished item's output is written after the next item's first weights
-    // are computed and before they are announced (that product overwrites O):
-    // the wait for the item's last product is then over.
+    // are computed: the wait for the item's last product is then over.  With two
+    // accumulators the weights are announced before it, with one after it (that
+    // product overwrites O).
     struct Pending {
       int64_t at;
       float sum;
@@ -506,13 +534,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     last.any = false;
     auto finish = [&] {
       last.any = false;
-      if (!__all_sync(0xffffffffu, mbar_wait(&c->o_full[x], no++ & 1u, limit))) {
+      const uint32_t buf = no % G::OUTS, from = outs + D * buf;
+      if (!__all_sync(0xffffffffu, mbar_wait(&c->o_full[x][buf], (no++ / G::OUTS) & 1u, limit))) {
         failed = true;
         return;
       }
       tc_fence_after();
       const float inv = 1.f / last.sum;
-      const bool bad = c->tile_bad[x] != 0;
+      const bool bad = c->tile_bad[x][buf] != 0;
       // A thread writes its own row, a 32-byte sector at a time.  Turning the
       // rows in shared memory first, so that a warp's store covers whole lines,
       // cost more than the lines do (1000 short requests 169 us for 155, 48 of
@@ -522,7 +551,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         float o[OUT];
         __syncwarp();
 #pragma unroll
-        for (int k = 0; k < OUT; k += 16) tmem_ld16(o + k, to + i + k);
+        for (int k = 0; k < OUT; k += 16) tmem_ld16(o + k, from + i + k);
         tmem_wait_ld();
         if (!last.valid) continue;
         if (bad) {
@@ -631,7 +660,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int k = 0; k < KEYS; ++k) s[k] -= base;
         if (far) offset = SHIFT;
       }
-      const bool hold = j == 0 && last.any;  // the last item's output comes first
+      const bool pending = j == 0 && last.any, hold = G::OUTS == 1 && pending;  // the last item's output
       const uint64_t scale2 = f2_pack(sc, sc), offset2 = f2_pack(offset, offset);
       uint64_t acc0 = f2_pack(0.f, 0.f), acc1 = acc0;
 #pragma unroll
@@ -667,6 +696,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_before();
       if (hold || KEYS == 64) mbar_arrive(&c->p_ready[x][0]);
       mbar_arrive(&c->p_ready[x][1]);
+      if (pending && !hold) {
+        const float keep = sum;
+        finish();
+        __syncwarp();
+        sum = keep;
+        if (failed) return false;
+      }
       return true;
     };
     Walk w;
@@ -688,6 +724,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       last.at = (int64_t)(it.start + tok) * p.o_tok + (int64_t)h * p.o_head;
       last.sum = sum;
       last.start = it.start, last.head = it.head, last.tok = tok, last.guard = it.guard;
+      if (G::OUTS == 2) to = to == outs ? outs + D : outs;
       last.any = true, last.valid = row_tok < p.tile_tokens && it.tok[x] + row_tok < it.rows;
     }
     if (!failed && last.any) finish();
