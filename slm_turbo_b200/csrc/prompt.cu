@@ -16,7 +16,8 @@
 // while one of them works on its scores, the tensor core computes the other
 // tile's products.  Warp 8 issues the products, warp 9 the tiled copies into
 // a ring of K and V tiles, warps 10 and 11 look at the V tiles on the
-// diagonal (below).  Every role walks the same list of items by itself.
+// diagonal (below).  Warp 9 also walks the list of items and hands them to the
+// other roles through a ring.
 //
 // What bounds it, per step of 256 rows by 128 keys at D 128 (cycles of an SM):
 // the products need 4 * 512, the exponentials 2 * 1024 of the 16-a-clock unit;
@@ -25,7 +26,7 @@
 // counts: one of 16384 tokens (32/8 heads, bf16) takes 1.72 ms, 1280 TFLOP/s,
 // in a short run and about 2.0 ms, 1100 TFLOP/s, with the clock held at 1.7
 // GHz.  Short ones are bound by their chain: products, softmax, products,
-// output (a prompt of 130 tokens beside three shorter ones: 9.6 us).
+// output (a prompt of 130 tokens beside three shorter ones: 9.5 us).
 // Measured and dropped, in turn on one box: scores of 64 keys at a time into
 // alternating halves (the softmax then never waits, but S costs 768 cycles in
 // place of 512 and its products change accumulators twice as often), one
@@ -39,8 +40,8 @@
 // the two do not run into the next item in step.  An item's output is written
 // behind the next one's first weights; at D 64 tensor memory has room for two
 // accumulators per tile, so those weights need not wait for it (48 prompts of
-// 5 to 393 tokens, 32/4 heads: 44.6 us; with one accumulator and the tiles
-// starting together 48.0).
+// 5 to 393 tokens, 32/4 heads: 42 us; with one accumulator and the tiles
+// starting together 3.4 more).
 //
 // Running maximum: the reference m of a row moves only when a score passes it
 // by more than 2^8 in weight; until then old weights stay on their scale, and
@@ -61,11 +62,28 @@ namespace slmt {
 
 namespace {
 
+// mbar_wait in fewer instructions.  The roles' code between two items runs once
+// and has left the instruction cache when it is needed again, so short items
+// pay for its length: with mbar_wait at every wait, and with the items walked
+// and the copies written out by each role that needs them, 1000 short requests
+// took 132 us instead of 115, 48 of 5 to 393 tokens 44.8 instead of 42.0.
+__device__ __forceinline__ bool wait_short(uint64_t* bar, uint32_t parity, uint64_t limit_ns) {
+  uint64_t t0 = 0;
+#pragma unroll 1
+  while (!mbar_try_wait(bar, parity)) {
+    const uint64_t now = global_timer_ns();
+    if (t0 == 0) t0 = now;
+    if (now - t0 > limit_ns) return false;
+  }
+  return true;
+}
+
 constexpr int kThreads = 384;
 constexpr int kMaxReqs = 1024;    // requests of one launch (sorted in shared memory)
 constexpr int kReqBits = 10;
 constexpr uint32_t kTmemCols = 512;
 constexpr int kMaxStages = 6;
+constexpr int kItems = 8;          // ring of work items
 
 struct PromptParams {
   const void* v;
@@ -81,15 +99,27 @@ struct PromptParams {
   uint32_t kv_recip;  // 2^32 / kv, rounded up
 };
 
+// One work item, as every role sees it.
+struct Item {
+  int head;          // kv head
+  int start, rows;   // the request's first row and its number of rows
+  int tok[2];        // first token of tile A and of tile B
+  int steps[2];      // 64-key steps of each (0: no rows in the tile)
+  int nk;            // 128-key tiles loaded (0: no more items)
+  int guard;         // first of these that some row of A or B does not see whole
+};
+
 struct PromptCtl {
   uint64_t q_full[2], q_empty[2], o_full[2][2], drain, never;  // o_full: [tile][accumulator]
   uint64_t s_full[2], p_ready[2][2];  // [tile], [tile][first or second 64 keys]
   uint64_t kv_full[kMaxStages], kv_empty[kMaxStages], v_ok[kMaxStages];
+  uint64_t item_full[kItems], item_empty[kItems];
   uint32_t tmem;
   uint32_t tile_bad[2][2];
   uint32_t slot_bad[kMaxStages][2];
   alignas(16) uint32_t sort_key[kMaxReqs];  // (pairs of tiles << kReqBits) | request, descending
   int start[kMaxReqs], rows[kMaxReqs];
+  Item items[kItems];
 };
 
 template <int D>
@@ -102,54 +132,59 @@ struct PromptGeom {
   static_assert(SMEM <= 227 * 1024 && STAGES % 2 == 0 && STAGES <= kMaxStages, "");
 };
 
-// One work item, as every role sees it.
-struct Item {
-  int req, head;     // request of this launch, kv head
-  int start, rows;   // the request's first row and its number of rows
-  int tok[2];        // first token of tile A and of tile B
-  int steps[2];      // 64-key steps of each (0: no rows in the tile)
-  int nk;            // 128-key tiles loaded
-  int guard;         // first of these that some row of A or B does not see whole
-};
-
 // The items in the order of falling cost -- requests' last tiles first -- dealt
-// to the CTAs back and forth, so that their sums stay within about one small
-// item of each other.  Level t holds the items of tile pair t of every request
-// that has one: those are the first `count` of the requests sorted by length.
+// to the CTAs in rows, each row in the direction that gives its longer items to
+// the end with the smaller sum so far (1999 + 777 + 63 tokens of 32 heads, D 80:
+// 50.4 us; back and forth in turn 54.5, the longest CTA has 24 steps instead of
+// 22).  Level t holds the items of tile pair t of every request that has one:
+// those are the first `count` of the requests sorted by length.
 // A whole warp walks together.
 struct Walk {
   int row, level, count, base;  // deal, tile pair, requests of the level, items before it
   int longest;                  // pairs of the longest request that is not among them
+  int first, lead;              // cost of the row's first item; first CTA's sum less the last one's
+  int back;                     // -1: the row runs from the last CTA to the first, else 0
   __device__ __forceinline__ void begin(const PromptCtl* c) {
-    row = 0, count = 0, base = 0;
+    row = 0, count = 0, base = 0, lead = 0, back = 0;
     level = longest = (int)(c->sort_key[0] >> kReqBits);
+    first = level - 1;
   }
   __device__ __forceinline__ bool next(const PromptCtl* c, const PromptParams& p, Item& it) {
     const int nc = gridDim.x, me = blockIdx.x;
-    const int at = row * nc + ((row & 1) ? nc - 1 - me : me);
-    ++row;
-    int in_level = count * p.kv;
-    while (at - base >= in_level) {
-      base += in_level;
-      if (--level < 0) return false;
-      while (longest > level) {  // requests join: 32 looked at together
-        const int i = count + (int)(threadIdx.x & 31);
-        const int pairs = i < p.num_reqs ? (int)(c->sort_key[i] >> kReqBits) : 0;
-        const uint32_t in = __ballot_sync(0xffffffffu, pairs > level);
-        count += __popc(in);
-        longest = in == 0xffffffffu ? (count < p.num_reqs ? (int)(c->sort_key[count] >> kReqBits) : 0)
-                                    : __shfl_sync(0xffffffffu, pairs, __ffs(~in) - 1);
+    int at = row == 0 ? me : row * nc;
+#pragma unroll 1
+    for (int pass = row == 0;; ++pass) {  // to the row's first item, then to this CTA's
+      int in_level = count * p.kv;
+      while (at - base >= in_level) {
+        base += in_level;
+        if (--level < 0) return false;
+        while (longest > level) {  // requests join: 32 looked at together
+          const int i = count + (int)(threadIdx.x & 31);
+          const int pairs = i < p.num_reqs ? (int)(c->sort_key[i] >> kReqBits) : 0;
+          const uint32_t in = __ballot_sync(0xffffffffu, pairs > level);
+          count += __popc(in);
+          longest = in == 0xffffffffu ? (count < p.num_reqs ? (int)(c->sort_key[count] >> kReqBits) : 0)
+                                      : __shfl_sync(0xffffffffu, pairs, __ffs(~in) - 1);
+        }
+        in_level = count * p.kv;
       }
-      in_level = count * p.kv;
+      if (pass) break;
+      // an item costs about its last key, in tile pairs; the last item of a row
+      // costs about what the first of the next does
+      lead += ((first - level) ^ back) - back;
+      first = level;
+      back = lead > 0 ? -1 : 0;
+      at += back ? nc - 1 - me : me;
     }
+    ++row;
     // rem / kv by 2^32 / kv rounded up (which kv 1 has no room for): at most one too large
     const int rem = at - base;
     int rank = p.kv == 1 ? rem : (int)__umulhi((uint32_t)rem, p.kv_recip);
     it.head = rem - rank * p.kv;
     if (it.head < 0) --rank, it.head += p.kv;
-    it.req = (int)(c->sort_key[rank] & ((1u << kReqBits) - 1));
-    it.start = c->start[it.req];
-    it.rows = c->rows[it.req];
+    const int req = (int)(c->sort_key[rank] & ((1u << kReqBits) - 1));
+    it.start = c->start[req];
+    it.rows = c->rows[req];
     const int lo = level * 2 * p.tile_tokens, hi = lo + p.tile_tokens;
     const int steps_lo = (min(hi, it.rows) + 63) >> 6;
     const int steps_hi = hi < it.rows ? (min(hi + p.tile_tokens, it.rows) + 63) >> 6 : 0;
@@ -209,6 +244,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&c->kv_full[s], 1);
       mbar_init(&c->kv_empty[s], s & 1 ? 3 : 1);  // the products; V tiles: and both guard warps
       mbar_init(&c->v_ok[s], 2);
+    }
+    for (int i = 0; i < kItems; ++i) {
+      mbar_init(&c->item_full[i], 1);
+      mbar_init(&c->item_empty[i], 11);  // the warps but the one that makes them
     }
     mbar_init(&c->drain, 1), mbar_init(&c->never, 1);
     fence_mbar_init();
@@ -298,49 +337,82 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t col_s = 0, col_o = 256;
 
   bool failed = false;
+  // the next item, for a warp that takes all of them in their order
+  uint32_t item_at = 0;
+  auto next_item = [&](Item& it) {
+    const uint32_t s = item_at % kItems;
+    if (!__all_sync(0xffffffffu, wait_short(&c->item_full[s], (item_at / kItems) & 1u, limit))) {
+      failed = true;
+      return false;
+    }
+    it = c->items[s];
+    ++item_at;
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&c->item_empty[s]);
+    return it.nk != 0;
+  };
   if (warp >= 8) {
     regs_lower<88>();
     if (warp == 9) {
       // ------------------------------------------------------------ copies
       {
         const bool leader = elect_one();
-        uint32_t fill = 0, nq[2] = {0, 0};
-        auto load_q = [&](const Item& it, int x) {
-          if (!__all_sync(0xffffffffu, mbar_wait(&c->q_empty[x], (nq[x] & 1u) ^ 1u, limit))) return false;
-          ++nq[x];
-          if (leader) {
-            mbar_arrive_expect_tx(&c->q_full[x], (uint32_t)(PANELS * 128 * p.tile_tokens * p.group));
-            for (int d = 0; d < PANELS; ++d)
-              tma_load_3d(smem + x * TILE + d * 16384, &map_q, d * 64, it.head * p.group, it.start + it.tok[x],
-                          &c->q_full[x]);
+        uint32_t fill = 0, queries = 0;  // bit x: parity of tile x's copies, bit 2 + x: whether there was one
+        // a tile of the ring or of the queries, once it is free; false: nothing is under way
+        auto load = [&](const CUtensorMap* map, uint64_t* empty, uint32_t phase, uint64_t* full, uint32_t bytes,
+                        uint8_t* to, int head, int row) {
+          if (!__all_sync(0xffffffffu, wait_short(empty, (phase & 1u) ^ 1u, limit))) {
+            failed = true;
+          } else if (leader) {
+            mbar_arrive_expect_tx(full, bytes);
+            for (int d = 0; d < PANELS; ++d) tma_load_3d(to + d * 16384, map, d * 64, head, row, full);
           }
-          return true;
+          return !failed;
         };
-        auto load_kv = [&](const Item& it, int j, const CUtensorMap* map) {
-          const uint32_t s = fill % STAGES;
-          if (!__all_sync(0xffffffffu, mbar_wait(&c->kv_empty[s], ((fill / STAGES) & 1u) ^ 1u, limit))) return false;
-          ++fill;
-          if (leader) {
-            mbar_arrive_expect_tx(&c->kv_full[s], TILE);
-            for (int d = 0; d < PANELS; ++d)
-              tma_load_3d(ring + s * TILE + d * 16384, map, d * 64, it.head, it.start + 128 * j, &c->kv_full[s]);
-          }
-          return true;
-        };
+        // The products look one item ahead: the next one is made known behind
+        // this one's first keys, queries and values.
         Walk w;
-        Item it;
+        Item it, nxt;
+        uint32_t at = 0;
+        int i = 2;
+        it.nk = 0;
         w.begin(c);
-        while (!failed && w.next(c, p, it)) {
-          bool ok = load_kv(it, 0, &map_k) && (it.steps[0] == 0 || load_q(it, 0)) && (it.steps[1] == 0 || load_q(it, 1));
-          ok = ok && load_kv(it, 0, &map_v);
-          for (int j = 1; ok && j < it.nk; ++j) ok = load_kv(it, j, &map_k) && load_kv(it, j, &map_v);
-          failed = !ok;
+        while (!failed) {
+          if (i == 2) {
+            if (!w.next(c, p, nxt)) nxt.nk = 0;
+            const uint32_t s = at % kItems;
+            if (!__all_sync(0xffffffffu, wait_short(&c->item_empty[s], ((at / kItems) & 1u) ^ 1u, limit))) {
+              failed = true;
+            } else if (leader) {
+              c->items[s] = nxt;
+              mbar_arrive(&c->item_full[s]);
+            }
+            ++at;
+          }
+          if (i >= 2 * it.nk) {
+            if (nxt.nk == 0) break;
+            it = nxt, i = 0;
+          }
+          const uint32_t s = fill % STAGES;  // K and V in turn
+          if (failed || !load(i & 1 ? &map_v : &map_k, &c->kv_empty[s], fill / STAGES, &c->kv_full[s], TILE,
+                              ring + s * TILE, it.head, it.start + 64 * (i & ~1)))
+            break;
+          ++fill;
+          if (i++ == 0) {
+#pragma unroll 1
+            for (int x = 0; x < 2; ++x)
+              if (!failed && (x ? it.steps[1] : it.steps[0]) &&
+                  load(&map_q, &c->q_empty[x], queries >> x, &c->q_full[x],
+                       (uint32_t)(PANELS * 128 * p.tile_tokens * p.group), smem + x * TILE, it.head * p.group,
+                       it.start + (x ? it.tok[1] : it.tok[0])))
+                queries = (queries ^ (1u << x)) | (4u << x);
+          }
         }
         // no copy is in flight when this warp is done, whatever happened
         for (uint32_t f = fill > (uint32_t)STAGES ? fill - STAGES : 0; f < fill; ++f)
-          if (!mbar_wait(&c->kv_full[f % STAGES], (f / STAGES) & 1u, drain_limit)) failed = true;
+          if (!wait_short(&c->kv_full[f % STAGES], (f / STAGES) & 1u, drain_limit)) failed = true;
         for (int x = 0; x < 2; ++x)
-          if (nq[x] && !mbar_wait(&c->q_full[x], (nq[x] - 1) & 1u, drain_limit)) failed = true;
+          if ((queries >> (2 + x) & 1u) && !wait_short(&c->q_full[x], (queries >> x & 1u) ^ 1u, drain_limit)) failed = true;
       }
     } else if (warp == 8) {
       // ----------------------------------------------------------- products
@@ -355,7 +427,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                      v_lo = desc_lo(smem_addr(ring), 16384);
       uint32_t fill = 0, nq[2] = {0, 0}, p_phase[2] = {0, 0}, ok_phase = 0, out[2] = {0, 0};
       auto wait = [&](uint64_t* bar, uint32_t phase) {
-        const bool ok = __all_sync(0xffffffffu, mbar_wait(bar, phase & 1u, limit));
+        const bool ok = __all_sync(0xffffffffu, wait_short(bar, phase & 1u, limit));
         failed |= !ok;
         return ok;
       };
@@ -391,11 +463,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       struct Next {
         int steps[2], nk, guard;
       };
-      Walk w;
-      w.begin(c);
       auto fetch = [&](Next& n) {
         Item it;
-        const bool more = w.next(c, p, it);
+        const bool more = next_item(it);
         n.steps[0] = __shfl_sync(0xffffffffu, more ? it.steps[0] : 0, 0);
         n.steps[1] = __shfl_sync(0xffffffffu, more ? it.steps[1] : 0, 0);
         n.nk = __shfl_sync(0xffffffffu, more ? it.nk : 0, 0);
@@ -407,8 +477,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_after();
         scores(x, f, n.steps[x] > 1, n.steps[x] <= 2);
       };
-      Next cur, nxt;
-      fetch(cur);
+      Next cur = {}, nxt;
       // Whether tile x's first scores of item n can go out without a wait.  The
       // queries are asked for behind the keys: once they are there, the keys'
       // barrier is in the phase that is looked at.
@@ -416,11 +485,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         return n.steps[x] != 0 && __all_sync(0xffffffffu, mbar_test(&c->q_full[x], nq[x] & 1u)) &&
                __all_sync(0xffffffffu, mbar_test(&c->kv_full[f % STAGES], (f / STAGES) & 1u));
       };
-#pragma unroll
-      for (int x = 0; x < 2; ++x)
-        if (!failed) begin_tile(cur, x, fill);
-      if (cur.nk) release(fill);
-      while (!failed && cur.nk) {
+      do {
         fetch(nxt);
         const uint32_t next_fill = fill + 2 * cur.nk;
         uint32_t bad = 0;
@@ -480,22 +545,20 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (nxt.nk && !failed) release(next_fill);
         fill = next_fill;
         cur = nxt;
-      }
+      } while (!failed && cur.nk);
       // products in flight read shared and tensor memory
       if (leader) mma_commit(&c->drain);
-      if (!mbar_wait(&c->drain, 0, drain_limit)) failed = true;
+      if (!wait_short(&c->drain, 0, drain_limit)) failed = true;
     } else {
       // ------------------------------------------- non-finite values in V
       constexpr uint32_t EXP = BF16 ? 0x7F80u : 0x7C00u;
       const int half = warp - 10;
       uint32_t fill = 0;
-      Walk w;
       Item it;
-      w.begin(c);
-      while (!failed && w.next(c, p, it)) {
+      while (!failed && next_item(it)) {
         for (int j = 0; j < it.nk; ++j) {
           const uint32_t f = fill + 2 * j + 1, s = f % STAGES;
-          if (!__all_sync(0xffffffffu, mbar_wait(&c->kv_full[s], (f / STAGES) & 1u, limit))) {
+          if (!__all_sync(0xffffffffu, wait_short(&c->kv_full[s], (f / STAGES) & 1u, limit))) {
             failed = true;
             break;
           }
@@ -555,7 +618,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     auto finish = [&] {
       last.any = false;
       const uint32_t buf = no % G::OUTS, from = outs + D * buf;
-      if (!__all_sync(0xffffffffu, mbar_wait(&c->o_full[x][buf], (no++ / G::OUTS) & 1u, limit))) {
+      if (!__all_sync(0xffffffffu, wait_short(&c->o_full[x][buf], (no++ / G::OUTS) & 1u, limit))) {
         failed = true;
         return;
       }
@@ -616,14 +679,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     };
     // test hook: a wait that runs out
-    if (p.stall && blockIdx.x == 0 && x == 0 && !__all_sync(0xffffffffu, mbar_wait(&c->never, 0, limit))) failed = true;
+    if (p.stall && blockIdx.x == 0 && x == 0 && !__all_sync(0xffffffffu, wait_short(&c->never, 0, limit))) failed = true;
     int tok = 0, first_hidden = 0;
     float m = 0.f, sum = 0.f;
     // The softmax of one step over KEYS keys: 128, or 64 where the others are
     // hidden from all of the tile.  False if a wait ran out.
     auto step = [&](auto keys, int j) {
       constexpr int KEYS = decltype(keys)::value;
-      if (!__all_sync(0xffffffffu, mbar_wait(&c->s_full[x], ns++ & 1u, limit))) return false;
+      if (!__all_sync(0xffffffffu, wait_short(&c->s_full[x], ns++ & 1u, limit))) return false;
       tc_fence_after();
       float s[KEYS];
 #pragma unroll
@@ -725,10 +788,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       return true;
     };
-    Walk w;
     Item it;
-    w.begin(c);
-    while (!failed && w.next(c, p, it)) {
+    while (!failed && next_item(it)) {
       const int steps = it.steps[x];
       if (steps == 0) continue;
       tok = min(it.tok[x] + row_tok, it.rows - 1);
