@@ -64,9 +64,10 @@ namespace {
 
 // mbar_wait in fewer instructions.  The roles' code between two items runs once
 // and has left the instruction cache when it is needed again, so short items
-// pay for its length: with mbar_wait at every wait, and with the items walked
-// and the copies written out by each role that needs them, 1000 short requests
-// took 132 us instead of 115, 48 of 5 to 393 tokens 44.8 instead of 42.0.
+// pay for its length: with mbar_wait at every wait, the items walked by every
+// role, and the copies and products written out at each of their places, 1000
+// short requests took 132 us instead of 105, 48 of 5 to 393 tokens 44.8 instead
+// of 41.8.
 __device__ __forceinline__ bool wait_short(uint64_t* bar, uint32_t parity, uint64_t limit_ns) {
   uint64_t t0 = 0;
 #pragma unroll 1
@@ -425,7 +426,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
       const uint32_t q_lo = desc_lo(smem_addr(smem), 16), k_lo = desc_lo(smem_addr(ring), 16),
                      v_lo = desc_lo(smem_addr(ring), 16384);
-      uint32_t fill = 0, nq[2] = {0, 0}, p_phase[2] = {0, 0}, ok_phase = 0, out[2] = {0, 0};
+      // bit x: tile x's phases of its queries and weights, its accumulator
+      uint32_t fill = 0, q_phase = 0, p_phase = 0, out = 0, ok_phase = 0;
       auto wait = [&](uint64_t* bar, uint32_t phase) {
         const bool ok = __all_sync(0xffffffffu, wait_short(bar, phase & 1u, limit));
         failed |= !ok;
@@ -453,11 +455,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       // second half's are still being computed
       auto weigh = [&](int x, int h, uint32_t f, bool first) {
         const uint32_t b = v_lo + (f % STAGES) * (TILE >> 4) + h * (8192 >> 4);
+        const uint32_t d = tm + col_o + D * (G::OUTS * x + (out >> x & 1u));
         if (leader) {
 #pragma unroll
           for (int u = 0; u < 4; ++u)
-            mma_ts(tm + col_o + D * (G::OUTS * x + out[x]), tm + col_s + 128 * x + 32 * h + 8 * u, b + u * (2048 >> 4), HI, idesc_o,
-                   u > 0 || !first);
+            mma_ts(d, tm + col_s + 128 * x + 32 * h + 8 * u, b + u * (2048 >> 4), HI, idesc_o, u > 0 || !first);
         }
       };
       struct Next {
@@ -471,77 +473,79 @@ __global__ void __launch_bounds__(kThreads, 1)
         n.nk = __shfl_sync(0xffffffffu, more ? it.nk : 0, 0);
         n.guard = __shfl_sync(0xffffffffu, more ? it.guard : 0, 0);
       };
-      // tile x's first scores of an item whose first keys are fill f
-      auto begin_tile = [&](const Next& n, int x, uint32_t f) {
-        if (n.steps[x] == 0 || !full(f) || !wait(&c->q_full[x], nq[x]++)) return;
-        tc_fence_after();
-        scores(x, f, n.steps[x] > 1, n.steps[x] <= 2);
-      };
+      // Half the code, with the tiles and halves as loops, is 4 us less for 1000
+      // short requests and 5 to 10% more for long ones: where a tile's operands
+      // lie is then worked out at every product.
       Next cur = {}, nxt;
-      // Whether tile x's first scores of item n can go out without a wait.  The
-      // queries are asked for behind the keys: once they are there, the keys'
-      // barrier is in the phase that is looked at.
-      auto at_hand = [&](const Next& n, int x, uint32_t f) {
-        return n.steps[x] != 0 && __all_sync(0xffffffffu, mbar_test(&c->q_full[x], nq[x] & 1u)) &&
-               __all_sync(0xffffffffu, mbar_test(&c->kv_full[f % STAGES], (f / STAGES) & 1u));
-      };
       do {
         fetch(nxt);
         const uint32_t next_fill = fill + 2 * cur.nk;
-        uint32_t bad = 0;
-        bool begun[2] = {false, false};  // with the next item
-        for (int j = 0; j < cur.nk; ++j) {
+        uint32_t bad = 0, begun = 0;  // bit x: tile x, with the next item
+#pragma unroll 1
+        for (int j = 0; j <= cur.nk && !failed; ++j) {  // the last pass begins what has not begun
           const uint32_t fv = fill + 2 * j + 1, fk = fv + 1;
           const bool more_keys = j + 1 < cur.nk;
-          if (j >= cur.guard) {  // looked at: there, too
-            const uint32_t s = fv % STAGES;
-            if (!wait(&c->v_ok[s], ok_phase >> s)) break;
-            ok_phase ^= 1u << s;
-            bad |= c->slot_bad[s][0] | c->slot_bad[s][1];
-          } else if (!full(fv)) {
-            break;
+          if (j < cur.nk) {
+            if (j >= cur.guard) {  // looked at: there, too
+              const uint32_t s = fv % STAGES;
+              if (!wait(&c->v_ok[s], ok_phase >> s)) break;
+              ok_phase ^= 1u << s;
+              bad |= c->slot_bad[s][0] | c->slot_bad[s][1];
+            } else if (!full(fv)) {
+              break;
+            }
+            if (more_keys && !full(fk)) break;
           }
-          if (more_keys && !full(fk)) break;
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
-            if (2 * j >= cur.steps[x] || failed) continue;
-            const bool two = 2 * j + 1 < cur.steps[x];
-            if (!wait(&c->p_ready[x][0], p_phase[x])) continue;
-            tc_fence_after();
-            weigh(x, 0, fv, j == 0);
-            if (two) {
-              if (!wait(&c->p_ready[x][1], p_phase[x])) continue;
-              tc_fence_after();
-              weigh(x, 1, fv, false);
-            }
-            p_phase[x] ^= 1u;
-            bool go = 2 * j + 2 < cur.steps[x];
-            uint32_t next_k = fk;
+            const int next_steps = nxt.steps[x];
             int left = cur.steps[x] - 2 * j - 2;
-            if (!go) {
-              if (leader) {
-                c->tile_bad[x][out[x]] = bad;
-                mbar_arrive(&c->o_full[x][out[x]]);
-                mma_commit(&c->o_full[x][out[x]]);
-              }
-              if (G::OUTS == 2) out[x] ^= 1u;
-              // the next item's first scores, where the other tile has products to come
-              if ((2 * j + 2 < cur.steps[x ^ 1] || (x == 0 && 2 * j < cur.steps[1])) && at_hand(nxt, x, next_fill)) {
-                ++nq[x];
+            uint32_t keys = fk;
+            if (left > -2) {
+              if (wait(&c->p_ready[x][0], p_phase >> x)) {
                 tc_fence_after();
-                go = begun[x] = true;
-                next_k = next_fill, left = nxt.steps[x];
+                weigh(x, 0, fv, j == 0);
+              }
+              if (left > -1 && !failed && wait(&c->p_ready[x][1], p_phase >> x)) {
+                tc_fence_after();
+                weigh(x, 1, fv, false);
+              }
+              if (failed) break;
+              p_phase ^= 1u << x;
+              if (left <= 0) {
+                const uint32_t o = G::OUTS == 2 ? out >> x & 1u : 0u;
+                if (leader) {
+                  c->tile_bad[x][o] = bad;
+                  mbar_arrive(&c->o_full[x][o]);
+                  mma_commit(&c->o_full[x][o]);
+                }
+                if (G::OUTS == 2) out ^= 1u << x;
               }
             }
-            if (go) scores(x, next_k, left > 1, left <= 2);
+            if (left <= 0) {
+              // The next item's first scores, if they can go out without a wait
+              // or nothing is left to do here.  (The queries are asked for behind
+              // the keys: once they are there, the keys' barrier is in the phase
+              // that is looked at.)
+              if (next_steps == 0 || (begun >> x & 1u)) continue;
+              if (j < cur.nk) {
+                if (!__all_sync(0xffffffffu, mbar_test(&c->q_full[x], q_phase >> x & 1u)) ||
+                    !__all_sync(0xffffffffu, mbar_test(&c->kv_full[next_fill % STAGES], (next_fill / STAGES) & 1u)))
+                  continue;
+              } else if (!wait(&c->q_full[x], q_phase >> x) || !full(next_fill)) {
+                break;
+              }
+              tc_fence_after();
+              q_phase ^= 1u << x;
+              begun |= 1u << x;
+              keys = next_fill, left = next_steps;
+            }
+            scores(x, keys, left > 1, left <= 2);
           }
           if (failed) break;
-          release(fv);
+          if (j < cur.nk) release(fv);
           if (more_keys) release(fk);
         }
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-          if (!failed && !begun[x]) begin_tile(nxt, x, next_fill);
         if (nxt.nk && !failed) release(next_fill);
         fill = next_fill;
         cur = nxt;
