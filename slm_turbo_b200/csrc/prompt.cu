@@ -473,9 +473,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         n.nk = __shfl_sync(0xffffffffu, more ? it.nk : 0, 0);
         n.guard = __shfl_sync(0xffffffffu, more ? it.guard : 0, 0);
       };
-      // Half the code, with the tiles and halves as loops, is 4 us less for 1000
-      // short requests and 5 to 10% more for long ones: where a tile's operands
-      // lie is then worked out at every product.
+      // Half the code, with the tiles and halves as loops, is 2 us less for the
+      // ragged batch above and up to 10% more for long prompts: where a tile's
+      // operands lie is then worked out at every product.
       Next cur = {}, nxt;
       do {
         fetch(nxt);
