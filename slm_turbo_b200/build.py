@@ -68,7 +68,7 @@ def build_host(force: bool = False, verbose: bool = False) -> Path:
            "-isystem", str(root / "include/torch/csrc/api/include"), "-I", sysconfig.get_paths()["include"],
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", str(HOST_SOURCE), "-o", str(tmp),
            "-L", str(HERE), f"-l:{LIB_NAME}", "-Wl,-rpath,$ORIGIN",
-           "-L", str(root / "lib"), "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_python"]
+           "-L", str(root / "lib"), "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python"]
     if verbose:
         print(" ".join(cmd), flush=True)
     subprocess.run(cmd, check=True)
