@@ -27,7 +27,7 @@
 // in a short run and about 2.0 ms, 1100 TFLOP/s, with the clock held at 1.7
 // GHz.  Short ones are bound by their chain: products, softmax, products,
 // output (a prompt of 130 tokens beside three shorter ones: 9.5 us).
-// Measured and dropped, in turn on one box: scores of 64 keys at a time into
+// Measured and dropped, in turn on one GPU: scores of 64 keys at a time into
 // alternating halves (the softmax then never waits, but S costs 768 cycles in
 // place of 512 and its products change accumulators twice as often), one
 // product warp per tile (products into different accumulators interleave), two

@@ -90,6 +90,17 @@ def test_prompt_attention(dev, name, heads, dtype):
     _check(out, *_ref(q, k, v, lens, scale, out_dtype))
 
 
+@pytest.mark.parametrize("lens, heads", [([1999, 777, 63], (32, 32, 80)), ([700] * 6 + [5, 90] * 150, (16, 4, 64)),
+                                         ([2100, 50, 1500, 1], (16, 16, 128))], ids=["d80", "d64", "d128"])
+def test_several_items_of_unequal_length_per_sm(dev, lens, heads):
+    """Hundreds of tile pairs of falling length: every one is done, once."""
+    hq, kv, d = heads
+    q, k, v, start = _inputs(lens, hq, kv, d, torch.bfloat16, dev)
+    out = torch.full(q.shape, float("nan"), dtype=torch.bfloat16, device=dev)
+    kd.kv_prompt_attention(q, k, v, start, max(lens), out=out)
+    _check(out, *_ref(q, k, v, lens, 1 / math.sqrt(d), torch.bfloat16))
+
+
 @pytest.mark.parametrize("hq", [127, 128])
 def test_widest_groups(dev, hq):
     lens = [3, 130, 1]
