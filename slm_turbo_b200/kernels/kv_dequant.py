@@ -530,7 +530,9 @@ def kv_rotary_inv_freq(rotary_dim, base=10000.0, scaling=None, device=None):
       "original_max_position_embeddings" (NTK-aware);
     * "yarn": frequencies that turn more than beta_fast times over the original
       length stay, those below beta_slow are divided by factor, a linear ramp
-      between; cos and sin are scaled by "attention_factor" (0.1 ln factor + 1);
+      between; cos and sin are scaled by "attention_factor", or without it by
+      g(mscale) / g(mscale_all_dim) if both are given, else by g(1), with
+      g(m) = 0.1 m ln factor + 1 for factors above 1 and 1 below;
     * "llama3": as yarn with the ramp between low_freq_factor and
       high_freq_factor turns, linear in the number of turns.
 
@@ -587,7 +589,15 @@ def kv_rotary_inv_freq(rotary_dim, base=10000.0, scaling=None, device=None):
             i = torch.arange(rotary_dim // 2, dtype=torch.float64)
             keep = 1.0 - ((i - first) / (last - first)).clamp(0.0, 1.0)
             given = scaling.get("attention_factor")
-            factor_out = float(given) if given is not None else (0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0)
+            mscale, all_dim = scaling.get("mscale"), scaling.get("mscale_all_dim")
+
+            def g(m):
+                return 0.1 * float(m) * math.log(factor) + 1.0 if factor > 1 else 1.0
+
+            if given is not None:
+                factor_out = float(given)
+            else:  # a zero counts as not given, as in transformers
+                factor_out = g(mscale) / g(all_dim) if mscale and all_dim else g(1.0)
         freq = keep * freq + (1.0 - keep) * freq / factor
     else:
         raise RuntimeError(f"rotary scaling {kind!r} is not one of default/linear/dynamic/yarn/llama3")
