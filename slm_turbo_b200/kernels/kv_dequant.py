@@ -537,13 +537,18 @@ def kv_rotary_inv_freq(rotary_dim, base=10000.0, scaling=None, device=None):
       high_freq_factor turns, linear in the number of turns.
 
     Returns (fp32 [rotary_dim / 2] on ``device``, attention scaling); computed
-    in 64 bits, rounded once.
+    in 64 bits, rounded once.  The entry's numbers have to be positive and
+    finite (low_freq_factor finite), the frequencies finite in fp32, and a
+    "rope_theta" in the entry has to be ``base``; anything else is refused.
     """
     if rotary_dim < 2 or rotary_dim % 2:
         raise RuntimeError(f"rotary_dim must be even and positive, got {rotary_dim}")
-    if not base > 0:
-        raise RuntimeError(f"rotary base must be positive, got {base}")
+    if not (base > 0 and math.isfinite(base)):
+        raise RuntimeError(f"rotary base must be positive and finite, got {base}")
     kind = "default" if scaling is None else scaling.get("rope_type", scaling.get("type", "default"))
+    theta = None if scaling is None else scaling.get("rope_theta")
+    if theta is not None and float(theta) != float(base):
+        raise RuntimeError(f"rotary base {base} is not the entry's rope_theta {theta}")
     exponent = torch.arange(0, rotary_dim, 2, dtype=torch.float64) / rotary_dim
     freq = float(base) ** -exponent
     factor_out = 1.0
@@ -551,7 +556,13 @@ def kv_rotary_inv_freq(rotary_dim, base=10000.0, scaling=None, device=None):
     def need(name):
         if name not in scaling or scaling[name] is None:
             raise RuntimeError(f"rotary scaling {kind!r} needs {name!r}")
-        return float(scaling[name])
+        return positive(name, scaling[name])
+
+    def positive(name, value):
+        value = float(value)
+        if not (value > 0 and math.isfinite(value)):
+            raise RuntimeError(f"rotary scaling {kind!r}: {name!r} must be positive and finite, got {value}")
+        return value
 
     if kind == "default":
         pass
@@ -567,15 +578,17 @@ def kv_rotary_inv_freq(rotary_dim, base=10000.0, scaling=None, device=None):
     elif kind in ("yarn", "llama3"):
         factor, orig = need("factor"), need("original_max_position_embeddings")
         if kind == "llama3":
-            low, high = need("low_freq_factor"), need("high_freq_factor")
-            if not high > low:
+            high, low = need("high_freq_factor"), scaling.get("low_freq_factor")
+            low = math.nan if low is None else float(low)  # may be 0: the ramp then starts there
+            if not (high > low and math.isfinite(low)):
                 raise RuntimeError(f"rotary scaling 'llama3': high_freq_factor {high} must exceed low_freq_factor {low}")
             turns = orig * freq / (2.0 * math.pi)  # over the original length
             keep = ((turns - low) / (high - low)).clamp(0.0, 1.0)
         else:
             if not base > 1:
                 raise RuntimeError(f"rotary scaling 'yarn' needs a base above 1, got {base}")
-            fast, slow = float(scaling.get("beta_fast") or 32.0), float(scaling.get("beta_slow") or 1.0)
+            fast = positive("beta_fast", scaling.get("beta_fast") or 32.0)
+            slow = positive("beta_slow", scaling.get("beta_slow") or 1.0)
 
             def index_of(turns):  # the pair that makes this many turns over the original length
                 return rotary_dim * math.log(orig / (turns * 2.0 * math.pi)) / (2.0 * math.log(base))
@@ -595,13 +608,18 @@ def kv_rotary_inv_freq(rotary_dim, base=10000.0, scaling=None, device=None):
                 return 0.1 * float(m) * math.log(factor) + 1.0 if factor > 1 else 1.0
 
             if given is not None:
-                factor_out = float(given)
-            else:  # a zero counts as not given, as in transformers
-                factor_out = g(mscale) / g(all_dim) if mscale and all_dim else g(1.0)
+                factor_out = positive("attention_factor", given)
+            elif mscale and all_dim:  # a zero counts as not given, as in transformers
+                factor_out = positive("g(mscale)", g(mscale)) / positive("g(mscale_all_dim)", g(all_dim))
+            else:
+                factor_out = g(1.0)
         freq = keep * freq + (1.0 - keep) * freq / factor
     else:
         raise RuntimeError(f"rotary scaling {kind!r} is not one of default/linear/dynamic/yarn/llama3")
-    return freq.to(torch.float32).to(device or "cpu"), factor_out
+    freq = freq.to(torch.float32)
+    if not bool(((freq >= 0) & freq.isfinite()).all()):
+        raise RuntimeError("rotary frequencies are not finite in fp32")
+    return freq.to(device or "cpu"), factor_out
 
 
 def kv_rotary(query, key, positions, inv_freq, interleaved=False, attention_scaling=1.0, query_out=None,
