@@ -164,7 +164,8 @@ __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
 // One row of k (turned) and v into its slot: the lanes of the row are
 // neighbours in the warp, and the whole warp takes part in the exchange.  The
 // rows hold 16-bit values, so their extremes are found on packed ones: k's in
-// the lower half of a word, v's in the upper.
+// the lower half of a word, v's in the upper.  They start from the infinities
+// as the store kernel's do: a row of NaN has a minimum of +infinity.
 template <int D, int LAYOUT, bool BF16>
 __device__ __forceinline__ void quantize8(const uint4& kw, const uint4& vw, uint8_t* row, bool act, bool write, int li,
                                           int d0, int d1) {
@@ -175,7 +176,7 @@ __device__ __forceinline__ void quantize8(const uint4& kw, const uint4& vw, uint
   const uint32_t v_hi = max2<BF16>(max2<BF16>(vw.x, vw.y), max2<BF16>(vw.z, vw.w));
   uint32_t lo = min2<BF16>(__byte_perm(k_lo, v_lo, 0x5410), __byte_perm(k_lo, v_lo, 0x7632));
   uint32_t hi = max2<BF16>(__byte_perm(k_hi, v_hi, 0x5410), __byte_perm(k_hi, v_hi, 0x7632));
-  if (!act) lo = INF, hi = NEG_INF;
+  lo = act ? min2<BF16>(lo, INF) : INF, hi = act ? max2<BF16>(hi, NEG_INF) : NEG_INF;
 #pragma unroll
   for (int o = RotGeom<D>::LANES / 2; o > 0; o >>= 1) {
     lo = min2<BF16>(lo, __shfl_xor_sync(0xffffffffu, lo, o));
