@@ -404,7 +404,7 @@ int slmt_page_plan(const int32_t* query_start_loc, const int32_t* seq_lens,
  * (dims i and i + rotary_dim/2, or 2i and 2i+1 when interleaved) turns by
  * theta = position * inv_freq[i], scaled by `scaling`:
  *     y1 = x1 c - x2 s, y2 = x2 c + x1 s, c = scaling cos, s = scaling sin;
- * the other dims are copied.  theta is taken in 64 bits, c and s rounded to
+ * the other dims are copied (a NaN stays one, its bits may change).  theta is taken in 64 bits, c and s rounded to
  * fp32, each product and sum rounded in fp32, the result once to the row
  * type.  q [num_tokens, num_q_heads, head_dim], k [num_tokens, num_kv_heads,
  * head_dim], fp16 or bf16 (dtype), either with 0 heads; positions int32 or

@@ -630,7 +630,7 @@ def kv_rotary(query, key, positions, inv_freq, interleaved=False, attention_scal
     (2i, 2i + 1) with ``interleaved`` -- of row n turns by positions[n] *
     inv_freq[i] (int32/int64 and fp32, on the device; the angle is taken in 64
     bits), its cos and sin times ``attention_scaling``; the other dims are
-    copied.  Negative positions turn back.  Returns (query, key) rotated: new
+    copied (a NaN stays one, its bits may change).  Negative positions turn back.  Returns (query, key) rotated: new
     tensors, or ``query_out`` / ``key_out``, which may be the inputs themselves.
     """
     return _lib.host().rotary(query, key, positions, inv_freq, interleaved, attention_scaling, query_out, key_out)
