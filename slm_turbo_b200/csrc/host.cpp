@@ -77,11 +77,17 @@ void same_device(const char* what, int index, std::initializer_list<const Tensor
       refuse(what, ": tensors on ", t->device(), " and cuda:", index);
 }
 
+// Neither direction of autograd passes: gradients that would be lost while it
+// records, and tangents of dual tensors, which no_grad does not switch off.
 void no_autograd(const char* what, std::initializer_list<const Tensor*> tensors) {
-  if (!at::GradMode::is_enabled()) return;
-  for (const Tensor* t : tensors)
-    if (t && t->requires_grad())
+  const bool records = at::GradMode::is_enabled();
+  for (const Tensor* t : tensors) {
+    if (!t) continue;
+    if (records && t->requires_grad())
       refuse(what, ": has no backward pass; call it under torch.no_grad() or on detached tensors");
+    if (t->_fw_grad(0).defined())
+      refuse(what, ": has no forward-mode or backward pass; call it on the primal of the dual tensor");
+  }
 }
 
 const Tensor* get(const Opt& t) { return t ? &*t : nullptr; }

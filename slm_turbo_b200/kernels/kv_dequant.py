@@ -25,7 +25,7 @@ and positions from request lengths), ``kv_rotary`` / ``kv_rotary_store``
 ``kv_rotary_inv_freq``), ``kv_prompt_attention`` (causal attention of packed
 prompts over their own K/V) and ``kv_dequantize_load`` (tokens read back).
 These are for serving: they have no backward pass and refuse inputs that
-require a gradient while autograd records.
+require a gradient while autograd records, and dual tensors.
 """
 from __future__ import annotations
 
