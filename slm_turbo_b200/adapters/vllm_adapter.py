@@ -205,12 +205,19 @@ def _register_custom_backend() -> bool:
             raise RuntimeError(f"slm-turbo 4-bit KV kernels unavailable in this process: "
                                f"{self._slm_kernel_err}")
 
-        def _prompt_kernel_takes(self, query, key):
-            """Whether fresh prompts go to kv_prompt_attention (the packed cache
-            takes the same types); anything else is left to SDPA."""
+        def _prompt_kernel_takes(self, query, key, value, out):
+            """Whether fresh prompts go to kv_prompt_attention: its types, head
+            sizes, groups and scales, output rows on 16 bytes, nothing that
+            autograd records.  Any other step is left to SDPA."""
+            unit = 16 // out.element_size()
             return (self._slm_kernel and query.is_cuda and query.dtype in (torch.float16, torch.bfloat16)
-                    and key.dtype == query.dtype and self.scale > 0 and query.shape[1] <= 128 * key.shape[1]
-                    and not (torch.is_grad_enabled() and query.requires_grad))
+                    and key.dtype == value.dtype == query.dtype
+                    and out.dtype in (torch.float16, torch.bfloat16, torch.float32)
+                    and query.shape[2] in SUPPORTED_HEAD_SIZES and key.shape == value.shape
+                    and query.shape[1] <= 128 * key.shape[1] and 1e-30 < self.scale < 1e30
+                    and out.data_ptr() % 16 == 0 and out.stride(2) == 1
+                    and out.stride(0) % unit == 0 and out.stride(1) % unit == 0
+                    and not (torch.is_grad_enabled() and any(t.requires_grad for t in (query, key, value, out))))
 
         def do_kv_cache_update(self, layer, key, value, kv_cache, slot_mapping):
             """Quantize the batch's K/V into their packed slots (ref :185-203)."""
@@ -271,7 +278,7 @@ def _register_custom_backend() -> bool:
                     longest = max(longest, b - a)
                 else:
                     longest_fresh = max(longest_fresh, b - a)
-            own = longest_fresh > 0 and self._prompt_kernel_takes(query, key)
+            own = longest_fresh > 0 and self._prompt_kernel_takes(query, key, value, out)
             if longest or own:
                 meta = torch.tensor(qsl + kernel_lens + fresh_lens, dtype=torch.int32).to(query.device,
                                                                                           non_blocking=True)
@@ -320,7 +327,7 @@ def _register_custom_backend() -> bool:
                 query, kv_cache, bt, vlen, block_size=kv_cache.shape[1], num_kv_heads=kv_cache.shape[2],
                 out=out, sm_scale=self.scale, max_seq_len=None)
             _KERNEL_CALLS += 1
-            if self._prompt_kernel_takes(query, key):
+            if self._prompt_kernel_takes(query, key, value, out):
                 from slm_turbo_b200.kernels.kv_dequant import kv_prompt_attention
                 rows = qsl[1:] - qsl[:-1]
                 own_lens = torch.where(ctx <= 0, rows, torch.full_like(rows, -1))
