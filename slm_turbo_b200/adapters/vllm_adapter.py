@@ -329,10 +329,10 @@ def _register_custom_backend() -> bool:
             _KERNEL_CALLS += 1
             if self._prompt_kernel_takes(query, key, value, out):
                 from slm_turbo_b200.kernels.kv_dequant import kv_prompt_attention
-                rows = qsl[1:] - qsl[:-1]
+                starts = qsl.clamp(max=n)  # a request may be cut behind the step's tokens
+                rows = starts[1:] - starts[:-1]
                 own_lens = torch.where(ctx <= 0, rows, torch.full_like(rows, -1))
-                kv_prompt_attention(query, key, value, qsl.clamp(max=n), n, seq_lens=own_lens, out=out,
-                                    sm_scale=self.scale)
+                kv_prompt_attention(query, key, value, starts, n, seq_lens=own_lens, out=out, sm_scale=self.scale)
                 _KERNEL_CALLS += 1
                 return out
             raw = self._first_chunk_attention(query, key, value, req)
