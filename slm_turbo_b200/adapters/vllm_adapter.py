@@ -173,6 +173,8 @@ def _register_custom_backend() -> bool:
     class _Impl(TritonAttentionImpl):
         """Quantize-on-write store + one batched paged decode launch per layer."""
 
+        _slm_prompt_kernel = True  # whether the host module of kv_prompt_attention loads
+
         def __init__(self, *args, **kwargs):
             super().__init__(*args, **kwargs)
             self._slm_kernel = False
@@ -199,6 +201,13 @@ def _register_custom_backend() -> bool:
                 self._slm_decode_batched = self._kernel_unavailable
                 self._slm_prefill = self._kernel_unavailable
                 self._slm_store = self._kernel_unavailable
+            else:
+                try:  # built for one torch and Python, unlike the library
+                    from slm_turbo_b200 import _lib
+                    _lib.host()
+                except ImportError as e:
+                    self._slm_prompt_kernel = False
+                    logger.warning("slm-turbo prompt kernel disabled in this process, fresh prompts go to SDPA: %s", e)
 
         def _kernel_unavailable(self, *args, **kwargs):
             # the cache is packed 4-bit: nothing else can write or read it
@@ -210,7 +219,8 @@ def _register_custom_backend() -> bool:
             sizes, groups and scales, output rows on 16 bytes, nothing that
             autograd records.  Any other step is left to SDPA."""
             unit = 16 // out.element_size()
-            return (self._slm_kernel and query.is_cuda and query.dtype in (torch.float16, torch.bfloat16)
+            return (self._slm_kernel and self._slm_prompt_kernel and query.is_cuda
+                    and query.dtype in (torch.float16, torch.bfloat16)
                     and key.dtype == value.dtype == query.dtype
                     and out.dtype in (torch.float16, torch.bfloat16, torch.float32)
                     and query.shape[2] in SUPPORTED_HEAD_SIZES and key.shape == value.shape
