@@ -5,13 +5,17 @@ a C++ file on top of the library and torch's headers) with g++.
     python -m slm_turbo_b200.build          # or build_library() from Python
 
 Both are written next to this file so that they travel with the source tree;
-there is no JIT cache.  Flags of the library: sm_100a
+there is no JIT cache.  The library needs nvcc alone; the module, torch (with
+its headers) and a C++ compiler ($CXX or g++): where they are missing the
+library is built all the same.  Flags of the library: sm_100a
 only, -O3, -lineinfo, IEEE division/rounding (no --use_fast_math: the
 quantizers must match the reference bit for bit).
 """
 from __future__ import annotations
 
+import importlib.util
 import os
+import shutil
 import subprocess
 import sys
 import sysconfig
@@ -55,19 +59,47 @@ def _stale() -> bool:
     return any(d.stat().st_mtime > t for d in deps)
 
 
-def build_host(force: bool = False, verbose: bool = False) -> Path:
-    """Compile the Python module on top of the library (skips if up to date)."""
+def _torch_root():
+    """Where torch is installed (not imported), None if it is not."""
+    spec = importlib.util.find_spec("torch")
+    return Path(spec.origin).resolve().parent if spec and spec.origin else None
+
+
+def _host_tools():
+    """What _host.so is built with: (paths by name, None), or (None, what is missing)."""
+    root, toolkit = _torch_root(), shutil.which(nvcc())
+    cxx = os.environ.get("CXX") or "g++"
+    paths = {"torch": root, "cxx": shutil.which(cxx), "python": Path(sysconfig.get_paths()["include"]),
+             "cuda": Path(toolkit).resolve().parent.parent / "include" if toolkit else None}
+    missing = ("torch" if root is None else
+               "torch's CUDA headers and libraries" if not ((root / "include/ATen/cuda/EmptyTensor.h").exists()
+                                                            and (root / "lib/libc10_cuda.so").exists()) else
+               f"the C++ compiler {cxx}" if paths["cxx"] is None else
+               "Python.h" if not (paths["python"] / "Python.h").exists() else
+               "the CUDA headers" if not (toolkit and (paths["cuda"] / "cuda_runtime_api.h").exists()) else None)
+    return (None, missing) if missing else (paths, None)
+
+
+def build_host(force: bool = False, verbose: bool = False):
+    """Compile the Python module on top of the library (skips if up to date).
+    Where torch or a C++ toolchain is missing it says so and returns None: the
+    library does not need them."""
+    tools, missing = _host_tools()
+    if missing:
+        print(f"_host.so is not built: {missing} not found (the C library does not need it; the serving-step "
+              "functions in Python do)", file=sys.stderr)
+        return None
     deps = [HOST_SOURCE, INCLUDE / "slm_turbo_b200.h"]
     if not force and HOST_PATH.exists() and all(d.stat().st_mtime <= HOST_PATH.stat().st_mtime for d in deps):
         return HOST_PATH
     import torch
-    root = Path(torch.__file__).resolve().parent
+    root = tools["torch"]
     tmp = HOST_PATH.with_suffix(".so.tmp")
-    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-I", str(INCLUDE),
-           "-I", "/usr/local/cuda/include", "-isystem", str(root / "include"),
-           "-isystem", str(root / "include/torch/csrc/api/include"), "-I", sysconfig.get_paths()["include"],
+    cmd = [tools["cxx"], "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-I", str(INCLUDE),
+           "-I", str(tools["cuda"]), "-isystem", str(root / "include"),
+           "-isystem", str(root / "include/torch/csrc/api/include"), "-I", str(tools["python"]),
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", str(HOST_SOURCE), "-o", str(tmp),
-           "-L", str(HERE), f"-l:{LIB_NAME}", "-Wl,-rpath,$ORIGIN",
+           "-L", str(LIB_PATH.parent), f"-l:{LIB_NAME}", "-Wl,-rpath,$ORIGIN",
            "-L", str(root / "lib"), "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python"]
     if verbose:
         print(" ".join(cmd), flush=True)

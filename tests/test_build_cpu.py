@@ -1,0 +1,57 @@
+"""CPU: what the build of the Python module next to the library depends on.
+Nothing is compiled: the compiler's command is recorded."""
+import subprocess
+from pathlib import Path
+
+import pytest
+
+from slm_turbo_b200 import build
+
+
+@pytest.fixture
+def tree(monkeypatch, tmp_path):
+    """An up-to-date library, and a module in a folder of its own; the commands
+    that a build runs."""
+    monkeypatch.setattr(build, "_stale", lambda: False)
+    monkeypatch.setattr(build, "HOST_PATH", tmp_path / "_host.so")
+    runs = []
+
+    def run(cmd, **kw):
+        runs.append(cmd)
+        Path(cmd[cmd.index("-o") + 1]).write_bytes(b"module")
+        return subprocess.CompletedProcess(cmd, 0)
+
+    monkeypatch.setattr(build.subprocess, "run", run)
+    return tmp_path, runs
+
+
+def test_the_library_does_not_need_torch_or_a_cxx_compiler(tree, monkeypatch, capsys):
+    tmp, runs = tree
+    with monkeypatch.context() as m:
+        m.setattr(build, "_torch_root", lambda: None)
+        assert build.build_library() == build.LIB_PATH
+    assert "torch" in capsys.readouterr().err
+    with monkeypatch.context() as m:
+        m.setattr(build, "_torch_root", lambda: tmp)  # a torch without CUDA
+        assert build.build_library() == build.LIB_PATH
+    assert "headers" in capsys.readouterr().err
+    with monkeypatch.context() as m:
+        m.setenv("CXX", str(tmp / "no-compiler"))
+        assert build.build_library() == build.LIB_PATH
+    assert "no-compiler" in capsys.readouterr().err
+    assert not runs and not build.HOST_PATH.exists()
+
+
+def test_compiler_and_toolkit_come_from_the_environment(tree, monkeypatch):
+    tmp, runs = tree
+    if build._host_tools()[1]:
+        pytest.skip("no torch or C++ toolchain here")
+    for d, f in (("toolkit/bin", "nvcc"), ("toolkit/include", "cuda_runtime_api.h"), ("cxx", "c++17")):
+        (tmp / d).mkdir(parents=True)
+        (tmp / d / f).write_text("")
+        (tmp / d / f).chmod(0o755)
+    monkeypatch.setenv("NVCC", str(tmp / "toolkit/bin/nvcc"))
+    monkeypatch.setenv("CXX", str(tmp / "cxx/c++17"))
+    build.build_library()
+    assert runs[0][0] == str(tmp / "cxx/c++17") and str(tmp / "toolkit/include") in runs[0]
+    assert "/usr/local/cuda/include" not in runs[0]
