@@ -13,6 +13,7 @@ quantizers must match the reference bit for bit).
 """
 from __future__ import annotations
 
+import importlib.metadata
 import importlib.util
 import os
 import shutil
@@ -30,6 +31,7 @@ LIB_NAME = "libslm_turbo_b200.so"
 LIB_PATH = HERE / LIB_NAME
 HOST_PATH = HERE / "_host.so"
 HOST_SOURCE = CSRC / "host.cpp"
+HOST_STAMP = HERE / "_build" / "host.stamp"  # what _host.so was built for
 SOURCES = ["decode.cu", "store.cu", "decode_noalloc.cu",
            "decode_d64_paged.cu", "decode_d64_contig.cu", "decode_d80_paged.cu", "decode_d80_contig.cu",
            "decode_d128_paged.cu", "decode_d128_contig.cu", "prefill.cu",
@@ -80,17 +82,28 @@ def _host_tools():
     return (None, missing) if missing else (paths, None)
 
 
+def _host_built_for() -> str:
+    """The torch and the Python that a module built now belongs to."""
+    try:
+        torch_version = importlib.metadata.version("torch")
+    except importlib.metadata.PackageNotFoundError:
+        torch_version = "unknown"
+    return f"torch {torch_version}, {sysconfig.get_config_var('SOABI')}\n"
+
+
 def build_host(force: bool = False, verbose: bool = False):
-    """Compile the Python module on top of the library (skips if up to date).
-    Where torch or a C++ toolchain is missing it says so and returns None: the
-    library does not need them."""
+    """Compile the Python module on top of the library (skips if it is up to
+    date, and built for this torch and Python).  Where torch or a C++ toolchain
+    is missing it says so and returns None: the library does not need them."""
     tools, missing = _host_tools()
     if missing:
         print(f"_host.so is not built: {missing} not found (the C library does not need it; the serving-step "
               "functions in Python do)", file=sys.stderr)
         return None
+    built_for = _host_built_for()
     deps = [HOST_SOURCE, INCLUDE / "slm_turbo_b200.h"]
-    if not force and HOST_PATH.exists() and all(d.stat().st_mtime <= HOST_PATH.stat().st_mtime for d in deps):
+    if (not force and HOST_PATH.exists() and all(d.stat().st_mtime <= HOST_PATH.stat().st_mtime for d in deps)
+            and HOST_STAMP.exists() and HOST_STAMP.read_text() == built_for):
         return HOST_PATH
     import torch
     root = tools["torch"]
@@ -105,6 +118,8 @@ def build_host(force: bool = False, verbose: bool = False):
         print(" ".join(cmd), flush=True)
     subprocess.run(cmd, check=True)
     os.replace(tmp, HOST_PATH)
+    HOST_STAMP.parent.mkdir(exist_ok=True)
+    HOST_STAMP.write_text(built_for)
     return HOST_PATH
 
 

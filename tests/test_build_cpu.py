@@ -10,10 +10,11 @@ from slm_turbo_b200 import build
 
 @pytest.fixture
 def tree(monkeypatch, tmp_path):
-    """An up-to-date library, and a module in a folder of its own; the commands
-    that a build runs."""
+    """An up-to-date library, a module and its stamp in a folder of their own;
+    the commands that a build runs."""
     monkeypatch.setattr(build, "_stale", lambda: False)
     monkeypatch.setattr(build, "HOST_PATH", tmp_path / "_host.so")
+    monkeypatch.setattr(build, "HOST_STAMP", tmp_path / "_build" / "host.stamp")
     runs = []
 
     def run(cmd, **kw):
@@ -40,6 +41,27 @@ def test_the_library_does_not_need_torch_or_a_cxx_compiler(tree, monkeypatch, ca
         assert build.build_library() == build.LIB_PATH
     assert "no-compiler" in capsys.readouterr().err
     assert not runs and not build.HOST_PATH.exists()
+
+
+def test_the_module_is_rebuilt_for_another_torch_or_python(tree, monkeypatch):
+    _, runs = tree
+    if build._host_tools()[1]:
+        pytest.skip("no torch or C++ toolchain here")
+    build.build_library()
+    assert len(runs) == 1 and build.HOST_PATH.exists()
+    build.build_library()
+    assert len(runs) == 1  # up to date
+    with monkeypatch.context() as m:
+        m.setattr(build.importlib.metadata, "version", lambda name: "9.9.9")
+        build.build_library()
+        assert len(runs) == 2
+        build.build_library()
+        assert len(runs) == 2
+    build.build_library()
+    assert len(runs) == 3
+    build.HOST_STAMP.unlink()  # of unknown origin
+    build.build_library()
+    assert len(runs) == 4
 
 
 def test_compiler_and_toolkit_come_from_the_environment(tree, monkeypatch):
