@@ -6,8 +6,7 @@ a C++ file on top of the library and torch's headers) with g++.
 
 Both are written next to this file so that they travel with the source tree;
 there is no JIT cache.  The library needs nvcc alone; the module, torch (with
-its headers) and a C++ compiler ($CXX or g++): where they are missing the
-library is built all the same.  Flags of the library: sm_100a
+its headers) and g++: where they are missing the library is built all the same.  Flags of the library: sm_100a
 only, -O3, -lineinfo, IEEE division/rounding (no --use_fast_math: the
 quantizers must match the reference bit for bit).
 """
@@ -70,13 +69,15 @@ def _torch_root():
 def _host_tools():
     """What _host.so is built with: (paths by name, None), or (None, what is missing)."""
     root, toolkit = _torch_root(), shutil.which(nvcc())
-    cxx = os.environ.get("CXX") or "g++"
-    paths = {"torch": root, "cxx": shutil.which(cxx), "python": Path(sysconfig.get_paths()["include"]),
+    # the system's g++ and not $CXX: the module throws and formats through the
+    # libstdc++ that torch has loaded, and a compiler that links its own copy
+    # in makes one that crashes
+    paths = {"torch": root, "cxx": shutil.which("g++"), "python": Path(sysconfig.get_paths()["include"]),
              "cuda": Path(toolkit).resolve().parent.parent / "include" if toolkit else None}
     missing = ("torch" if root is None else
                "torch's CUDA headers and libraries" if not ((root / "include/ATen/cuda/EmptyTensor.h").exists()
                                                             and (root / "lib/libc10_cuda.so").exists()) else
-               f"the C++ compiler {cxx}" if paths["cxx"] is None else
+               "g++" if paths["cxx"] is None else
                "Python.h" if not (paths["python"] / "Python.h").exists() else
                "the CUDA headers" if not (toolkit and (paths["cuda"] / "cuda_runtime_api.h").exists()) else None)
     return (None, missing) if missing else (paths, None)
