@@ -382,8 +382,9 @@ int slmt_paged_decode_noalloc(const void* q, int q_dtype, int64_t q_seq_stride,
  * complete already.  slot_mapping / positions: int64 [num_tokens]; row t of
  * request r gets block_tables[r][pos / block_size] * block_size + pos %
  * block_size and pos.  Rows of no request (padding) get slot -1 and position
- * 0.  *cursor_out (optional, not free_cursor itself) becomes the next free
- * index.  Only entries of new pages are written to block_tables.
+ * 0; the two outputs must not overlap (SLMT_ERR_SHAPE).  *cursor_out (optional,
+ * not free_cursor itself) becomes the next free index.  Only entries of new
+ * pages are written to block_tables.
  * A free list that is too short gives -1 entries and slots and sets
  * SLMT_DEVERR_FREE_BLOCKS (cursor_out: num_free); a negative table or
  * free-list entry gives slot -1 and SLMT_DEVERR_BLOCK_ID; lengths beyond the
@@ -404,8 +405,8 @@ int slmt_page_plan(const int32_t* query_start_loc, const int32_t* seq_lens,
  * (dims i and i + rotary_dim/2, or 2i and 2i+1 when interleaved) turns by
  * theta = position * inv_freq[i], scaled by `scaling`:
  *     y1 = x1 c - x2 s, y2 = x2 c + x1 s, c = scaling cos, s = scaling sin;
- * the other dims are copied (a NaN stays one, its bits may change).  theta is taken in 64 bits, c and s rounded to
- * fp32, each product and sum rounded in fp32, the result once to the row
+ * the other dims are copied (a NaN stays one, its bits may change).  theta is
+ * taken in 64 bits, c and s rounded to fp32, each product and sum rounded in fp32, the result once to the row
  * type.  q [num_tokens, num_q_heads, head_dim], k [num_tokens, num_kv_heads,
  * head_dim], fp16 or bf16 (dtype), either with 0 heads; positions int32 or
  * int64 [num_tokens] (negative ones turn back); inv_freq fp32 [rotary_dim/2],
@@ -447,7 +448,8 @@ int slmt_rotary_store(const void* q, int64_t q_token_stride,
  * Tokens read back out of the paged cache: key / value [num_tokens,
  * num_kv_heads, head_dim] contiguous, 16-byte aligned, in out_dtype
  * (f32/f16/bf16) get code * step + min of slot_mapping[t]'s rows (one fp32
- * rounding, then one to out_dtype).  A negative slot gives a row of zeros,
+ * rounding, then one to out_dtype).  key, value and kv_cache must not overlap
+ * (SLMT_ERR_SHAPE).  A negative slot gives a row of zeros,
  * one beyond the cache too and sets SLMT_DEVERR_SLOT.
  */
 int slmt_kv_dequantize_load(const uint8_t* kv_cache, int64_t num_blocks,

@@ -19,6 +19,12 @@ inline bool rows_overlap(int64_t tokens, int64_t heads, int64_t token_stride, in
   return (tokens > 1 && token_stride == 0) || (heads > 1 && head_stride == 0);
 }
 
+// Whether two buffers share memory.
+inline bool ranges_overlap(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return x < y + (uintptr_t)b_bytes && y < x + (uintptr_t)a_bytes;
+}
+
 // Status of the launch just issued (clears the sticky-free launch error).
 inline int launch_status() {
   const cudaError_t e = cudaGetLastError();

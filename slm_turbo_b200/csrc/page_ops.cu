@@ -367,6 +367,7 @@ extern "C" int slmt_page_plan(const int32_t* query_start_loc, const int32_t* seq
     return SLMT_ERR_NULL;
   if (num_tokens > 0 && (!slot_mapping || !positions)) return SLMT_ERR_NULL;
   if (cursor_out && cursor_out == free_cursor) return SLMT_ERR_SHAPE;  // every CTA reads one, CTA 0 writes the other
+  if (ranges_overlap(slot_mapping, 8 * num_tokens, positions, 8 * num_tokens)) return SLMT_ERR_SHAPE;
   if (num_tokens == 0 && !cursor_out) return SLMT_OK;
   PlanParams p;
   p.qsl = query_start_loc;
@@ -406,6 +407,11 @@ extern "C" int slmt_kv_dequantize_load(const uint8_t* kv_cache, int64_t num_bloc
       reinterpret_cast<uintptr_t>(value) % 16 != 0)
     return SLMT_ERR_ALIGN;
   const int64_t slots = num_blocks * block_size;
+  const int64_t out_bytes = num_tokens * num_kv_heads * head_dim * (out_dtype == SLMT_DTYPE_F32 ? 4 : 2);
+  const int64_t cache_bytes = slots * num_kv_heads * (head_dim + 8);
+  if (ranges_overlap(key, out_bytes, value, out_bytes) || ranges_overlap(key, out_bytes, kv_cache, cache_bytes) ||
+      ranges_overlap(value, out_bytes, kv_cache, cache_bytes))
+    return SLMT_ERR_SHAPE;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const int kv = (int)num_kv_heads;
   switch (head_dim) {

@@ -512,7 +512,7 @@ def kv_page_plan(query_start_loc, seq_lens, block_tables, block_size, num_tokens
     ``kv_rotary_store``, positions int64 [num_tokens] for ``kv_rotary``, and
     the next free index, int32 [1]); rows behind the last request get slot -1
     and position 0.  ``slot_mapping`` / ``positions`` may be given to be
-    written in place.  A free list that is too short, entries below 0 and
+    written in place (two tensors that share no memory).  A free list that is too short, entries below 0 and
     lengths beyond the table give slot -1 and set a device error bit.
     """
     return _lib.host().page_plan(query_start_loc, seq_lens, block_tables, block_size, num_tokens, free_blocks,
@@ -657,7 +657,7 @@ def kv_dequantize_load(kv_cache, slot_mapping, dtype=torch.float16, key_out=None
     ``dtype`` (fp16/bf16/fp32), code * step + min of the rows at slot_mapping
     [N] (int64).  Negative slots give zeros; slots beyond the cache too, and
     set a device error bit.  ``key_out`` / ``value_out``: contiguous tensors to
-    write instead of new ones.
+    write instead of new ones, which share no memory with each other or the cache.
     """
     return _lib.host().dequantize_load(kv_cache, slot_mapping, dtype, key_out, value_out)
 

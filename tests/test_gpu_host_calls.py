@@ -55,3 +55,22 @@ def test_memory_that_runs_out_is_an_out_of_memory_error(dev):
         kd.kv_dequantize_load(cache, slots, torch.float32)
     k, _ = kd.kv_dequantize_load(cache, slots[:3])
     assert k.shape == (3, 64, 128)
+
+
+def test_outputs_that_share_memory_are_refused(dev):
+    """And buffers next to one another are not."""
+    *_, cache, slots, start = _args(dev)
+    both = torch.zeros(8, 2, 64, device=dev)
+    for a, b in ((both[:4], both[:4]), (both[:4], both[3:7])):
+        with pytest.raises(RuntimeError):
+            kd.kv_dequantize_load(cache, slots, torch.float32, key_out=a, value_out=b)
+    kd.kv_dequantize_load(cache, slots, torch.float32, key_out=both[:4], value_out=both[4:])
+    bt = torch.tensor([[1]], dtype=torch.int32, device=dev)
+    lens = torch.tensor([4], dtype=torch.int32, device=dev)
+    ids = torch.zeros(8, dtype=torch.int64, device=dev)
+    for a, b in ((ids[:4], ids[:4]), (ids[3:7], ids[:4])):
+        with pytest.raises(RuntimeError):
+            kd.kv_page_plan(start, lens, bt, 16, 4, slot_mapping=a, positions=b)
+    kd.kv_page_plan(start, lens, bt, 16, 4, slot_mapping=ids[:4], positions=ids[4:])
+    assert ids.tolist() == [16, 17, 18, 19, 0, 1, 2, 3]
+    assert kd.kv_page_plan(start[:1], lens[:0], bt[:0], 16, 0, slot_mapping=ids[:0], positions=ids[:0])[2].item() == 0
