@@ -43,6 +43,11 @@
 // 5 to 393 tokens, 32/4 heads: 42 us; with one accumulator and the tiles
 // starting together 3.4 more).
 //
+// P is held in the inputs' 16 bits because the tensor core takes both operands
+// of a product in one type; each weight is off by half a step of it (bf16 2^-8,
+// fp16 2^-11, relative), the output's error as a norm goes from 0.0016 to
+// 0.0022 (bf16) and from 0.0002 to 0.00025 (fp16).
+//
 // Running maximum: the reference m of a row moves only when a score passes it
 // by more than 2^8 in weight; until then old weights stay on their scale, and
 // O is rescaled in TMEM only then.  Sums are fp32, of the unrounded weights.
